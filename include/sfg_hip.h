@@ -354,6 +354,117 @@ int sfg_hip_kv_gather_paged_v1(const uint16_t* k_pool, const uint16_t* v_pool,
                                int64_t pages_per_seq, int64_t num_pages, float* keys, float* values,
                                void* stream);
 
+/* ---------------- what a paged cache keeps and reads ----------------
+ * No counterparts in the reference: its caches grow at the end and are read
+ * whole.  These work on the same pools and tables (any head_dim up to 256, any
+ * page size, fp32 or bf16).  Common to all:
+ *   - seq_lens[b] (device) is clamped to [0, max_context]; NULL: every sequence
+ *     holds max_context tokens;
+ *   - a page id outside [0, num_pages) is never followed: its tokens are not seen,
+ *     scored or moved;
+ *   - what no row sees may hold anything (NaN and infinities included) and does
+ *     not reach the result; a row that sees nothing comes out NaN (0 / 0);
+ *   - no call allocates, copies to the host or records anything but kernels, so
+ *     all of them can be captured into a graph.  Calls that overlap need
+ *     workspaces of their own (captured graphs too). */
+
+/* Arguments shared by the three attentions: q and out head-major
+ * [B][Hq][rows][D] in q_dtype and out_dtype (SFG_F32 or SFG_BF16), group
+ * Hq / Hkv of any size.  kv_splits <= 0 picks a split count, scale <= 0 means
+ * 1 / sqrt(D).  bf16 queries with a bf16 output run with probabilities rounded to
+ * bf16 once before the value product; every other combination keeps queries and
+ * probabilities at fp32 precision. */
+typedef struct {
+    const void* q; int32_t q_dtype;
+    const void* k_pool; const void* v_pool; int32_t kv_dtype;
+    const int32_t* page_table;   /* [B][pages_per_seq] */
+    const int32_t* seq_lens;     /* [B] or NULL */
+    void* out; int32_t out_dtype;
+    int64_t batch, q_heads, kv_heads, rows, head_dim;
+    int64_t page_tokens, pages_per_seq, num_pages;
+    int64_t max_context;
+    int32_t kv_splits;
+    float scale;
+} sfg_paged_attn_args;
+
+/* Attention of a tree of drafted tokens: sequence b holds seq_lens[b] committed
+ * tokens (at most max_context) and behind them, at positions seq_lens[b] + u, the
+ * keys and values of `rows` drafted tokens (sfg_hip_kv_append_pool_v1 with
+ * advance 0 puts them there).  Row t sees every committed token, and draft u iff
+ * bit u & 31 of word u >> 5 of tree_mask[b * mask_stride + t * W], W =
+ * ceil(rows / 32), is set: for a tree, u is t or one of its ancestors.  The mask is
+ * taken as it is (a row does not see itself unless its bit says so).  mask_stride
+ * 0: one mask for all sequences, else at least rows * W words.  The tables must
+ * cover max_context + rows tokens. */
+size_t sfg_hip_attn_tree_workspace_v1(const sfg_paged_attn_args* args);
+int sfg_hip_attn_tree_v1(const sfg_paged_attn_args* args, const uint32_t* tree_mask,
+                         int64_t mask_stride, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/* Causal attention of the newest `rows` tokens (row i sees token j iff
+ * j <= L_b - rows + i, as sfg_hip_attn_paged_v1) that also adds to
+ * weights[b][g][j], fp32 [B][Hkv][weights_ld], the softmax weight that token j
+ * drew, summed over the rows and the query heads of kv head g.  weights_ld >=
+ * max_context; entries from L_b on are not touched.  The same call gives the same
+ * bits (no atomics).  The workspace holds the scores, 4 bytes per query column
+ * and token. */
+size_t sfg_hip_attn_weights_workspace_v1(const sfg_paged_attn_args* args);
+int sfg_hip_attn_weights_v1(const sfg_paged_attn_args* args, float* weights, int64_t weights_ld,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* Which tokens a cache keeps: of the L_b tokens of a sequence, for each kv head,
+ * the newest `recent` and of the others the budget - recent of the largest
+ * weight, ties to the lower position, NaN below every number; all of them if
+ * L_b <= budget.  keep [B][Hkv][budget] receives their positions ascending (-1
+ * behind), kept_lens[b] = min(L_b, budget), and kept_weights (NULL, weights
+ * itself, or a buffer of its shape that does not overlap it) their weights in
+ * that order with zeros behind, up to weights_ld.  kept_lens must not be seq_lens.
+ * sfg_hip_kv_compact_v1 with these lists then evicts the others. */
+int sfg_hip_kv_select_v1(const float* weights, int64_t weights_ld, const int32_t* seq_lens,
+                         int64_t max_context, int64_t budget, int64_t recent, int32_t* keep,
+                         int32_t* kept_lens, float* kept_weights, int64_t batch, int64_t kv_heads,
+                         void* stream);
+
+/* Moves kept tokens to the front, in place: for i < counts[b], K and V of token
+ * base[b] + keep[i] of each kv head become token base[b] + i, and new_lens[b] =
+ * base[b] + counts[b] (base NULL: 0; counts clamped to [0, max_keep], the lengths
+ * to the capacity).  keep is [B][keep_heads][keep_ld], keep_heads 1 (one list for
+ * all heads: an accepted path of drafted tokens, base the committed lengths) or
+ * kv_heads (evictions, base NULL), ascending; an entry below its index or past the
+ * capacity moves nothing.  Tokens are rotated already: they keep their original
+ * positions' RoPE.  new_lens may be base or counts.  No page may be in two
+ * tables.  Page bounds of moved tokens must be made anew. */
+int sfg_hip_kv_compact_v1(void* k_pool, void* v_pool, int pool_dtype, const int32_t* page_table,
+                          const int32_t* base, const int32_t* keep, int64_t keep_heads,
+                          int64_t keep_ld, const int32_t* counts, int32_t* new_lens,
+                          int64_t max_keep, int64_t batch, int64_t kv_heads, int64_t head_dim,
+                          int64_t page_tokens, int64_t pages_per_seq, int64_t num_pages,
+                          void* stream);
+
+/* The smallest and largest value of each key dim over a page's cached tokens:
+ * bounds [num_pages][Hkv][2][D] (lowest, then highest) in the pool's dtype, exact.
+ * Refreshes the pages that hold the newest `fresh` tokens of each sequence (fresh
+ * >= max_context: all its pages); other entries stay.  NaN keys are passed over. */
+int sfg_hip_kv_page_bounds_v1(const void* k_pool, int pool_dtype, const int32_t* page_table,
+                              const int32_t* seq_lens, int64_t max_context, int64_t fresh,
+                              void* bounds, int64_t batch, int64_t kv_heads, int64_t head_dim,
+                              int64_t page_tokens, int64_t pages_per_seq, int64_t num_pages,
+                              void* stream);
+
+/* Causal attention of the newest `rows` tokens over at most top_pages pages,
+ * chosen for each query row and kv head: of the pages that hold tokens the row
+ * sees, the first sink_pages, the newest recent_pages and the others of the
+ * highest score, the sum over the group's query heads and the dims of
+ * max(q lo, q hi) -- a bound of the group's summed q.k on the page -- taken in 64
+ * bits; ties go to the lower page, NaN scores and pages outside the pool come
+ * last.  selected [B][rows][Hkv][top_pages] receives the logical pages ascending,
+ * -1 behind.  Rows see the bounds of whole pages, later rows' tokens included.
+ * sink_pages + recent_pages <= top_pages. */
+size_t sfg_hip_attn_sparse_workspace_v1(const sfg_paged_attn_args* args, int64_t top_pages);
+int sfg_hip_attn_sparse_v1(const sfg_paged_attn_args* args, const void* bounds, int64_t top_pages,
+                           int64_t sink_pages, int64_t recent_pages, int32_t* selected,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
 /* MoE routing: Router -> Softmax -> TopK -> Histogram -> PrefixSum -> Dispatch
  * (route_topk, moe_compiler.cpp:412-455; dispatch_tokens, 496-528).
  * x fp32 [T][H], router fp32 [H][E], bias fp32 [E] or NULL.  Logits are

@@ -67,6 +67,18 @@ class GemmArgs(ctypes.Structure):
     ]
 
 
+class PagedAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_vp), ("q_dtype", c_i32),
+        ("k_pool", c_vp), ("v_pool", c_vp), ("kv_dtype", c_i32),
+        ("page_table", c_vp), ("seq_lens", c_vp),
+        ("out", c_vp), ("out_dtype", c_i32),
+        ("batch", c_i64), ("q_heads", c_i64), ("kv_heads", c_i64), ("rows", c_i64), ("head_dim", c_i64),
+        ("page_tokens", c_i64), ("pages_per_seq", c_i64), ("num_pages", c_i64),
+        ("max_context", c_i64), ("kv_splits", c_i32), ("scale", c_f32),
+    ]
+
+
 class LayerDesc(ctypes.Structure):
     _fields_ = [
         ("abi", c_i32),
@@ -158,6 +170,18 @@ _SIGNATURES = {
                                            c_i64, c_vp]),
     "sfg_hip_kv_gather_paged_v1": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
                                            c_i64, c_vp, c_vp, c_vp]),
+    "sfg_hip_attn_tree_workspace_v1": (c_sz, [ctypes.POINTER(PagedAttnArgs)]),
+    "sfg_hip_attn_tree_v1": (c_i32, [ctypes.POINTER(PagedAttnArgs), c_vp, c_i64, c_vp, c_sz, c_vp]),
+    "sfg_hip_attn_weights_workspace_v1": (c_sz, [ctypes.POINTER(PagedAttnArgs)]),
+    "sfg_hip_attn_weights_v1": (c_i32, [ctypes.POINTER(PagedAttnArgs), c_vp, c_i64, c_vp, c_sz, c_vp]),
+    "sfg_hip_attn_sparse_workspace_v1": (c_sz, [ctypes.POINTER(PagedAttnArgs), c_i64]),
+    "sfg_hip_attn_sparse_v1": (c_i32, [ctypes.POINTER(PagedAttnArgs), c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_sz,
+                                       c_vp]),
+    "sfg_hip_kv_page_bounds_v1": (c_i32, [c_vp, ctypes.c_int, c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64,
+                                          c_i64, c_i64, c_i64, c_vp]),
+    "sfg_hip_kv_select_v1": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64, c_vp]),
+    "sfg_hip_kv_compact_v1": (c_i32, [c_vp, c_vp, ctypes.c_int, c_vp, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64,
+                                      c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp]),
     "sfg_hip_moe_route_workspace_v1": (c_sz, [c_i64, c_i64, c_i64]),
     "sfg_hip_moe_route_v1": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp,
                                      c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),

@@ -16,6 +16,7 @@
 #include <string>
 #include <vector>
 
+#include "sfg_api_util.hpp"
 #include "sfg_kernels.hpp"
 
 // Library-held split partials of the paged decode, for callers that cannot
@@ -29,22 +30,8 @@ namespace {
 
 thread_local std::string g_last_error;
 
-int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
-int fail(int code, const char* fmt, ...) {
-    char buf[512];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof buf, fmt, ap);
-    va_end(ap);
-    g_last_error = buf;
-    return code;
-}
-
-int check_launch(const char* what) {
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return fail(SFG_ERR_DEVICE, "%s: %s", what, hipGetErrorString(e));
-    return SFG_OK;
-}
+using sfg::check_launch;
+using sfg::fail;
 
 hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
 
@@ -183,6 +170,22 @@ int scratch_on_current_device(void** out) {
 }  // namespace
 
 namespace sfg {
+
+int fail(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    g_last_error = buf;
+    return code;
+}
+
+int check_launch(const char* what) {
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return fail(SFG_ERR_DEVICE, "%s: %s", what, hipGetErrorString(e));
+    return SFG_OK;
+}
 
 int device_xcds(hipStream_t stream) {
     // One query per device, kept in a lock-free table: concurrent first calls

@@ -24,6 +24,7 @@
 #include <type_traits>
 
 #include "sfg_kernels.hpp"
+#include "sfg_paged.hpp"
 
 namespace sfg {
 
@@ -31,8 +32,6 @@ namespace sfg {
 // Row-per-wave prefill, any head_dim up to kRowMaxD: the fp32 and bf16 shapes
 // the MFMA kernels do not lower (head_dim other than 64 / 128).
 // ===========================================================================
-constexpr int kRowMaxD = 256;
-
 template <typename InT>
 __device__ __forceinline__ float in_f32(const InT* p, int64_t i) {
     if constexpr (sizeof(InT) == 4) return p[i];
@@ -752,12 +751,6 @@ int launch_attn_prefill_vt(const uint16_t* q, const uint16_t* k, const uint16_t*
 // query per lane: the online softmax needs only a 4-lane max per page and a
 // per-lane rescale.
 // ===========================================================================
-constexpr int kPageTok = 16;
-
-typedef short short4v __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ short4v as_short4(const uint2& v) { return __builtin_bit_cast(short4v, v); }
-
 template <int G, int kDecD>
 __global__ __launch_bounds__(256) void attn_decode_split_kernel(
     const float* __restrict__ q, int64_t q_row_stride, const float* __restrict__ rope,
@@ -1154,12 +1147,6 @@ struct PagedRowsArgs {
 };
 
 template <typename KvT>
-__device__ __forceinline__ float kv_f32(const KvT* p, int64_t i) {
-    if constexpr (sizeof(KvT) == 4) return p[i];
-    else return bf16_to_f32(p[i]);
-}
-
-template <typename KvT>
 __global__ __launch_bounds__(64) void attn_paged_rows_kernel(PagedRowsArgs p) {
     const int lane = threadIdx.x;
     const int slot = blockIdx.x;  // (b seq_q + i) q_heads + h
@@ -1277,22 +1264,6 @@ __global__ __launch_bounds__(64) void attn_paged_rows_kernel(PagedRowsArgs p) {
 // finite at the end walks its pages once more: keys' non-finite elements meet
 // the leading term only, and pages with a non-finite value go token by token.
 // ===========================================================================
-struct Bf16x3 {
-    bf16x8 t[3];
-};
-// (truncated terms: a rounded leading one could overflow to infinity)
-__device__ __forceinline__ void split3(float v, uint16_t& hi, uint16_t& mid, uint16_t& lo) {
-    hi = static_cast<uint16_t>(__float_as_uint(v) >> 16);
-    const float r = v - bf16_to_f32(hi);
-    mid = static_cast<uint16_t>(__float_as_uint(r) >> 16);
-    lo = static_cast<uint16_t>(__float_as_uint(r - bf16_to_f32(mid)) >> 16);
-}
-// two bf16 values, the infinite and NaN ones replaced by zero
-__device__ __forceinline__ uint32_t finite_bf16x2(uint32_t w) {
-    const uint32_t bad = ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;  // exponent all ones
-    return w & ~((bad >> 15) * 0xFFFFu);
-}
-
 // (The bounds keep the registers of the second walk out of the way: at head_dim 64
 // three waves per SIMD instead of four cost 10%.)
 template <typename KvT, int kDecD>

@@ -144,6 +144,52 @@ int paged_rows_split_count(int64_t rows, int64_t max_keys, int32_t requested);
 size_t paged_rows_workspace_bytes(int64_t rows, int64_t head_dim, int splits);
 int launch_attn_paged_rows(const PagedRowsLaunch& a, void* workspace, hipStream_t stream);
 
+// Attention over chosen tokens of a paged cache (sfg_attention_chosen.hip): rows of
+// drafted tokens under a tree mask, decode rows that accumulate their weights, decode
+// rows over selected pages.  q and out head-major [B][Hq][rows][D].
+enum ChosenMode { kChosenTree = 0, kChosenWeights = 1, kChosenSparse = 2 };
+struct ChosenLaunch {
+    int mode;
+    const void* q; int q_dtype;
+    const void* k_pool; const void* v_pool; int kv_dtype;
+    const int32_t* page_table; const int32_t* seq_lens;
+    void* out; int out_dtype;
+    int64_t batch, q_heads, kv_heads, rows, head_dim, page_tokens, pages_per_seq, num_pages;
+    int64_t max_context;                            // no sequence is longer (tree: committed tokens)
+    float scale;
+    const uint32_t* mask; int64_t mask_stride;      // tree
+    float* weights; int64_t weights_ld;             // weights
+    const int32_t* selected; int64_t top;           // sparse
+};
+// keys: the tokens a unit walks at most.  The workspace holds the splits' partials and
+// for the weights the scaled scores.
+struct ChosenPlan {
+    int splits;
+    size_t ml_bytes, acc_bytes, scores_bytes;
+    int64_t scores_ld;
+    size_t bytes() const { return ml_bytes + acc_bytes + scores_bytes; }
+};
+ChosenPlan plan_chosen(int mode, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t rows, int64_t head_dim,
+                       int64_t page_tokens, int64_t keys, int32_t requested);
+void launch_chosen(const ChosenLaunch& a, const ChosenPlan& plan, void* workspace, hipStream_t stream);
+
+// What a paged cache keeps (sfg_kv_keep.hip).
+void launch_page_bounds(const void* k_pool, int pool_dtype, const int32_t* page_table, const int32_t* seq_lens,
+                        int64_t max_context, int64_t fresh, void* bounds, int64_t batch, int64_t kv_heads,
+                        int64_t head_dim, int64_t page_tokens, int64_t pages_per_seq, int64_t num_pages,
+                        hipStream_t stream);
+// Scores (64-bit) and the pages taken; the workspace holds the pages' sort keys.
+size_t page_select_workspace_bytes(int64_t batch, int64_t kv_heads, int64_t rows, int64_t max_pages);
+void launch_page_select(const ChosenLaunch& a, const void* bounds, int64_t sink, int64_t recent, int32_t* selected,
+                        void* workspace, hipStream_t stream);
+void launch_kv_select(const float* weights, int64_t ld, const int32_t* seq_lens, int64_t max_context, int64_t budget,
+                      int64_t recent, int32_t* keep, int32_t* kept_lens, float* kept_weights, int64_t batch,
+                      int64_t kv_heads, hipStream_t stream);
+void launch_kv_compact(void* k_pool, void* v_pool, int pool_dtype, const int32_t* page_table, const int32_t* base,
+                       const int32_t* keep, int64_t keep_heads, int64_t keep_ld, const int32_t* counts,
+                       int32_t* new_lens, int64_t max_keep, int64_t batch, int64_t kv_heads, int64_t head_dim,
+                       int64_t page_tokens, int64_t pages_per_seq, int64_t num_pages, hipStream_t stream);
+
 // Paged KV append / gather (pages pre-assigned in the tables), any head_dim and
 // page size, pools fp32 or bf16.  Sources are [b][h][t][D] with element
 // strides sb / sh / st; rope (optional) rotates the keys at their positions;

@@ -1,0 +1,39 @@
+// sfg_paged.hpp -- what the kernels over the paged KV pools share
+// (K [page][Hkv][page_tokens][D], V [page][Hkv][D][page_tokens]).
+#pragma once
+
+#include "sfg_device.hpp"
+
+namespace sfg {
+
+constexpr int kRowMaxD = 256;  // head_dim of the row-per-wave kernels
+constexpr int kPageTok = 16;   // page size of the matrix-core kernels
+
+typedef short short4v __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ short4v as_short4(const uint2& v) { return __builtin_bit_cast(short4v, v); }
+
+// An fp32 operand of the bf16 matrix instructions as three bf16 terms (24 bits).
+struct Bf16x3 {
+    bf16x8 t[3];
+};
+// (truncated terms: a rounded leading one could overflow to infinity)
+__device__ __forceinline__ void split3(float v, uint16_t& hi, uint16_t& mid, uint16_t& lo) {
+    hi = static_cast<uint16_t>(__float_as_uint(v) >> 16);
+    const float r = v - bf16_to_f32(hi);
+    mid = static_cast<uint16_t>(__float_as_uint(r) >> 16);
+    lo = static_cast<uint16_t>(__float_as_uint(r - bf16_to_f32(mid)) >> 16);
+}
+// two bf16 values, the infinite and NaN ones replaced by zero
+__device__ __forceinline__ uint32_t finite_bf16x2(uint32_t w) {
+    const uint32_t bad = ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;  // exponent all ones
+    return w & ~((bad >> 15) * 0xFFFFu);
+}
+
+template <typename KvT>
+__device__ __forceinline__ float kv_f32(const KvT* p, int64_t i) {
+    if constexpr (sizeof(KvT) == 4) return p[i];
+    else return bf16_to_f32(p[i]);
+}
+
+}  // namespace sfg

@@ -13,6 +13,7 @@
 // pages a (sequence, row, kv head) with group columns.  Splits of a unit's tokens
 // leave (m, l, acc) partials, merged in split order.
 #include <algorithm>
+#include <type_traits>
 
 #include "sfg_kernels.hpp"
 #include "sfg_paged.hpp"
@@ -211,12 +212,350 @@ __global__ __launch_bounds__(64) void chosen_any_kernel(ChosenArgs p) {
     }
 }
 
-// ===========================================================================
-// The splits of a column merged: weights 2^(m_s - M), output sum / L.
-// ===========================================================================
 // A split's weight; one without a maximum enters as it is (0, or NaN where a score was NaN).
 __device__ __forceinline__ float split_weight(float m, float M) { return m == -INFINITY ? 1.f : fast_exp2(m - M); }
 
+// ===========================================================================
+// head_dim 64 / 128 and 16-token pages on the matrix cores.  A workgroup owns 16
+// columns of a unit and one split; its four waves take a quarter of the pages each,
+// with the next page's K and V loads behind the current page's products:
+//   S^T[16 tok][16 col] = K[16 tok][D] Q^T[D][16 col]
+//   O^T[D][16 col]     += V^T[D][16 tok] P^T[16 tok][16 col]
+// The S^T accumulator (lane: column l & 15, tokens 4 (l >> 4) + r) is the P^T
+// operand's layout, so the running maximum needs two cross-lane steps a page and the
+// rescale is one factor per lane.
+//
+// FAST (bf16 queries and output over bf16 pools): Q is exact in one bf16 operand; P
+// is rounded to bf16 once, half a step (2^-8) of each weight, whose sum is as far off
+// as the rounding of the result itself.  Otherwise Q and P keep 24 bits: three bf16
+// terms over bf16 pools, fp32 matrix instructions over fp32 pools.
+//
+// What a column does not see reaches it neither as a score (replaced by -inf) nor as
+// 0 * inf: V past the unit's end is zeroed, and a page with a hidden non-finite value
+// is taken token by token.  With three terms a visible infinity would meet terms of
+// zero, so a wave whose sums are not finite walks its pages once more: keys'
+// non-finite elements meet the leading term only, values go token by token.
+// ===========================================================================
+template <typename KvT, int kD, int MODE, bool FAST>
+__global__ __launch_bounds__(256, sizeof(KvT) == 4 ? 1 : 2) void chosen_mfma_kernel(ChosenArgs p, int chunks) {
+    constexpr bool kF32 = sizeof(KvT) == 4;
+    static_assert(!(FAST && kF32), "fp32 pools keep fp32 precision");
+    constexpr int kTerms = FAST ? 1 : 3;
+    constexpr int kStep = kF32 ? 16 : 32, kKs = kD / kStep, kDt = kD / 16;
+    constexpr int kLane = kStep / 4;  // dims of a k-step per lane
+    using VecV = std::conditional_t<kF32, uint4, uint2>;  // four tokens of V
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lr = lane & 15, lg = lane >> 4;
+    const int split = blockIdx.x % p.splits;
+    const int64_t uc = blockIdx.x / p.splits;
+    const int chunk = static_cast<int>(uc % chunks);
+    const int uid = static_cast<int>(uc / chunks);
+    const int per_b = MODE == kChosenSparse ? p.rows * p.kv_heads : p.kv_heads;
+    const Unit<MODE> u = unit_of<MODE>(p, uid / per_b, uid % per_b);
+    const int col0 = 16 * chunk;
+    const int pages = (u.walk + kPageTok - 1) / kPageTok;
+    const int sp_begin = static_cast<int>(static_cast<int64_t>(pages) * split / p.splits);
+    const int sp_end = static_cast<int>(static_cast<int64_t>(pages) * (split + 1) / p.splits);
+    const int n_sp = sp_end - sp_begin;
+    const int w_begin = sp_begin + n_sp * wave / 4;
+    const int w_end = sp_begin + n_sp * (wave + 1) / 4;
+
+    // Q^T operand: this lane's column, dims kStep s + kLane lg + [0, kLane)
+    const bool has = col0 + lr < u.cols;
+    int row, head;
+    column_of<MODE>(p, u, has ? col0 + lr : col0, row, head);
+    bf16x8 qf[kF32 ? 1 : kKs][kTerms];
+    float4 qf32[kF32 ? kKs : 1];
+    {
+        const int64_t qo = column_offset(p, u.b, row, head) + kLane * lg;
+#pragma unroll
+        for (int s = 0; s < kKs; ++s) {
+            if constexpr (FAST) {
+                const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + qo + kStep * s);
+                qf[s][0] = as_bf16x8(has ? w : make_uint4(0, 0, 0, 0));
+            } else {
+                float v[kLane];
+                if (p.q_f32) {
+#pragma unroll
+                    for (int e = 0; e < kLane; e += 4)
+                        *reinterpret_cast<float4*>(v + e) = *reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + qo + kStep * s + e);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kLane; ++e) v[e] = bf16_to_f32(static_cast<const uint16_t*>(p.q)[qo + kStep * s + e]);
+                }
+#pragma unroll
+                for (int e = 0; e < kLane; ++e) v[e] = has ? v[e] : 0.f;
+                if constexpr (kF32) {
+                    qf32[s] = make_float4(v[0], v[1], v[2], v[3]);
+                } else {
+                    uint32_t w[3][4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint16_t a[3], c[3];
+                        split3(v[2 * e], a[0], a[1], a[2]);
+                        split3(v[2 * e + 1], c[0], c[1], c[2]);
+#pragma unroll
+                        for (int t = 0; t < 3; ++t) w[t][e] = static_cast<uint32_t>(a[t]) | (static_cast<uint32_t>(c[t]) << 16);
+                    }
+#pragma unroll
+                    for (int t = 0; t < kTerms; ++t) qf[s][t] = as_bf16x8(make_uint4(w[t][0], w[t][1], w[t][2], w[t][3]));
+                }
+            }
+        }
+    }
+
+    floatx4 acc[kDt];
+    float m_run, l_run;
+    const int32_t* table = p.page_table + static_cast<int64_t>(u.b) * p.pages_per_seq;
+    const int64_t head_stride = static_cast<int64_t>(kPageTok) * kD;
+    const int64_t page_stride = head_stride * p.kv_heads;
+    const KvT* kpool = static_cast<const KvT*>(p.k_pool) + u.kvh * head_stride + lr * kD + kLane * lg;
+    const KvT* vpool = static_cast<const KvT*>(p.v_pool) + u.kvh * head_stride + lr * kPageTok + 4 * lg;
+    float* scores = MODE == kChosenWeights ? p.scores + (u.id * u.cols + col0 + lr) * p.scores_ld : nullptr;
+    uint4 kb[kKs];
+    VecV vb[kDt];
+    bool okb = false;
+    int lpb = 0;
+    // logical pages and their ids 64 at a time, one per lane, so that a page's loads
+    // wait on no read of their own; an id outside the pool reads page 0 and shows no key
+    int ids = 0, lps = 0, ids_base = 0;
+    auto load_page = [&](int at) __attribute__((always_inline)) {
+        if (at - ids_base >= 64) {  // wave-uniform
+            ids_base = at;
+            int lp = at + lane;
+            if constexpr (MODE == kChosenSparse) lp = lp < w_end ? u.list[lp] : -1;
+            lps = lp;
+            ids = at + lane < w_end && lp >= 0 && lp < p.pages_per_seq ? table[lp] : -1;
+        }
+        const int id = __builtin_amdgcn_readlane(ids, at - ids_base);
+        lpb = MODE == kChosenSparse ? __builtin_amdgcn_readlane(lps, at - ids_base) : at;
+        okb = id >= 0 && id < p.num_pages;
+        const int64_t base = okb ? static_cast<int64_t>(id) * page_stride : 0;
+#pragma unroll
+        for (int s = 0; s < kKs; ++s) kb[s] = *reinterpret_cast<const uint4*>(kpool + base + kStep * s);
+#pragma unroll
+        for (int dt = 0; dt < kDt; ++dt) vb[dt] = *reinterpret_cast<const VecV*>(vpool + base + dt * 16 * kPageTok);
+    };
+    auto walk_pages = [&](auto second_c) __attribute__((always_inline)) {
+        constexpr bool kSecond = decltype(second_c)::value;
+        m_run = -INFINITY;
+        l_run = 0.f;
+#pragma unroll
+        for (int i = 0; i < kDt; ++i) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+        ids_base = w_begin - 64;
+        if (w_begin < w_end) load_page(w_begin);
+        for (int at = w_begin; at < w_end; ++at) {
+            uint4 kc[kKs];
+            VecV vc[kDt];
+#pragma unroll
+            for (int s = 0; s < kKs; ++s) kc[s] = kb[s];
+#pragma unroll
+            for (int dt = 0; dt < kDt; ++dt) vc[dt] = vb[dt];
+            const bool ok = okb;
+            const int lp = lpb;
+            if (at + 1 < w_end) load_page(at + 1);
+            const int tok0 = lp * kPageTok + 4 * lg;  // this lane's four tokens
+            const bool whole = ok && (lp + 1) * kPageTok <= u.all_see;  // wave-uniform: every column sees every token
+            uint32_t vis = 15;  // bit r: the lane's column sees token tok0 + r
+            bool slow = false;
+            if (!whole || kSecond) {
+                if (!whole) {
+                    vis = 0;
+                    if (ok && has)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (tok0 + r < u.total && sees<MODE>(p, u, row, tok0 + r)) vis |= 1u << r;
+                }
+                // tokens past the end (or of no page) are not data
+                bool bad = false;
+#pragma unroll
+                for (int dt = 0; dt < kDt; ++dt) {
+                    if constexpr (kF32) {
+                        uint32_t w[4] = {vc[dt].x, vc[dt].y, vc[dt].z, vc[dt].w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (!ok || tok0 + e >= u.total) w[e] = 0u;
+                            bad |= (w[e] & 0x7F800000u) == 0x7F800000u;
+                        }
+                        vc[dt] = make_uint4(w[0], w[1], w[2], w[3]);
+                    } else {
+                        uint32_t w[2] = {vc[dt].x, vc[dt].y};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t mask = 0xFFFFu << (16 * (e & 1));
+                            if (!ok || tok0 + e >= u.total) w[e >> 1] &= ~mask;
+                            const uint32_t expo = (w[e >> 1] >> (16 * (e & 1))) & 0x7F80u;
+                            bad |= expo == 0x7F80u;
+                        }
+                        vc[dt] = make_uint2(w[0], w[1]);
+                    }
+                }
+                slow = __any(bad);
+            }
+            floatx4 st;
+            if constexpr (kF32) {
+                // two chains; a lane's four dims feed four MFMAs
+                floatx4 s2[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                for (int s = 0; s < kKs; ++s) {
+                    const float4 kf = __builtin_bit_cast(float4, kc[s]), qq = qf32[s];
+                    s2[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf.x, qq.x, s2[0], 0, 0, 0);
+                    s2[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf.y, qq.y, s2[1], 0, 0, 0);
+                    s2[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf.z, qq.z, s2[0], 0, 0, 0);
+                    s2[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf.w, qq.w, s2[1], 0, 0, 0);
+                }
+                st = s2[0] + s2[1];
+            } else {
+                // a chain per term, the small terms summed first
+                floatx4 sk[kTerms];
+#pragma unroll
+                for (int t = 0; t < kTerms; ++t) sk[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < kKs; ++s)
+#pragma unroll
+                    for (int t = 0; t < kTerms; ++t) {
+                        uint4 k = kc[s];
+                        if (kSecond && t > 0)
+                            k = make_uint4(finite_bf16x2(k.x), finite_bf16x2(k.y), finite_bf16x2(k.z), finite_bf16x2(k.w));
+                        sk[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(k), qf[s][t], sk[t], 0, 0, 0);
+                    }
+                if constexpr (FAST) st = sk[0];
+                else st = sk[0] + (sk[1] + sk[2]);
+            }
+            float sv[4];
+            float mx = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                sv[r] = (vis >> r) & 1u ? st[r] * p.scale_log2 : -INFINITY;
+                mx = fmaxf(mx, sv[r]);
+            }
+            if constexpr (MODE == kChosenWeights)
+                if (has) *reinterpret_cast<float4*>(scores + tok0) = make_float4(sv[0], sv[1], sv[2], sv[3]);
+            mx = xor16_max(mx);
+            mx = xor32_max(mx);
+            const float m_new = fmaxf(m_run, mx);
+            const float alpha = m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_new);
+            float pv[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) pv[r] = sv[r] == -INFINITY ? 0.f : fast_exp2(sv[r] - m_new);
+            l_run = l_run * alpha + ((pv[0] + pv[1]) + (pv[2] + pv[3]));
+            m_run = m_new;
+#pragma unroll
+            for (int dt = 0; dt < kDt; ++dt) acc[dt] *= alpha;
+            if (!slow) {
+                if constexpr (kF32) {
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int dt = 0; dt < kDt; ++dt) {
+                            const float4 vf = __builtin_bit_cast(float4, vc[dt]);
+                            const float vt = t == 0 ? vf.x : t == 1 ? vf.y : t == 2 ? vf.z : vf.w;
+                            acc[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vt, pv[t], acc[dt], 0, 0, 0);
+                        }
+                } else if constexpr (FAST) {
+                    const short4v pb = as_short4(make_uint2(cvt_pk_bf16(pv[0], pv[1]), cvt_pk_bf16(pv[2], pv[3])));
+#pragma unroll
+                    for (int dt = 0; dt < kDt; ++dt)
+                        acc[dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(as_short4(vc[dt]), pb, acc[dt], 0, 0, 0);
+                } else {
+                    uint16_t w[3][4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) split3(pv[r], w[0][r], w[1][r], w[2][r]);
+#pragma unroll
+                    for (int t = 2; t >= 0; --t) {
+                        const short4v pb = as_short4(make_uint2(static_cast<uint32_t>(w[t][0]) | (static_cast<uint32_t>(w[t][1]) << 16),
+                                                                static_cast<uint32_t>(w[t][2]) | (static_cast<uint32_t>(w[t][3]) << 16)));
+#pragma unroll
+                        for (int dt = 0; dt < kDt; ++dt)
+                            acc[dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(as_short4(vc[dt]), pb, acc[dt], 0, 0, 0);
+                    }
+                }
+            } else {
+                // token by token: lane (lr, t / 4) holds its probability and whether the
+                // column sees it, lane (4 lg + r, t / 4) V of this lane's dims
+#pragma unroll 1
+                for (int t = 0; t < kPageTok; ++t) {
+                    const float mine = (t & 3) == 0 ? pv[0] : (t & 3) == 1 ? pv[1] : (t & 3) == 2 ? pv[2] : pv[3];
+                    const float pt = __shfl(mine, 16 * (t >> 2) + lr, 64);
+                    const bool seen = (__shfl(static_cast<int>(vis), 16 * (t >> 2) + lr, 64) >> (t & 3)) & 1;
+#pragma unroll
+                    for (int dt = 0; dt < kDt; ++dt) {
+                        // (masked, not selected: a select between the words is turned into
+                        // a load from scratch memory, which would hold V for every page)
+                        const uint32_t hi = 0u - static_cast<uint32_t>((t >> 1) & 1);
+                        uint32_t word;
+                        if constexpr (kF32) {
+                            const uint32_t odd = 0u - static_cast<uint32_t>(t & 1);
+                            const uint32_t lo2 = vc[dt].x ^ ((vc[dt].x ^ vc[dt].y) & odd), hi2 = vc[dt].z ^ ((vc[dt].z ^ vc[dt].w) & odd);
+                            word = lo2 ^ ((lo2 ^ hi2) & hi);
+                        } else {
+                            word = vc[dt].x ^ ((vc[dt].x ^ vc[dt].y) & hi);
+                        }
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const uint32_t w = __shfl(static_cast<int>(word), 16 * (t >> 2) + 4 * lg + r, 64);
+                            const float v = kF32 ? __uint_as_float(w) : bf16_to_f32(static_cast<uint16_t>(w >> (16 * (t & 1))));
+                            if (seen) acc[dt][r] = fmaf(pt, v, acc[dt][r]);
+                        }
+                    }
+                }
+            }
+        }
+    };
+    walk_pages(std::false_type{});
+    if constexpr (!kF32 && !FAST) {
+        float t = l_run * 0.f;  // NaN unless every sum is finite
+#pragma unroll
+        for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) t = fmaf(acc[dt][r], 0.f, t);
+        if (__any(has && t != 0.f)) walk_pages(std::true_type{});
+    }
+    // the four waves merged in LDS: acc[dt][r] = O^T[dim 16 dt + 4 lg + r][column lr]
+    __shared__ float s_m[4][16], s_l[4][16];
+    __shared__ float s_acc[4][16][kD];
+    const float l_sum = xor32_sum(xor16_sum(l_run));
+#pragma unroll
+    for (int dt = 0; dt < kDt; ++dt) *reinterpret_cast<floatx4*>(&s_acc[wave][lr][16 * dt + 4 * lg]) = acc[dt];
+    if (lg == 0) {
+        s_m[wave][lr] = m_run;
+        s_l[wave][lr] = l_sum;
+    }
+    __syncthreads();
+    for (int o = threadIdx.x; o < min(16, u.cols - col0) * kD; o += 256) {
+        const int c = o / kD, d = o % kD;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, s_m[w][c]);
+        float L = 0.f, a = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = split_weight(s_m[w][c], M);
+            L = fmaf(s_l[w][c], f, L);
+            a = fmaf(s_acc[w][c][d], f, a);
+        }
+        if (MODE != kChosenWeights && p.splits == 1) {
+            int ro, he;
+            column_of<MODE>(p, u, col0 + c, ro, he);
+            const int64_t o0 = column_offset(p, u.b, ro, he) + d;
+            const float v = a / L;  // nothing visible: 0 / 0
+            if (p.out_f32) static_cast<float*>(p.out)[o0] = v;
+            else static_cast<uint16_t*>(p.out)[o0] = f32_to_bf16(v);
+        } else {
+            const int64_t part = (u.id * u.cols + col0 + c) * p.splits + split;
+            p.part_acc[part * kD + d] = a;
+            if (d == 0) {
+                p.part_ml[2 * part] = M;
+                p.part_ml[2 * part + 1] = L;
+            }
+        }
+    }
+}
+
+// ===========================================================================
+// The splits of a column merged: weights 2^(m_s - M), output sum / L.
+// ===========================================================================
 __device__ __forceinline__ float split_max(const float* ml, int splits) {
     float M = -INFINITY;
     for (int s = 0; s < splits; ++s) M = fmaxf(M, ml[2 * s]);
@@ -232,12 +571,27 @@ __device__ __forceinline__ void merge_column(const ChosenArgs& p, const Unit<MOD
     int row, head;
     column_of<MODE>(p, u, col, row, head);
     const int64_t o0 = column_offset(p, u.b, row, head);
+    // eight splits at a time, their loads all issued before the ordered sum (slots past
+    // the count re-read the last split and are left out)
+    constexpr int kBatch = 8;
     for (int d = lane; d < p.head_dim; d += lanes) {
         float L = 0.f, o = 0.f;
-        for (int s = 0; s < p.splits; ++s) {
-            const float w = split_weight(ml[2 * s], M);
-            L = fmaf(ml[2 * s + 1], w, L);
-            o = fmaf(w, pa[static_cast<int64_t>(s) * p.head_dim + d], o);
+        for (int s0 = 0; s0 < p.splits; s0 += kBatch) {
+            float ms[kBatch], ls[kBatch], av[kBatch];
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+                const int64_t sc = min(s0 + e, p.splits - 1);
+                ms[e] = ml[2 * sc];
+                ls[e] = ml[2 * sc + 1];
+                av[e] = pa[sc * p.head_dim + d];
+            }
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+                const float w = s0 + e < p.splits ? split_weight(ms[e], M) : 0.f;
+                if (w == 0.f) continue;
+                L = fmaf(ls[e], w, L);
+                o = fmaf(w, av[e], o);
+            }
         }
         const float v = o / L;  // nothing visible: 0 / 0
         if (p.out_f32) static_cast<float*>(p.out)[o0 + d] = v;
@@ -283,14 +637,36 @@ __global__ __launch_bounds__(256) void chosen_weights_kernel(ChosenArgs p, float
     for (int c = blockIdx.y; c < u.cols; c += gridDim.y) merge_column<kChosenWeights>(p, u, c, threadIdx.x, 256);
 }
 
+constexpr int64_t kMaxGroups = 1 << 23;  // workgroups of 256 threads in a launch
+
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+template <int MODE, int kD>
+void launch_mfma(const ChosenLaunch& a, const ChosenArgs& p, unsigned grid, int chunks, hipStream_t stream) {
+    if (a.kv_dtype == SFG_F32) chosen_mfma_kernel<float, kD, MODE, false><<<grid, 256, 0, stream>>>(p, chunks);
+    else if (a.q_dtype == SFG_BF16 && a.out_dtype == SFG_BF16)
+        chosen_mfma_kernel<uint16_t, kD, MODE, true><<<grid, 256, 0, stream>>>(p, chunks);
+    else chosen_mfma_kernel<uint16_t, kD, MODE, false><<<grid, 256, 0, stream>>>(p, chunks);
+}
 
 template <int MODE>
 void launch_mode(const ChosenLaunch& a, const ChosenArgs& p, const ChosenPlan& plan, hipStream_t stream) {
     const unsigned columns = static_cast<unsigned>(a.batch * a.rows * a.q_heads);
-    const dim3 grid(columns, static_cast<unsigned>(plan.splits));
-    if (a.kv_dtype == SFG_F32) chosen_any_kernel<float, MODE><<<grid, 64, 0, stream>>>(p);
-    else chosen_any_kernel<uint16_t, MODE><<<grid, 64, 0, stream>>>(p);
+    const int64_t units = a.batch * a.kv_heads * (MODE == kChosenSparse ? a.rows : 1);
+    const int64_t chunks = (columns / units + 15) / 16;
+    // Q, K and (fp32) V are read as 16-byte vectors, bf16 V as 8-byte ones; rows of 64 or
+    // 128 elements keep a base's boundary
+    const bool aligned = ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k_pool)) & 15) == 0 &&
+                         (reinterpret_cast<uintptr_t>(a.v_pool) & (a.kv_dtype == SFG_F32 ? 15 : 7)) == 0;
+    if (plan.mfma && aligned && units * chunks * plan.splits <= kMaxGroups) {
+        const unsigned grid = static_cast<unsigned>(units * chunks * plan.splits);
+        if (a.head_dim == 128) launch_mfma<MODE, 128>(a, p, grid, static_cast<int>(chunks), stream);
+        else launch_mfma<MODE, 64>(a, p, grid, static_cast<int>(chunks), stream);
+    } else {
+        const dim3 grid(columns, static_cast<unsigned>(plan.splits));
+        if (a.kv_dtype == SFG_F32) chosen_any_kernel<float, MODE><<<grid, 64, 0, stream>>>(p);
+        else chosen_any_kernel<uint16_t, MODE><<<grid, 64, 0, stream>>>(p);
+    }
     if constexpr (MODE == kChosenWeights)
         chosen_weights_kernel<<<dim3(static_cast<unsigned>(a.batch * a.kv_heads), static_cast<unsigned>((a.max_context + 255) / 256)),
                                 256, 0, stream>>>(p, a.weights, a.weights_ld);
@@ -303,11 +679,16 @@ ChosenPlan plan_chosen(int mode, int64_t batch, int64_t q_heads, int64_t kv_head
                        int64_t page_tokens, int64_t keys, int32_t requested) {
     ChosenPlan plan{};
     const int64_t columns = batch * rows * q_heads;
-    // >= 1024 waves while every split keeps >= 256 tokens
+    plan.mfma = (head_dim == 64 || head_dim == 128) && page_tokens == kPageTok;
+    const int64_t units = batch * kv_heads * (mode == kChosenSparse ? rows : 1);
+    const int64_t base = plan.mfma ? units * ((columns / units + 15) / 16) : columns;
+    const int64_t most = plan.mfma ? (keys + kPageTok - 1) / kPageTok : keys;
     int64_t s = 1;
-    if (requested > 0) s = std::min<int64_t>(requested, std::max<int64_t>(keys, 1));
+    if (requested > 0) s = std::min<int64_t>(requested, std::max<int64_t>(most, 1));
+    // matrix cores: two workgroups per CU while a split keeps 8 pages (two per wave);
+    // else >= 1024 waves while a split keeps >= 256 tokens
     else
-        while (columns * s < 1024 && keys / (s * 2) >= 256) s *= 2;
+        while (base * s < (plan.mfma ? 512 : 1024) && most / (s * 2) >= (plan.mfma ? 8 : 256)) s *= 2;
     plan.splits = static_cast<int>(std::min<int64_t>(s, 65535));
     if (mode == kChosenWeights || plan.splits > 1) {
         const size_t parts = static_cast<size_t>(columns) * plan.splits;

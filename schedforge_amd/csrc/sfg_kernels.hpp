@@ -165,6 +165,7 @@ struct ChosenLaunch {
 // for the weights the scaled scores.
 struct ChosenPlan {
     int splits;
+    bool mfma;                                      // the matrix-core kernel's head_dim and page size
     size_t ml_bytes, acc_bytes, scores_bytes;
     int64_t scores_ld;
     size_t bytes() const { return ml_bytes + acc_bytes + scores_bytes; }

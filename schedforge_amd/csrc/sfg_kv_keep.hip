@@ -304,8 +304,11 @@ __global__ __launch_bounds__(256) void kv_kept_lens_kernel(CompactArgs a, int ba
 // every earlier destination, so a workgroup may read ahead; a chunk is written once
 // the whole chunk is read (an earlier token's source may be a later destination of
 // the same chunk).
+//
+// Any head_dim up to 256 and page size: one workgroup per (sequence, kv head), thread
+// d moving dim d.
 template <typename KvT>
-__global__ __launch_bounds__(256) void kv_compact_kernel(CompactArgs a) {
+__global__ __launch_bounds__(256) void kv_compact_any_kernel(CompactArgs a) {
     constexpr int kChunk = 8;  // tokens a step
     const int b = blockIdx.x / a.kv_heads, h = blockIdx.x % a.kv_heads;
     const int D = a.head_dim, pt = a.page_tokens;
@@ -350,6 +353,111 @@ __global__ __launch_bounds__(256) void kv_compact_kernel(CompactArgs a) {
                 kp[(to[e] * pt + slot[e]) * D + d] = kv[e];
                 vp[(to[e] * D + d) * pt + slot[e]] = vv[e];
             }
+    }
+}
+
+// 16-token pages, K rows of whole 16-byte vectors: the order above binds only what a
+// destination shares with a source, so each (sequence, kv head) splits into slices of
+// its own -- K by vectors of a row, V by dims -- and a workgroup walks its slice's
+// destinations in order.  The sources of 2048 tokens at a time are looked up first
+// (list, then table) and kept in LDS, so that a chunk's loads wait on nothing else.
+//   K: a thread moves one vector of each of 8 tokens a chunk.
+//   V: a thread builds one dim's run of a destination page (16 tokens, 32 or 64 bytes)
+//      from its tokens' pages; tokens that stay are read from their own place.
+constexpr int kCompactSeg = 2048;
+constexpr uint32_t kStays = 0xFFFFFFFFu;
+
+template <typename KvT>
+__global__ __launch_bounds__(256) void kv_compact_pages_kernel(CompactArgs a, int k_shift, int d_shift, int k_slices, int slices) {
+    constexpr int kVecs = 16 / sizeof(KvT);  // elements of a vector
+    __shared__ uint32_t src[kCompactSeg];    // page id * 16 + slot, or kStays
+    __shared__ int dpage[kCompactSeg / 16];  // destination pages' ids, -1 where nothing may be written
+    const int unit = blockIdx.x / slices, slice = blockIdx.x % slices;
+    const int b = unit / a.kv_heads, h = unit % a.kv_heads;
+    const int D = a.head_dim;
+    const int capacity = a.pages_per_seq * kPageTok;
+    const int base = a.base ? min(max(a.base[b], 0), capacity) : 0;
+    const int n = min(max(a.counts[b], 0), a.max_keep);
+    if (a.new_lens != a.base && a.new_lens != a.counts && h == 0 && slice == 0 && threadIdx.x == 0)
+        a.new_lens[b] = kept_length(base, n, capacity);
+    const int32_t* keep = a.keep + (static_cast<int64_t>(b) * a.keep_heads + (a.keep_heads == 1 ? 0 : h)) * a.keep_ld;
+    const int32_t* table = a.page_table + static_cast<int64_t>(b) * a.pages_per_seq;
+    KvT* kp = static_cast<KvT*>(a.k_pool);
+    KvT* vp = static_cast<KvT*>(a.v_pool);
+    const int end = min(base + n, capacity);  // base + n <= 2^30 + 2^30
+    for (int s0 = base & ~15; s0 < end; s0 += kCompactSeg) {
+        const int count = min(kCompactSeg, (end - s0 + 15) & ~15);
+        __syncthreads();
+        for (int q = threadIdx.x; q < count; q += 256) {
+            const int pos = s0 + q, i = pos - base;
+            uint32_t code = kStays;
+            if (pos >= base && pos < end) {
+                const int k = keep[i];
+                if (k > i && k < capacity - base) {
+                    const int id = table[(base + k) / kPageTok];
+                    if (id >= 0 && id < a.num_pages) code = static_cast<uint32_t>(id) * kPageTok + ((base + k) & 15);
+                }
+            }
+            src[q] = code;
+            if ((q & 15) == 0) {
+                const int id = table[pos / kPageTok];
+                dpage[q / 16] = id >= 0 && id < a.num_pages ? id : -1;
+            }
+        }
+        __syncthreads();
+        if (slice < k_slices) {
+            const int vecs = D / kVecs;
+            const int vec = (slice << k_shift) + (threadIdx.x & ((1 << k_shift) - 1));
+            const int per = 256 >> k_shift;  // tokens a step of the workgroup
+            uint4* kv4 = reinterpret_cast<uint4*>(kp);
+            for (int c0 = 0; c0 < count; c0 += 8 * per) {
+                uint4 r[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int q = c0 + j * per + (threadIdx.x >> k_shift);
+                    const uint32_t code = q < count ? src[q] : kStays;
+                    r[j] = make_uint4(0, 0, 0, 0);
+                    if (code != kStays && vec < vecs)
+                        r[j] = kv4[((static_cast<int64_t>(code >> 4) * a.kv_heads + h) * kPageTok + (code & 15)) * vecs + vec];
+                }
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int q = c0 + j * per + (threadIdx.x >> k_shift);
+                    if (q < count && src[q] != kStays && dpage[q / 16] >= 0 && vec < vecs)
+                        kv4[((static_cast<int64_t>(dpage[q / 16]) * a.kv_heads + h) * kPageTok + (q & 15)) * vecs + vec] = r[j];
+                }
+            }
+        } else {
+            const int d = ((slice - k_slices) << d_shift) + (threadIdx.x & ((1 << d_shift) - 1));
+            const int per = 256 >> d_shift;  // pages a step
+            for (int g0 = 0; g0 < count / 16; g0 += per) {
+                const int g = g0 + (threadIdx.x >> d_shift);
+                KvT r[kPageTok];
+                bool moves = false;
+                int64_t own = 0;
+                if (g < count / 16 && d < D && dpage[g] >= 0) {
+                    own = ((static_cast<int64_t>(dpage[g]) * a.kv_heads + h) * D + d) * kPageTok;
+#pragma unroll
+                    for (int e = 0; e < kPageTok; ++e) moves |= src[16 * g + e] != kStays;
+                    if (moves)
+#pragma unroll
+                        for (int e = 0; e < kPageTok; ++e) {
+                            const uint32_t code = src[16 * g + e];
+                            const int64_t at = ((static_cast<int64_t>(code >> 4) * a.kv_heads + h) * D + d) * kPageTok + (code & 15);
+                            r[e] = vp[code == kStays ? own + e : at];
+                        }
+                }
+                __syncthreads();
+                if (moves) {
+                    constexpr int kRun = kPageTok * sizeof(KvT) / 16;
+                    uint4 w[kRun];
+                    __builtin_memcpy(w, r, sizeof w);
+#pragma unroll
+                    for (int e = 0; e < kRun; ++e) reinterpret_cast<uint4*>(vp + own)[e] = w[e];
+                }
+            }
+        }
     }
 }
 
@@ -417,9 +525,28 @@ void launch_kv_compact(void* k_pool, void* v_pool, int pool_dtype, const int32_t
     a.kv_heads = static_cast<int>(kv_heads); a.head_dim = static_cast<int>(head_dim);
     a.page_tokens = static_cast<int>(page_tokens); a.pages_per_seq = static_cast<int>(pages_per_seq);
     a.num_pages = static_cast<int>(num_pages);
-    const unsigned grid = static_cast<unsigned>(batch * kv_heads);
-    if (pool_dtype == SFG_F32) kv_compact_kernel<float><<<grid, 256, 0, stream>>>(a);
-    else kv_compact_kernel<uint16_t><<<grid, 256, 0, stream>>>(a);
+    const int64_t units = batch * kv_heads, esz = pool_dtype == SFG_F32 ? 4 : 2;
+    const bool pages = page_tokens == kPageTok && head_dim * esz % 16 == 0 && num_pages <= (1 << 27) &&
+                       ((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) & 15) == 0;
+    if (pages) {
+        // slices of 16 vectors and 64 dims, halved while fewer than 512 workgroups result
+        int k_shift = 4, d_shift = 6;
+        const int64_t vecs = head_dim * esz / 16;
+        auto ks = [&] { return (vecs + (1 << k_shift) - 1) >> k_shift; };
+        auto ds = [&] { return (head_dim + (1 << d_shift) - 1) >> d_shift; };
+        while (k_shift > 1 && units * (ks() + ds()) < 512) {
+            --k_shift;
+            --d_shift;
+        }
+        const int slices = static_cast<int>(ks() + ds());
+        const unsigned grid = static_cast<unsigned>(units * slices);
+        if (pool_dtype == SFG_F32) kv_compact_pages_kernel<float><<<grid, 256, 0, stream>>>(a, k_shift, d_shift, static_cast<int>(ks()), slices);
+        else kv_compact_pages_kernel<uint16_t><<<grid, 256, 0, stream>>>(a, k_shift, d_shift, static_cast<int>(ks()), slices);
+    } else if (pool_dtype == SFG_F32) {
+        kv_compact_any_kernel<float><<<static_cast<unsigned>(units), 256, 0, stream>>>(a);
+    } else {
+        kv_compact_any_kernel<uint16_t><<<static_cast<unsigned>(units), 256, 0, stream>>>(a);
+    }
     if (new_lens == base || new_lens == counts)
         kv_kept_lens_kernel<<<static_cast<unsigned>((batch + 255) / 256), 256, 0, stream>>>(a, static_cast<int>(batch));
 }

@@ -556,42 +556,43 @@ __global__ __launch_bounds__(256, sizeof(KvT) == 4 ? 1 : 2) void chosen_mfma_ker
 // ===========================================================================
 // The splits of a column merged: weights 2^(m_s - M), output sum / L.
 // ===========================================================================
-__device__ __forceinline__ float split_max(const float* ml, int splits) {
-    float M = -INFINITY;
-    for (int s = 0; s < splits; ++s) M = fmaxf(M, ml[2 * s]);
-    return M;
+// A column's maximum and sum over its splits, by the whole wave.
+__device__ __forceinline__ void merge_ml(const float* ml, int splits, int lane, float& M, float& L) {
+    float m = -INFINITY;
+    for (int s = lane; s < splits; s += 64) m = fmaxf(m, ml[2 * s]);
+    M = wave_max(m);
+    float l = 0.f;
+    for (int s = lane; s < splits; s += 64) l = fmaf(ml[2 * s + 1], split_weight(ml[2 * s], M), l);
+    L = wave_sum(l);
 }
 
+// By `lanes` threads (whole waves), thread t the dims t, t + lanes, ...
 template <int MODE>
-__device__ __forceinline__ void merge_column(const ChosenArgs& p, const Unit<MODE>& u, int col, int lane, int lanes) {
+__device__ __forceinline__ void merge_column(const ChosenArgs& p, const Unit<MODE>& u, int col, int t, int lanes) {
     const int64_t slot = u.id * u.cols + col;
     const float* ml = p.part_ml + 2 * slot * p.splits;
     const float* pa = p.part_acc + slot * p.splits * p.head_dim;
-    const float M = split_max(ml, p.splits);
+    float M, L;
+    merge_ml(ml, p.splits, t & 63, M, L);
     int row, head;
     column_of<MODE>(p, u, col, row, head);
     const int64_t o0 = column_offset(p, u.b, row, head);
     // eight splits at a time, their loads all issued before the ordered sum (slots past
     // the count re-read the last split and are left out)
     constexpr int kBatch = 8;
-    for (int d = lane; d < p.head_dim; d += lanes) {
-        float L = 0.f, o = 0.f;
+    for (int d = t; d < p.head_dim; d += lanes) {
+        float o = 0.f;
         for (int s0 = 0; s0 < p.splits; s0 += kBatch) {
-            float ms[kBatch], ls[kBatch], av[kBatch];
+            float ms[kBatch], av[kBatch];
 #pragma unroll
             for (int e = 0; e < kBatch; ++e) {
                 const int64_t sc = min(s0 + e, p.splits - 1);
                 ms[e] = ml[2 * sc];
-                ls[e] = ml[2 * sc + 1];
                 av[e] = pa[sc * p.head_dim + d];
             }
 #pragma unroll
-            for (int e = 0; e < kBatch; ++e) {
-                const float w = s0 + e < p.splits ? split_weight(ms[e], M) : 0.f;
-                if (w == 0.f) continue;
-                L = fmaf(ls[e], w, L);
-                o = fmaf(w, av[e], o);
-            }
+            for (int e = 0; e < kBatch; ++e)
+                if (s0 + e < p.splits) o = fmaf(split_weight(ms[e], M), av[e], o);
         }
         const float v = o / L;  // nothing visible: 0 / 0
         if (p.out_f32) static_cast<float*>(p.out)[o0 + d] = v;
@@ -600,10 +601,10 @@ __device__ __forceinline__ void merge_column(const ChosenArgs& p, const Unit<MOD
 }
 
 template <int MODE>
-__global__ __launch_bounds__(64) void chosen_combine_kernel(ChosenArgs p) {
+__global__ __launch_bounds__(128) void chosen_combine_kernel(ChosenArgs p) {
     int col;
     const Unit<MODE> u = unit_of_slot<MODE>(p, blockIdx.x, col);
-    merge_column<MODE>(p, u, col, threadIdx.x, 64);
+    merge_column<MODE>(p, u, col, threadIdx.x, blockDim.x);
 }
 
 // The weights' end: every workgroup merges the columns' (m, l) of its (sequence,
@@ -618,13 +619,13 @@ __global__ __launch_bounds__(256) void chosen_weights_kernel(ChosenArgs p, float
     for (int c0 = 0; c0 < u.cols; c0 += kCols) {
         const int n = min(kCols, u.cols - c0);
         __syncthreads();
-        for (int c = threadIdx.x; c < n; c += 256) {
-            const float* ml = p.part_ml + 2 * (u.id * u.cols + c0 + c) * p.splits;
-            const float M = split_max(ml, p.splits);
-            float L = 0.f;
-            for (int s = 0; s < p.splits; ++s) L = fmaf(ml[2 * s + 1], split_weight(ml[2 * s], M), L);
-            sM[c] = M;
-            sR[c] = L == 0.f ? 0.f : 1.f / L;
+        for (int c = threadIdx.x >> 6; c < n; c += 4) {
+            float M, L;
+            merge_ml(p.part_ml + 2 * (u.id * u.cols + c0 + c) * p.splits, p.splits, threadIdx.x & 63, M, L);
+            if ((threadIdx.x & 63) == 0) {
+                sM[c] = M;
+                sR[c] = L == 0.f ? 0.f : 1.f / L;
+            }
         }
         __syncthreads();
         if (tok < u.total)
@@ -670,7 +671,7 @@ void launch_mode(const ChosenLaunch& a, const ChosenArgs& p, const ChosenPlan& p
     if constexpr (MODE == kChosenWeights)
         chosen_weights_kernel<<<dim3(static_cast<unsigned>(a.batch * a.kv_heads), static_cast<unsigned>((a.max_context + 255) / 256)),
                                 256, 0, stream>>>(p, a.weights, a.weights_ld);
-    else if (plan.splits > 1) chosen_combine_kernel<MODE><<<columns, 64, 0, stream>>>(p);
+    else if (plan.splits > 1) chosen_combine_kernel<MODE><<<columns, a.head_dim > 64 ? 128 : 64, 0, stream>>>(p);
 }
 
 }  // namespace

@@ -72,76 +72,203 @@ __global__ __launch_bounds__(64) void page_bounds_kernel(BoundsArgs a) {
 }
 
 // ---------------------------------------------------------------- selection
-constexpr int kSelThreads = 1024;
-constexpr int kSelBins = 2048;
+// One workgroup of 1024 threads selects among n keys, thread t holding kSelKeys
+// consecutive ones of each tile of 4096 in registers (the keys of more than one tile
+// are read again for every pass).
+constexpr int kSelThreads = 1024, kSelKeys = 4, kSelTile = kSelThreads * kSelKeys;
+constexpr int kSelBits = 11, kSelBins = 1 << kSelBits;
+constexpr int kSelFew = 64;
 
+template <typename Key>
 struct SelShared {
     int hist[kSelBins];
-    int wave[kSelThreads / 64];
-    int bin, above;
+    int2 wave[kSelThreads / 64];
+    Key lo[kSelThreads / 64], hi[kSelThreads / 64];
+    Key few[kSelFew];
+    int bin, above, count, fill;
+    Key found; int ties;
 };
 
-// Exclusive sum over the workgroup's threads; total in `all`.
-__device__ __forceinline__ int block_exclusive(int v, SelShared& sh, int& all) {
+// Exclusive sums over the workgroup's threads; totals in `all`.
+template <typename Key>
+__device__ __forceinline__ int2 block_exclusive(int2 v, SelShared<Key>& sh, int2& all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = v;
+    int2 x = v;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o, 64);
-        if (lane >= o) x += y;
+        const int a = __shfl_up(x.x, o, 64), c = __shfl_up(x.y, o, 64);
+        if (lane >= o) {
+            x.x += a;
+            x.y += c;
+        }
     }
     __syncthreads();
     if (lane == 63) sh.wave[wave] = x;
     __syncthreads();
-    int before = 0;
-    all = 0;
+    int2 before = make_int2(0, 0);
+    all = before;
+#pragma unroll
     for (int w = 0; w < kSelThreads / 64; ++w) {
-        if (w < wave) before += sh.wave[w];
-        all += sh.wave[w];
+        const int2 s = sh.wave[w];
+        if (w < wave) {
+            before.x += s.x;
+            before.y += s.y;
+        }
+        all.x += s.x;
+        all.y += s.y;
     }
-    return before + x - v;
+    return make_int2(before.x + x.x - v.x, before.y + x.y - v.y);
 }
 
-// The need-th largest of n keys (1 <= need <= n): every key above `key` is taken, and
-// `ties` of those equal to it.  Radix selection from the top, 11 bits a pass: the
-// workgroup counts a digit of the keys that match the digits found so far, and the
-// bin in which the count from above passes `need` is the next digit.
-template <typename Key, typename Load>
-__device__ void select_threshold(Load load, int n, int need, SelShared& sh, Key& key, int& ties) {
+// The need-th largest of n candidates (1 <= need <= n): every key above `key` is taken
+// and `ties` of those equal to it.  Radix selection below the bits that all keys share,
+// 11 bits a pass: the workgroup counts a digit of the keys that match the digits found
+// so far; the bin in which the count from above passes `need` is the next digit.  Once
+// that bin holds at most 64 keys, they are ranked against each other.
+// each(f): calls f(key) for every candidate key of this thread.
+template <typename Key, typename Each>
+__device__ __forceinline__ void select_threshold(Each each, int need, SelShared<Key>& sh, Key& key, int& ties) {
     constexpr int kBits = sizeof(Key) * 8;
-    Key prefix = 0;
-    int done = 0;
-    while (done < kBits) {
-        const int width = min(11, kBits - done);
-        const int shift = kBits - done - width;
-        __syncthreads();
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    Key lo = ~Key(0), hi = 0;
+    each([&](Key k) {
+        lo = min(lo, k);
+        hi = max(hi, k);
+    });
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        lo = min(lo, static_cast<Key>(__shfl_xor(lo, o, 64)));
+        hi = max(hi, static_cast<Key>(__shfl_xor(hi, o, 64)));
+    }
+    if (lane == 0) {
+        sh.lo[wave] = lo;
+        sh.hi[wave] = hi;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSelThreads / 64; ++w) {
+        lo = min(lo, sh.lo[w]);
+        hi = max(hi, sh.hi[w]);
+    }
+    if (lo == hi) {
+        key = lo;
+        ties = need;
+        return;
+    }
+    // bits from `open` down are not known yet; keys that match agree with `key` above them
+    int open = kBits - (kBits == 64 ? __clzll(static_cast<long long>(lo ^ hi)) : __clz(static_cast<int>(lo ^ hi)));
+    key = open == kBits ? Key(0) : hi >> open;
+    while (open > 0) {
+        const int width = min(kSelBits, open), shift = open - width;
         for (int i = threadIdx.x; i < kSelBins; i += kSelThreads) sh.hist[i] = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < n; i += kSelThreads) {
-            const Key k = load(i);
-            if (done == 0 || (k >> (shift + width)) == prefix)
-                atomicAdd(&sh.hist[static_cast<int>(k >> shift) & ((1 << width) - 1)], 1);
-        }
+        each([&](Key k) {
+            if (open == kBits || (k >> open) == key) atomicAdd(&sh.hist[static_cast<int>(k >> shift) & ((1 << width) - 1)], 1);
+        });
         __syncthreads();
         // two bins a thread, counted from the top one
         const int top = kSelBins - 1 - 2 * static_cast<int>(threadIdx.x);
         const int c1 = sh.hist[top], c0 = sh.hist[top - 1];
-        int all;
-        const int above = block_exclusive(c1 + c0, sh, all);
+        int2 all;
+        const int above = block_exclusive(make_int2(c1 + c0, 0), sh, all).x;
         if (above < need && need <= above + c1) {
             sh.bin = top;
             sh.above = above;
+            sh.count = c1;
         } else if (above + c1 < need && need <= above + c1 + c0) {
             sh.bin = top - 1;
             sh.above = above + c1;
+            sh.count = c0;
         }
+        if (threadIdx.x == 0) sh.fill = 0;
         __syncthreads();
-        prefix = (prefix << width) | static_cast<Key>(sh.bin);
+        key = (key << width) | static_cast<Key>(sh.bin);
         need -= sh.above;
-        done += width;
+        open = shift;
+        if (open > 0 && sh.count <= kSelFew) {
+            each([&](Key k) {
+                if ((k >> open) == key) sh.few[atomicAdd(&sh.fill, 1)] = k;
+            });
+            __syncthreads();
+            // the key with fewer than `need` above it and at least `need` not below it
+            if (static_cast<int>(threadIdx.x) < sh.count) {
+                const Key mine = sh.few[threadIdx.x];
+                int above_me = 0, same = 0;
+                for (int i = 0; i < sh.count; ++i) {
+                    above_me += sh.few[i] > mine;
+                    same += sh.few[i] == mine;
+                }
+                if (above_me < need && need <= above_me + same) {
+                    sh.found = mine;
+                    sh.ties = need - above_me;
+                }
+            }
+            __syncthreads();
+            key = sh.found;
+            need = sh.ties;
+            open = 0;
+        }
     }
-    key = prefix;
     ties = need;
+}
+
+// Emits, ascending, the indexes taken among [0, n): those with must(i), and of the
+// candidates (the others) the `need` largest keys, ties to the lower index.
+// load(i): the key of candidate i; emit(at, i).  Returns how many were taken.
+template <typename Key, typename Load, typename Must, typename Emit>
+__device__ __forceinline__ int select_and_emit(int n, int need, bool everything, Load load, Must must, Emit emit, SelShared<Key>& sh) {
+    const bool single = n <= kSelTile;
+    const int first = kSelKeys * static_cast<int>(threadIdx.x);
+    Key k[kSelKeys];
+    auto read = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < kSelKeys; ++r) {
+            const int i = tile + first + r;
+            k[r] = i < n && !everything && !must(i) ? load(i) : Key(0);
+        }
+    };
+    if (single) read(0);
+    Key key = 0;
+    int ties = 0;
+    if (!everything && need > 0)
+        select_threshold<Key>([&](auto f) __attribute__((always_inline)) {
+            for (int tile = 0; tile < n; tile += kSelTile) {
+                if (!single) read(tile);
+#pragma unroll
+                for (int r = 0; r < kSelKeys; ++r) {
+                    const int i = tile + first + r;
+                    if (i < n && !must(i)) f(k[r]);
+                }
+            }
+        }, need, sh, key, ties);
+    int written = 0, tied = 0;
+    for (int tile = 0; tile < n; tile += kSelTile) {
+        if (!single) read(tile);
+        int2 mine = make_int2(0, 0);  // taken for sure, equal to the threshold
+        uint32_t sure = 0, equal = 0;
+#pragma unroll
+        for (int r = 0; r < kSelKeys; ++r) {
+            const int i = tile + first + r;
+            if (i >= n) continue;
+            if (everything || must(i) || (need > 0 && k[r] > key)) sure |= 1u << r;
+            else if (need > 0 && k[r] == key) equal |= 1u << r;
+        }
+        mine.x = __popc(sure);
+        mine.y = __popc(equal);
+        int2 all;
+        const int2 before = block_exclusive(mine, sh, all);
+        int at = written + before.x + min(tied + before.y, ties) - min(tied, ties);
+        int rank = tied + before.y;
+#pragma unroll
+        for (int r = 0; r < kSelKeys; ++r) {
+            const bool take = (sure >> r) & 1u || ((equal >> r) & 1u && rank < ties);
+            rank += (equal >> r) & 1u;
+            if (take) emit(at++, tile + first + r);
+        }
+        written += all.x + min(tied + all.y, ties) - min(tied, ties);
+        tied += all.y;
+    }
+    return written;
 }
 
 struct TokenSelectArgs {
@@ -153,7 +280,7 @@ struct TokenSelectArgs {
 
 // One workgroup per (sequence, kv head).
 __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(TokenSelectArgs a) {
-    __shared__ SelShared sh;
+    __shared__ SelShared<uint32_t> sh;
     const int b = blockIdx.x / a.kv_heads, h = blockIdx.x % a.kv_heads;
     const int len = a.seq_lens ? min(max(a.seq_lens[b], 0), a.max_len) : a.max_len;
     const int n = min(len, a.budget);
@@ -162,39 +289,29 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(TokenSelectArgs 
     int32_t* keep = a.keep + static_cast<int64_t>(blockIdx.x) * a.budget;
     if (h == 0 && threadIdx.x == 0) a.kept_lens[b] = n;
     // tokens from `old` on are kept; of those before, `need` of the largest weight
-    const int old = max(len - a.recent, 0), need = len > n ? a.budget - a.recent : old;
-    uint32_t key = 0;
-    int ties = 0;
-    if (need > 0 && need < old) select_threshold<uint32_t>([&](int i) { return order_key(w[i]); }, old, need, sh, key, ties);
-    const bool all_old = need >= old;
-    int written = 0, tied = 0;
-    for (int base = 0; base < len; base += kSelThreads) {
-        const int i = base + threadIdx.x;
-        const float v = i < len ? w[i] : 0.f;
-        bool equal = false, take = false;
-        if (i < len) {
-            if (i >= old || all_old) take = true;
-            else if (need > 0) {
-                const uint32_t k = order_key(v);
-                take = k > key;
-                equal = k == key;
-            }
-        }
-        int all;
-        const int rank = block_exclusive(equal ? 1 : 0, sh, all);
-        if (equal && tied + rank < ties) take = true;
-        tied += all;
-        const int at = written + block_exclusive(take ? 1 : 0, sh, all);
-        written += all;
-        // (every load of this chunk is behind the sums' barriers, and later chunks
-        // read beyond what is written here: kept may be the weights themselves)
-        if (take) {
-            keep[at] = i;
-            if (kept) kept[at] = v;
-        }
-    }
+    const int old = max(len - a.recent, 0);
+    select_and_emit<uint32_t>(len, a.budget - a.recent, len <= a.budget,
+                              [&](int i) { return order_key(w[i]); }, [&](int i) { return i >= old; },
+                              [&](int at, int i) { keep[at] = i; }, sh);
     for (int i = n + threadIdx.x; i < a.budget; i += kSelThreads) keep[i] = -1;
     if (kept) {
+        // the weights in the list's order, a tile at a time: sources lie at or behind their
+        // destinations, and a tile is read whole before it is written
+        __syncthreads();
+        for (int base = 0; base < n; base += kSelTile) {
+            float x[kSelKeys];
+#pragma unroll
+            for (int r = 0; r < kSelKeys; ++r) {
+                const int i = base + r * kSelThreads + static_cast<int>(threadIdx.x);
+                x[r] = i < n ? w[keep[i]] : 0.f;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < kSelKeys; ++r) {
+                const int i = base + r * kSelThreads + static_cast<int>(threadIdx.x);
+                if (i < n) kept[i] = x[r];
+            }
+        }
         __syncthreads();
         for (int64_t i = n + threadIdx.x; i < a.ld; i += kSelThreads) kept[i] = 0.f;
     }
@@ -207,6 +324,7 @@ struct PageScoreArgs {
     uint64_t* keys; int64_t max_pages;
     int32_t* selected;
     int q_heads, kv_heads, rows, head_dim, page_tokens, pages_per_seq, num_pages, top, sink, recent;
+    int pages_per_wave;
 };
 
 __device__ __forceinline__ int row_pages(const PageScoreArgs& a, int b, int row) {
@@ -214,14 +332,10 @@ __device__ __forceinline__ int row_pages(const PageScoreArgs& a, int b, int row)
     return (max(len - a.rows + row + 1, 0) + a.page_tokens - 1) / a.page_tokens;
 }
 
-// Workgroups of a (sequence, row, kv head) walk its pages, one wave a page.
-template <typename KvT>
-__global__ __launch_bounds__(256) void page_score_kernel(PageScoreArgs a) {
-    __shared__ double up[kRowMaxD], down[kRowMaxD];
-    const int64_t unit = blockIdx.x;
-    const int h = static_cast<int>(unit % a.kv_heads);
-    const int row = static_cast<int>(unit / a.kv_heads % a.rows), b = static_cast<int>(unit / a.kv_heads / a.rows);
-    const int pages = row_pages(a, b, row), D = a.head_dim, G = a.q_heads / a.kv_heads;
+// score = sum_d P_d hi_d + N_d lo_d, P and N the group's sums of max(q, 0) and min(q, 0)
+// (which makes the work per page independent of the group's size): P and N to LDS.
+__device__ __forceinline__ void group_query(const PageScoreArgs& a, int b, int h, int row, double* up, double* down) {
+    const int D = a.head_dim, G = a.q_heads / a.kv_heads;
     for (int d = threadIdx.x; d < D; d += 256) {
         double hi = 0.0, lo = 0.0;
         for (int g = 0; g < G; ++g) {
@@ -234,6 +348,18 @@ __global__ __launch_bounds__(256) void page_score_kernel(PageScoreArgs a) {
         down[d] = lo;
     }
     __syncthreads();
+}
+
+// Any head_dim: workgroups of a (sequence, row, kv head) walk its pages, one wave a page.
+template <typename KvT>
+__global__ __launch_bounds__(256) void page_score_any_kernel(PageScoreArgs a) {
+    __shared__ double up[kRowMaxD], down[kRowMaxD];
+    const int64_t unit = blockIdx.x;
+    const int h = static_cast<int>(unit % a.kv_heads);
+    const int row = static_cast<int>(unit / a.kv_heads % a.rows), b = static_cast<int>(unit / a.kv_heads / a.rows);
+    const int pages = row_pages(a, b, row), D = a.head_dim;
+    if (static_cast<int>(blockIdx.y) * 4 >= pages) return;
+    group_query(a, b, h, row, up, down);
     const int lane = threadIdx.x & 63;
     for (int page = blockIdx.y * 4 + (threadIdx.x >> 6); page < pages; page += gridDim.y * 4) {
         const int id = a.page_table[static_cast<int64_t>(b) * a.pages_per_seq + page];
@@ -248,35 +374,96 @@ __global__ __launch_bounds__(256) void page_score_kernel(PageScoreArgs a) {
         } else {
             s = -INFINITY;
         }
-        if (lane == 0)
-            a.keys[unit * a.max_pages + page] = page < a.sink || page >= pages - a.recent ? ~0ull : order_key(s);
+        if (lane == 0) a.keys[unit * a.max_pages + page] = order_key(s);
+    }
+}
+
+// The value of lane l ^ X in 16-lane rows, both halves of a double.
+template <int X>
+__device__ __forceinline__ double lane_xor_f64(double v) {
+    const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));
+    float lo = __uint_as_float(static_cast<uint32_t>(u)), hi = __uint_as_float(static_cast<uint32_t>(u >> 32));
+    if constexpr (X == 1) { lo = lane_xor1(lo); hi = lane_xor1(hi); }
+    else if constexpr (X == 2) { lo = lane_xor2(lo); hi = lane_xor2(hi); }
+    else if constexpr (X == 4) { lo = lane_xor4(lo); hi = lane_xor4(hi); }
+    else { lo = lane_xor8(lo); hi = lane_xor8(hi); }
+    return __longlong_as_double(static_cast<long long>((static_cast<uint64_t>(__float_as_uint(hi)) << 32) | __float_as_uint(lo)));
+}
+
+// head_dim 64 / 128: 8 or 16 lanes a page, eight dims each, their P and N in registers;
+// a wave takes 8 or 4 pages at a time, four such groups' bounds in flight.  Bound by
+// reading the bounds (4 D bytes a bf16 page and head).
+template <typename KvT, int kD>
+__global__ __launch_bounds__(256) void page_score_kernel(PageScoreArgs a) {
+    constexpr int kLanes = kD / 8, kPer = 64 / kLanes, kGroups = 4;
+    __shared__ double up[kD], down[kD];
+    const int64_t unit = blockIdx.x;
+    const int h = static_cast<int>(unit % a.kv_heads);
+    const int row = static_cast<int>(unit / a.kv_heads % a.rows), b = static_cast<int>(unit / a.kv_heads / a.rows);
+    const int pages = row_pages(a, b, row);
+    if (static_cast<int>(blockIdx.y) * 4 * a.pages_per_wave >= pages) return;
+    group_query(a, b, h, row, up, down);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int sub = lane / kLanes, d0 = (lane % kLanes) * 8;
+    double P[8], N[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        P[e] = up[d0 + e];
+        N[e] = down[d0 + e];
+    }
+    const int begin = (static_cast<int>(blockIdx.y) * 4 + wave) * a.pages_per_wave;
+    const int end = min(begin + a.pages_per_wave, pages);
+    // pages_per_wave is at most 64: the wave's page ids, one a lane
+    const int mine = begin + lane < end ? a.page_table[static_cast<int64_t>(b) * a.pages_per_seq + begin + lane] : -1;
+    uint64_t* keys = a.keys + unit * a.max_pages;
+    for (int p0 = begin; p0 < end; p0 += kPer * kGroups) {
+        constexpr int kV = 8 * sizeof(KvT) / 16;  // vectors of eight dims
+        uint4 lo[kGroups][kV], hi[kGroups][kV];
+        bool ok[kGroups];
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            const int page = p0 + g * kPer + sub;
+            const int id = __shfl(mine, (page - begin) & 63, 64);
+            ok[g] = page < end && id >= 0 && id < a.num_pages;
+            const KvT* at = static_cast<const KvT*>(a.bounds) + (static_cast<int64_t>(ok[g] ? id : 0) * a.kv_heads + h) * 2 * kD + d0;
+#pragma unroll
+            for (int v = 0; v < kV; ++v) {
+                lo[g][v] = reinterpret_cast<const uint4*>(at)[v];
+                hi[g][v] = reinterpret_cast<const uint4*>(at + kD)[v];
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            KvT l[8], u[8];
+            __builtin_memcpy(l, lo[g], sizeof l);
+            __builtin_memcpy(u, hi[g], sizeof u);
+            double s = 0.0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                s = fma(P[e], static_cast<double>(kv_f32(u, e)), s);
+                s = fma(N[e], static_cast<double>(kv_f32(l, e)), s);
+            }
+            s += lane_xor_f64<1>(s);
+            s += lane_xor_f64<2>(s);
+            s += lane_xor_f64<4>(s);
+            if constexpr (kLanes == 16) s += lane_xor_f64<8>(s);
+            const int page = p0 + g * kPer + sub;
+            if (lane % kLanes == 0 && page < end) keys[page] = order_key(ok[g] ? s : -INFINITY);
+        }
     }
 }
 
 __global__ __launch_bounds__(kSelThreads) void page_select_kernel(PageScoreArgs a) {
-    __shared__ SelShared sh;
+    __shared__ SelShared<uint64_t> sh;
     const int64_t unit = blockIdx.x;
     const int row = static_cast<int>(unit / a.kv_heads % a.rows), b = static_cast<int>(unit / a.kv_heads / a.rows);
     const int pages = row_pages(a, b, row), n = min(pages, a.top);
     const uint64_t* keys = a.keys + unit * a.max_pages;
     int32_t* out = a.selected + unit * a.top;
-    uint64_t key = 0;
-    int ties = 0;
-    if (n < pages) select_threshold<uint64_t>([&](int i) { return keys[i]; }, pages, n, sh, key, ties);
-    int written = 0, tied = 0;
-    for (int base = 0; base < pages; base += kSelThreads) {
-        const int i = base + threadIdx.x;
-        const uint64_t k = i < pages ? keys[i] : 0;
-        const bool equal = i < pages && n < pages && k == key;
-        bool take = i < pages && (n == pages || k > key);
-        int all;
-        const int rank = block_exclusive(equal ? 1 : 0, sh, all);
-        if (equal && tied + rank < ties) take = true;
-        tied += all;
-        const int at = written + block_exclusive(take ? 1 : 0, sh, all);
-        written += all;
-        if (take) out[at] = i;
-    }
+    // (top >= sink + recent: with more pages than top, sink and recent do not meet)
+    select_and_emit<uint64_t>(pages, a.top - a.sink - a.recent, pages <= a.top, [&](int i) { return keys[i]; },
+                              [&](int i) { return i < a.sink || i >= pages - a.recent; },
+                              [&](int at, int i) { out[at] = i; }, sh);
     for (int i = n + threadIdx.x; i < a.top; i += kSelThreads) out[i] = -1;
 }
 
@@ -498,9 +685,26 @@ void launch_page_select(const ChosenLaunch& c, const void* bounds, int64_t sink,
     a.num_pages = static_cast<int>(c.num_pages); a.top = static_cast<int>(c.top);
     a.sink = static_cast<int>(sink); a.recent = static_cast<int>(recent);
     const unsigned units = static_cast<unsigned>(c.batch * c.rows * c.kv_heads);
-    const dim3 grid(units, static_cast<unsigned>(std::min<int64_t>((a.max_pages + 15) / 16, 1024)));
-    if (c.kv_dtype == SFG_F32) page_score_kernel<float><<<grid, 256, 0, stream>>>(a);
-    else page_score_kernel<uint16_t><<<grid, 256, 0, stream>>>(a);
+    const bool fast = (c.head_dim == 64 || c.head_dim == 128) && (reinterpret_cast<uintptr_t>(bounds) & 15) == 0;
+    // a wave takes 64 pages, fewer while that leaves CUs idle
+    a.pages_per_wave = 64;
+    while (a.pages_per_wave > 16 && units * ((a.max_pages + 4 * a.pages_per_wave - 1) / (4 * a.pages_per_wave)) < 512)
+        a.pages_per_wave /= 2;
+    const int64_t groups = (a.max_pages + 4 * a.pages_per_wave - 1) / (4 * a.pages_per_wave);
+    if (fast && groups <= 65535) {
+        const dim3 grid(units, static_cast<unsigned>(groups));
+        if (c.kv_dtype == SFG_F32) {
+            if (c.head_dim == 128) page_score_kernel<float, 128><<<grid, 256, 0, stream>>>(a);
+            else page_score_kernel<float, 64><<<grid, 256, 0, stream>>>(a);
+        } else {
+            if (c.head_dim == 128) page_score_kernel<uint16_t, 128><<<grid, 256, 0, stream>>>(a);
+            else page_score_kernel<uint16_t, 64><<<grid, 256, 0, stream>>>(a);
+        }
+    } else {
+        const dim3 grid(units, static_cast<unsigned>(std::min<int64_t>((a.max_pages + 15) / 16, 1024)));
+        if (c.kv_dtype == SFG_F32) page_score_any_kernel<float><<<grid, 256, 0, stream>>>(a);
+        else page_score_any_kernel<uint16_t><<<grid, 256, 0, stream>>>(a);
+    }
     page_select_kernel<<<units, kSelThreads, 0, stream>>>(a);
 }
 

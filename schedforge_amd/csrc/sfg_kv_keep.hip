@@ -10,6 +10,7 @@
 // Selections are exact: ties go to the lower index, and the page scores are summed
 // in 64 bits, so that which page is taken does not hang on an order of summation.
 #include <algorithm>
+#include <type_traits>
 
 #include "sfg_kernels.hpp"
 #include "sfg_paged.hpp"
@@ -72,135 +73,137 @@ __global__ __launch_bounds__(64) void page_bounds_kernel(BoundsArgs a) {
 }
 
 // ---------------------------------------------------------------- selection
-// One workgroup of 1024 threads selects among n keys, thread t holding kSelKeys
-// consecutive ones of each tile of 4096 in registers (the keys of more than one tile
-// are read again for every pass).
-constexpr int kSelThreads = 1024, kSelKeys = 4, kSelTile = kSelThreads * kSelKeys;
+// One workgroup of NT threads selects among n values in tiles of NT * K: wave w holds
+// 64 K consecutive ones, lane l those at l, l + 64, ... (loads coalesce, and a ballot
+// gives the order inside a wave).  Values of one tile stay in registers; those of more
+// are read again for each pass.
 constexpr int kSelBits = 11, kSelBins = 1 << kSelBits;
 constexpr int kSelFew = 64;
 
-template <typename Key>
+template <typename Key, int NT>
 struct SelShared {
     int hist[kSelBins];
-    int2 wave[kSelThreads / 64];
-    Key lo[kSelThreads / 64], hi[kSelThreads / 64];
+    int sum[NT / 64], equal[NT / 64];
+    Key ones[NT / 64], all[NT / 64];
     Key few[kSelFew];
     int bin, above, count, fill;
     Key found; int ties;
 };
 
-// Exclusive sums over the workgroup's threads; totals in `all`.
-template <typename Key>
-__device__ __forceinline__ int2 block_exclusive(int2 v, SelShared<Key>& sh, int2& all) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int2 x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int a = __shfl_up(x.x, o, 64), c = __shfl_up(x.y, o, 64);
-        if (lane >= o) {
-            x.x += a;
-            x.y += c;
-        }
-    }
-    __syncthreads();
-    if (lane == 63) sh.wave[wave] = x;
-    __syncthreads();
-    int2 before = make_int2(0, 0);
-    all = before;
-#pragma unroll
-    for (int w = 0; w < kSelThreads / 64; ++w) {
-        const int2 s = sh.wave[w];
-        if (w < wave) {
-            before.x += s.x;
-            before.y += s.y;
-        }
-        all.x += s.x;
-        all.y += s.y;
-    }
-    return make_int2(before.x + x.x - v.x, before.y + x.y - v.y);
+// Sum of the lanes up to this one, by DPP: row shifts, then the rows' totals broadcast.
+__device__ __forceinline__ int wave_inclusive(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr:1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15 to rows 1, 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast:31 to rows 2, 3
+    return x;
 }
+// OR over the wave, in every lane (an AND is the complement of the complements' OR).
+__device__ __forceinline__ uint32_t wave_or(uint32_t v) {
+    int x = static_cast<int>(v);
+    x |= __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
+    x |= __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x |= __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x |= __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x |= __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+    x |= __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(x, 63));
+}
+__device__ __forceinline__ uint64_t wave_or(uint64_t v) {
+    return static_cast<uint64_t>(wave_or(static_cast<uint32_t>(v))) |
+           (static_cast<uint64_t>(wave_or(static_cast<uint32_t>(v >> 32))) << 32);
+}
+__device__ __forceinline__ int bit_length(uint32_t v) { return v ? 32 - __clz(static_cast<int>(v)) : 0; }
+__device__ __forceinline__ int bit_length(uint64_t v) { return v ? 64 - __clzll(static_cast<long long>(v)) : 0; }
 
-// The need-th largest of n candidates (1 <= need <= n): every key above `key` is taken
-// and `ties` of those equal to it.  Radix selection below the bits that all keys share,
-// 11 bits a pass: the workgroup counts a digit of the keys that match the digits found
-// so far; the bin in which the count from above passes `need` is the next digit.  Once
-// that bin holds at most 64 keys, they are ranked against each other.
+// The need-th largest of the candidates (1 <= need <= their number): every key above
+// `key` is taken and `ties` of those equal to it.  Radix selection below the bits that
+// all keys share, 11 bits a pass: the workgroup counts a digit of the keys that match
+// the digits found so far; the bin in which the count from above passes `need` is the
+// next digit.  Once that bin holds at most 64 keys, one wave ranks them.
 // each(f): calls f(key) for every candidate key of this thread.
-template <typename Key, typename Each>
-__device__ __forceinline__ void select_threshold(Each each, int need, SelShared<Key>& sh, Key& key, int& ties) {
-    constexpr int kBits = sizeof(Key) * 8;
+template <typename Key, int NT, typename Each>
+__device__ __forceinline__ void select_threshold(Each each, int need, SelShared<Key, NT>& sh, Key& key, int& ties) {
+    constexpr int kBits = sizeof(Key) * 8, kWaves = NT / 64, kOwn = kSelBins / NT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    Key lo = ~Key(0), hi = 0;
-    each([&](Key k) {
-        lo = min(lo, k);
-        hi = max(hi, k);
+    Key ones = 0, zeros = 0;  // bits that are set, or clear, in some key
+    each([&](Key k) __attribute__((always_inline)) {
+        ones |= k;
+        zeros |= ~k;
     });
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        lo = min(lo, static_cast<Key>(__shfl_xor(lo, o, 64)));
-        hi = max(hi, static_cast<Key>(__shfl_xor(hi, o, 64)));
-    }
+    ones = wave_or(ones);
+    zeros = wave_or(zeros);
     if (lane == 0) {
-        sh.lo[wave] = lo;
-        sh.hi[wave] = hi;
+        sh.ones[wave] = ones;
+        sh.all[wave] = zeros;
     }
-    __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kSelThreads / 64; ++w) {
-        lo = min(lo, sh.lo[w]);
-        hi = max(hi, sh.hi[w]);
-    }
-    if (lo == hi) {
-        key = lo;
-        ties = need;
-        return;
+    for (int i = 0; i < kOwn; ++i) sh.hist[threadIdx.x + i * NT] = 0;
+    __syncthreads();
+    ones = zeros = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        ones |= sh.ones[w];
+        zeros |= sh.all[w];
     }
     // bits from `open` down are not known yet; keys that match agree with `key` above them
-    int open = kBits - (kBits == 64 ? __clzll(static_cast<long long>(lo ^ hi)) : __clz(static_cast<int>(lo ^ hi)));
-    key = open == kBits ? Key(0) : hi >> open;
+    int open = bit_length(static_cast<Key>(ones & zeros));
+    key = open == kBits ? Key(0) : ones >> open;
     while (open > 0) {
         const int width = min(kSelBits, open), shift = open - width;
-        for (int i = threadIdx.x; i < kSelBins; i += kSelThreads) sh.hist[i] = 0;
-        __syncthreads();
-        each([&](Key k) {
+        each([&](Key k) __attribute__((always_inline)) {
             if (open == kBits || (k >> open) == key) atomicAdd(&sh.hist[static_cast<int>(k >> shift) & ((1 << width) - 1)], 1);
         });
         __syncthreads();
-        // two bins a thread, counted from the top one
-        const int top = kSelBins - 1 - 2 * static_cast<int>(threadIdx.x);
-        const int c1 = sh.hist[top], c0 = sh.hist[top - 1];
-        int2 all;
-        const int above = block_exclusive(make_int2(c1 + c0, 0), sh, all).x;
-        if (above < need && need <= above + c1) {
-            sh.bin = top;
-            sh.above = above;
-            sh.count = c1;
-        } else if (above + c1 < need && need <= above + c1 + c0) {
-            sh.bin = top - 1;
-            sh.above = above + c1;
-            sh.count = c0;
+        // kOwn bins a thread, counted from the top one
+        const int top = kSelBins - 1 - kOwn * static_cast<int>(threadIdx.x);
+        int c[kOwn], mine = 0;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            c[i] = sh.hist[top - i];
+            mine += c[i];
         }
+        const int upto = wave_inclusive(mine);
+        if (lane == 63) sh.sum[wave] = upto;
         if (threadIdx.x == 0) sh.fill = 0;
+        __syncthreads();
+        int above = upto - mine;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) above += w < wave ? sh.sum[w] : 0;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            if (above < need && need <= above + c[i]) {
+                sh.bin = top - i;
+                sh.above = above;
+                sh.count = c[i];
+            }
+            above += c[i];
+            sh.hist[top - i] = 0;  // for the next pass
+        }
         __syncthreads();
         key = (key << width) | static_cast<Key>(sh.bin);
         need -= sh.above;
         open = shift;
-        if (open > 0 && sh.count <= kSelFew) {
-            each([&](Key k) {
+        const int count = sh.count;
+        if (open > 0 && count <= kSelFew) {
+            each([&](Key k) __attribute__((always_inline)) {
                 if ((k >> open) == key) sh.few[atomicAdd(&sh.fill, 1)] = k;
             });
             __syncthreads();
             // the key with fewer than `need` above it and at least `need` not below it
-            if (static_cast<int>(threadIdx.x) < sh.count) {
-                const Key mine = sh.few[threadIdx.x];
-                int above_me = 0, same = 0;
-                for (int i = 0; i < sh.count; ++i) {
-                    above_me += sh.few[i] > mine;
-                    same += sh.few[i] == mine;
+            if (wave == 0) {
+                const Key me = lane < count ? sh.few[lane] : Key(0);
+                int over = 0, same = 0;
+                for (int i = 0; i < count; ++i) {
+                    const Key k = sh.few[i];
+                    over += k > me;
+                    same += k == me;
                 }
-                if (above_me < need && need <= above_me + same) {
-                    sh.found = mine;
-                    sh.ties = need - above_me;
+                if (lane < count && over < need && need <= over + same) {
+                    sh.found = me;
+                    sh.ties = need - over;
                 }
             }
             __syncthreads();
@@ -212,63 +215,88 @@ __device__ __forceinline__ void select_threshold(Each each, int need, SelShared<
     ties = need;
 }
 
+__device__ __forceinline__ int lanes_below(uint64_t mask) {
+    return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+}
+
 // Emits, ascending, the indexes taken among [0, n): those with must(i), and of the
 // candidates (the others) the `need` largest keys, ties to the lower index.
-// load(i): the key of candidate i; emit(at, i).  Returns how many were taken.
-template <typename Key, typename Load, typename Must, typename Emit>
-__device__ __forceinline__ int select_and_emit(int n, int need, bool everything, Load load, Must must, Emit emit, SelShared<Key>& sh) {
-    const bool single = n <= kSelTile;
-    const int first = kSelKeys * static_cast<int>(threadIdx.x);
-    Key k[kSelKeys];
+// load(i): value i; to_key(value); emit(at, i, value).  A tile's values are all read
+// before anything of it is emitted.
+template <typename Key, int NT, int K, typename Load, typename ToKey, typename Must, typename Emit>
+__device__ __forceinline__ void select_and_emit(int n, int need, bool everything, Load load, ToKey to_key, Must must, Emit emit,
+                                                SelShared<Key, NT>& sh) {
+    constexpr int kTile = NT * K, kWaves = NT / 64;
+    const bool single = n <= kTile;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int first = wave * 64 * K + lane;
+    decltype(load(0)) v[K];
     auto read = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
-        for (int r = 0; r < kSelKeys; ++r) {
-            const int i = tile + first + r;
-            k[r] = i < n && !everything && !must(i) ? load(i) : Key(0);
+        for (int r = 0; r < K; ++r) {
+            const int i = tile + first + 64 * r;
+            v[r] = load(min(i, n - 1));
         }
     };
-    if (single) read(0);
+    if (n > 0 && single) read(0);
     Key key = 0;
     int ties = 0;
-    if (!everything && need > 0)
-        select_threshold<Key>([&](auto f) __attribute__((always_inline)) {
-            for (int tile = 0; tile < n; tile += kSelTile) {
+    const bool ranked = !everything && need > 0;
+    if (ranked)
+        select_threshold<Key, NT>([&](auto f) __attribute__((always_inline)) {
+            for (int tile = 0; tile < n; tile += kTile) {
                 if (!single) read(tile);
 #pragma unroll
-                for (int r = 0; r < kSelKeys; ++r) {
-                    const int i = tile + first + r;
-                    if (i < n && !must(i)) f(k[r]);
+                for (int r = 0; r < K; ++r) {
+                    const int i = tile + first + 64 * r;
+                    if (i < n && !must(i)) f(to_key(v[r]));
                 }
             }
         }, need, sh, key, ties);
     int written = 0, tied = 0;
-    for (int tile = 0; tile < n; tile += kSelTile) {
+    for (int tile = 0; tile < n; tile += kTile) {
         if (!single) read(tile);
-        int2 mine = make_int2(0, 0);  // taken for sure, equal to the threshold
-        uint32_t sure = 0, equal = 0;
+        uint64_t sure[K], equal[K];
+        int n_sure = 0, n_equal = 0;
 #pragma unroll
-        for (int r = 0; r < kSelKeys; ++r) {
-            const int i = tile + first + r;
-            if (i >= n) continue;
-            if (everything || must(i) || (need > 0 && k[r] > key)) sure |= 1u << r;
-            else if (need > 0 && k[r] == key) equal |= 1u << r;
+        for (int r = 0; r < K; ++r) {
+            const int i = tile + first + 64 * r;
+            const bool in = i < n, fixed = everything || must(i);
+            const Key k = to_key(v[r]);
+            sure[r] = __ballot(in && (fixed || (ranked && k > key)));
+            equal[r] = __ballot(in && !fixed && ranked && k == key);
+            n_sure += __popcll(sure[r]);
+            n_equal += __popcll(equal[r]);
         }
-        mine.x = __popc(sure);
-        mine.y = __popc(equal);
-        int2 all;
-        const int2 before = block_exclusive(mine, sh, all);
-        int at = written + before.x + min(tied + before.y, ties) - min(tied, ties);
-        int rank = tied + before.y;
+        __syncthreads();
+        if (lane == 0) {
+            sh.sum[wave] = n_sure;
+            sh.equal[wave] = n_equal;
+        }
+        __syncthreads();
+        int sure_before = 0, sure_all = 0, equal_before = 0, equal_all = 0;
 #pragma unroll
-        for (int r = 0; r < kSelKeys; ++r) {
-            const bool take = (sure >> r) & 1u || ((equal >> r) & 1u && rank < ties);
-            rank += (equal >> r) & 1u;
-            if (take) emit(at++, tile + first + r);
+        for (int w = 0; w < kWaves; ++w) {
+            const int s = sh.sum[w], e = sh.equal[w];
+            sure_before += w < wave ? s : 0;
+            equal_before += w < wave ? e : 0;
+            sure_all += s;
+            equal_all += e;
         }
-        written += all.x + min(tied + all.y, ties) - min(tied, ties);
-        tied += all.y;
+        int rank = tied + equal_before;
+        int at = written + sure_before + min(rank, ties) - min(tied, ties);
+#pragma unroll
+        for (int r = 0; r < K; ++r) {
+            const bool tie = (equal[r] >> lane) & 1u;
+            const bool take = ((sure[r] >> lane) & 1u) || (tie && rank + lanes_below(equal[r]) < ties);
+            const uint64_t taken = __ballot(take);
+            if (take) emit(at + lanes_below(taken), tile + first + 64 * r, v[r]);
+            at += __popcll(taken);
+            rank += __popcll(equal[r]);
+        }
+        written += sure_all + min(tied + equal_all, ties) - min(tied, ties);
+        tied += equal_all;
     }
-    return written;
 }
 
 struct TokenSelectArgs {
@@ -279,8 +307,9 @@ struct TokenSelectArgs {
 };
 
 // One workgroup per (sequence, kv head).
-__global__ __launch_bounds__(kSelThreads) void kv_select_kernel(TokenSelectArgs a) {
-    __shared__ SelShared<uint32_t> sh;
+template <int NT, int K>
+__global__ __launch_bounds__(NT) void kv_select_kernel(TokenSelectArgs a) {
+    __shared__ SelShared<uint32_t, NT> sh;
     const int b = blockIdx.x / a.kv_heads, h = blockIdx.x % a.kv_heads;
     const int len = a.seq_lens ? min(max(a.seq_lens[b], 0), a.max_len) : a.max_len;
     const int n = min(len, a.budget);
@@ -288,32 +317,21 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(TokenSelectArgs 
     float* kept = a.kept ? a.kept + static_cast<int64_t>(blockIdx.x) * a.ld : nullptr;
     int32_t* keep = a.keep + static_cast<int64_t>(blockIdx.x) * a.budget;
     if (h == 0 && threadIdx.x == 0) a.kept_lens[b] = n;
-    // tokens from `old` on are kept; of those before, `need` of the largest weight
+    // tokens from `old` on are kept; of those before, budget - recent of the largest weight
     const int old = max(len - a.recent, 0);
-    select_and_emit<uint32_t>(len, a.budget - a.recent, len <= a.budget,
-                              [&](int i) { return order_key(w[i]); }, [&](int i) { return i >= old; },
-                              [&](int at, int i) { keep[at] = i; }, sh);
-    for (int i = n + threadIdx.x; i < a.budget; i += kSelThreads) keep[i] = -1;
+    // (kept may be the weights themselves: a token's place in the list is at or before its
+    // position, so what a tile writes no later tile reads)
+    select_and_emit<uint32_t, NT, K>(
+        len, a.budget - a.recent, len <= a.budget, [&](int i) { return w[i]; }, [](float v) { return order_key(v); },
+        [&](int i) { return i >= old; },
+        [&](int at, int i, float v) {
+            keep[at] = i;
+            if (kept) kept[at] = v;
+        }, sh);
+    for (int i = n + threadIdx.x; i < a.budget; i += NT) keep[i] = -1;
     if (kept) {
-        // the weights in the list's order, a tile at a time: sources lie at or behind their
-        // destinations, and a tile is read whole before it is written
         __syncthreads();
-        for (int base = 0; base < n; base += kSelTile) {
-            float x[kSelKeys];
-#pragma unroll
-            for (int r = 0; r < kSelKeys; ++r) {
-                const int i = base + r * kSelThreads + static_cast<int>(threadIdx.x);
-                x[r] = i < n ? w[keep[i]] : 0.f;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int r = 0; r < kSelKeys; ++r) {
-                const int i = base + r * kSelThreads + static_cast<int>(threadIdx.x);
-                if (i < n) kept[i] = x[r];
-            }
-        }
-        __syncthreads();
-        for (int64_t i = n + threadIdx.x; i < a.ld; i += kSelThreads) kept[i] = 0.f;
+        for (int64_t i = n + threadIdx.x; i < a.ld; i += NT) kept[i] = 0.f;
     }
 }
 
@@ -453,18 +471,29 @@ __global__ __launch_bounds__(256) void page_score_kernel(PageScoreArgs a) {
     }
 }
 
-__global__ __launch_bounds__(kSelThreads) void page_select_kernel(PageScoreArgs a) {
-    __shared__ SelShared<uint64_t> sh;
+template <int NT, int K>
+__global__ __launch_bounds__(NT) void page_select_kernel(PageScoreArgs a) {
+    __shared__ SelShared<uint64_t, NT> sh;
     const int64_t unit = blockIdx.x;
     const int row = static_cast<int>(unit / a.kv_heads % a.rows), b = static_cast<int>(unit / a.kv_heads / a.rows);
     const int pages = row_pages(a, b, row), n = min(pages, a.top);
     const uint64_t* keys = a.keys + unit * a.max_pages;
     int32_t* out = a.selected + unit * a.top;
-    // (top >= sink + recent: with more pages than top, sink and recent do not meet)
-    select_and_emit<uint64_t>(pages, a.top - a.sink - a.recent, pages <= a.top, [&](int i) { return keys[i]; },
-                              [&](int i) { return i < a.sink || i >= pages - a.recent; },
-                              [&](int at, int i) { out[at] = i; }, sh);
-    for (int i = n + threadIdx.x; i < a.top; i += kSelThreads) out[i] = -1;
+    // (top >= sink + recent: with more pages than top, the first and the newest do not meet)
+    select_and_emit<uint64_t, NT, K>(
+        pages, a.top - a.sink - a.recent, pages <= a.top, [&](int i) { return keys[i]; }, [](uint64_t k) { return k; },
+        [&](int i) { return i < a.sink || i >= pages - a.recent; }, [&](int at, int i, uint64_t) { out[at] = i; }, sh);
+    for (int i = n + threadIdx.x; i < a.top; i += NT) out[i] = -1;
+}
+
+// Threads and values a thread for up to n values: four waves while they hold them all
+// (fewer waves pass their barriers sooner), else sixteen.
+template <typename Go>
+void by_size(int64_t n, Go go) {
+    if (n <= 512) go(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+    else if (n <= 2048) go(std::integral_constant<int, 256>{}, std::integral_constant<int, 8>{});
+    else if (n <= 4096) go(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 1024>{}, std::integral_constant<int, 16>{});
 }
 
 // ---------------------------------------------------------------- compaction
@@ -705,7 +734,9 @@ void launch_page_select(const ChosenLaunch& c, const void* bounds, int64_t sink,
         if (c.kv_dtype == SFG_F32) page_score_any_kernel<float><<<grid, 256, 0, stream>>>(a);
         else page_score_any_kernel<uint16_t><<<grid, 256, 0, stream>>>(a);
     }
-    page_select_kernel<<<units, kSelThreads, 0, stream>>>(a);
+    by_size(a.max_pages, [&](auto nt, auto k) {
+        page_select_kernel<decltype(nt)::value, decltype(k)::value><<<units, decltype(nt)::value, 0, stream>>>(a);
+    });
 }
 
 void launch_kv_select(const float* weights, int64_t ld, const int32_t* seq_lens, int64_t max_context, int64_t budget,
@@ -715,7 +746,10 @@ void launch_kv_select(const float* weights, int64_t ld, const int32_t* seq_lens,
     a.weights = weights; a.ld = ld; a.seq_lens = seq_lens; a.max_len = static_cast<int>(max_context);
     a.budget = static_cast<int>(budget); a.recent = static_cast<int>(recent);
     a.keep = keep; a.kept_lens = kept_lens; a.kept = kept_weights; a.kv_heads = static_cast<int>(kv_heads);
-    kv_select_kernel<<<static_cast<unsigned>(batch * kv_heads), kSelThreads, 0, stream>>>(a);
+    by_size(max_context, [&](auto nt, auto k) {
+        kv_select_kernel<decltype(nt)::value, decltype(k)::value>
+            <<<static_cast<unsigned>(batch * kv_heads), decltype(nt)::value, 0, stream>>>(a);
+    });
 }
 
 void launch_kv_compact(void* k_pool, void* v_pool, int pool_dtype, const int32_t* page_table, const int32_t* base,

@@ -85,8 +85,9 @@ int64_t walked(int mode, const sfg_paged_attn_args& a, int64_t top) {
 }
 
 sfg::ChosenPlan plan_of(int mode, const sfg_paged_attn_args& a, int64_t top) {
-    return sfg::plan_chosen(mode, a.batch, a.q_heads, a.kv_heads, a.rows, a.head_dim, a.page_tokens, walked(mode, a, top),
-                            a.kv_splits);
+    const bool bf16 = a.q_dtype == SFG_BF16 && a.kv_dtype == SFG_BF16 && a.out_dtype == SFG_BF16;
+    return sfg::plan_chosen(mode, bf16, a.batch, a.q_heads, a.kv_heads, a.rows, a.head_dim, a.page_tokens,
+                            walked(mode, a, top), a.kv_splits);
 }
 
 size_t page_keys_bytes(const sfg_paged_attn_args& a) {

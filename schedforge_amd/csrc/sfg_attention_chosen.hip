@@ -15,110 +15,11 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "sfg_kernels.hpp"
-#include "sfg_paged.hpp"
+#include "sfg_chosen.hpp"
 
 namespace sfg {
 
 namespace {
-
-struct ChosenArgs {
-    const void* q; int q_f32;               // [B][Hq][rows][D]
-    const void* k_pool; const void* v_pool;
-    const int32_t* page_table; const int32_t* seq_lens; int max_len;   // lengths are clamped to max_len
-    void* out; int out_f32;                 // [B][Hq][rows][D]
-    float* part_ml; float* part_acc;        // [unit column][split] of (m, l) and [D]
-    int q_heads, kv_heads, rows, head_dim, page_tokens, pages_per_seq, num_pages, splits;
-    float scale_log2;                       // scale * log2(e): scores are exponents of 2
-    const uint32_t* mask; int64_t mask_stride; int mask_words;   // tree
-    float* scores; int64_t scores_ld;       // weights: scaled scores [unit column][ld]
-    const int32_t* selected; int top;       // sparse: logical pages [unit][top], ascending, -1 behind
-};
-
-// A unit's columns, the tokens it walks and who sees them.
-template <int MODE>
-struct Unit {
-    int b, kvh, row;    // row: the selected pages' query row
-    int64_t id;         // (b, kvh) or (b, row, kvh) in order
-    int cols;           // query columns
-    int walk;           // tokens walked: logical tokens, or the selected pages' in list order
-    int total;          // logical tokens that exist
-    int all_see;        // tokens below this every column sees
-    const int32_t* list;
-};
-
-template <int MODE>
-__device__ __forceinline__ Unit<MODE> unit_of(const ChosenArgs& p, int b, int y) {
-    Unit<MODE> u;
-    const int G = p.q_heads / p.kv_heads;
-    const int len = p.seq_lens ? min(max(p.seq_lens[b], 0), p.max_len) : p.max_len;
-    u.b = b;
-    u.list = nullptr;
-    if constexpr (MODE == kChosenSparse) {
-        u.row = y / p.kv_heads;
-        u.kvh = y % p.kv_heads;
-        u.id = (static_cast<int64_t>(b) * p.rows + u.row) * p.kv_heads + u.kvh;
-        u.cols = G;
-        u.total = max(len - p.rows + u.row + 1, 0);
-        u.all_see = u.total;
-        u.list = p.selected + u.id * p.top;
-        // entries in use: the list is packed
-        const int pages = (u.total + p.page_tokens - 1) / p.page_tokens;
-        u.walk = min(p.top, pages) * p.page_tokens;
-    } else {
-        u.row = 0;
-        u.kvh = y;
-        u.id = static_cast<int64_t>(b) * p.kv_heads + y;
-        u.cols = p.rows * G;
-        if constexpr (MODE == kChosenTree) {
-            u.total = len + p.rows;
-            u.all_see = len;
-        } else {
-            u.total = len;
-            u.all_see = len - p.rows + 1;
-        }
-        u.walk = u.total;
-    }
-    return u;
-}
-
-// Query row and head of a unit's column.
-template <int MODE>
-__device__ __forceinline__ void column_of(const ChosenArgs& p, const Unit<MODE>& u, int col, int& row, int& head) {
-    const int G = p.q_heads / p.kv_heads;
-    row = MODE == kChosenSparse ? u.row : col / G;
-    head = u.kvh * G + (MODE == kChosenSparse ? col : col % G);
-}
-
-// Whether query row `row` sees logical token `tok` (< total).
-template <int MODE>
-__device__ __forceinline__ bool sees(const ChosenArgs& p, const Unit<MODE>& u, int row, int tok) {
-    if constexpr (MODE == kChosenTree) {
-        const int t = tok - u.all_see;  // all_see: the committed tokens
-        if (t < 0) return true;
-        return (p.mask[u.b * p.mask_stride + static_cast<int64_t>(row) * p.mask_words + (t >> 5)] >> (t & 31)) & 1u;
-    } else if constexpr (MODE == kChosenWeights) {
-        return tok < u.total - p.rows + row + 1;
-    } else {
-        return tok < u.total;
-    }
-}
-
-// The unit and column of a (unit column) slot, counted through all units.
-template <int MODE>
-__device__ __forceinline__ Unit<MODE> unit_of_slot(const ChosenArgs& p, int64_t slot, int& col) {
-    const int G = p.q_heads / p.kv_heads;
-    const int per_unit = MODE == kChosenSparse ? G : p.rows * G;
-    const int per_b = MODE == kChosenSparse ? p.rows * p.kv_heads : p.kv_heads;
-    const int64_t uid = slot / per_unit;
-    col = static_cast<int>(slot % per_unit);
-    return unit_of<MODE>(p, static_cast<int>(uid / per_b), static_cast<int>(uid % per_b));
-}
-
-// Element offset of column (row, head) of q and out.
-__device__ __forceinline__ int64_t column_offset(const ChosenArgs& p, int b, int row, int head) {
-    return ((static_cast<int64_t>(b) * p.q_heads + head) * p.rows + row) * p.head_dim;
-}
 
 // ===========================================================================
 // Any head_dim up to kRowMaxD, any page size, any alignment: one wave per
@@ -211,9 +112,6 @@ __global__ __launch_bounds__(64) void chosen_any_kernel(ChosenArgs p) {
         if (d < D) p.part_acc[part * D + d] = acc[r];
     }
 }
-
-// A split's weight; one without a maximum enters as it is (0, or NaN where a score was NaN).
-__device__ __forceinline__ float split_weight(float m, float M) { return m == -INFINITY ? 1.f : fast_exp2(m - M); }
 
 // ===========================================================================
 // head_dim 64 / 128 and 16-token pages on the matrix cores.  A workgroup owns 16
@@ -638,6 +536,7 @@ __global__ __launch_bounds__(256) void chosen_weights_kernel(ChosenArgs p, float
     for (int c = blockIdx.y; c < u.cols; c += gridDim.y) merge_column<kChosenWeights>(p, u, c, threadIdx.x, 256);
 }
 
+constexpr int64_t kTreeTileCols = 32;    // more columns than these run the tree's tile kernel
 constexpr int64_t kMaxGroups = 1 << 23;  // workgroups of 256 threads in a launch
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
@@ -655,11 +554,12 @@ void launch_mode(const ChosenLaunch& a, const ChosenArgs& p, const ChosenPlan& p
     const unsigned columns = static_cast<unsigned>(a.batch * a.rows * a.q_heads);
     const int64_t units = a.batch * a.kv_heads * (MODE == kChosenSparse ? a.rows : 1);
     const int64_t chunks = (columns / units + 15) / 16;
-    // Q, K and (fp32) V are read as 16-byte vectors, bf16 V as 8-byte ones; rows of 64 or
-    // 128 elements keep a base's boundary
-    const bool aligned = ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k_pool)) & 15) == 0 &&
-                         (reinterpret_cast<uintptr_t>(a.v_pool) & (a.kv_dtype == SFG_F32 ? 15 : 7)) == 0;
-    if (plan.mfma && aligned && units * chunks * plan.splits <= kMaxGroups) {
+    // Q, K and V are read as 16-byte vectors; rows of 64 or 128 elements keep a base's boundary
+    const bool aligned = ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k_pool) | reinterpret_cast<uintptr_t>(a.v_pool)) & 15) == 0;
+    const TreeTiles tiles = tree_tiles(columns / units);
+    if (plan.tiles && aligned && units * tiles.chunks * plan.splits <= kMaxGroups) {
+        launch_tree_tiles(p, tiles, units, stream);
+    } else if (plan.mfma && aligned && units * chunks * plan.splits <= kMaxGroups) {
         const unsigned grid = static_cast<unsigned>(units * chunks * plan.splits);
         if (a.head_dim == 128) launch_mfma<MODE, 128>(a, p, grid, static_cast<int>(chunks), stream);
         else launch_mfma<MODE, 64>(a, p, grid, static_cast<int>(chunks), stream);
@@ -676,18 +576,23 @@ void launch_mode(const ChosenLaunch& a, const ChosenArgs& p, const ChosenPlan& p
 
 }  // namespace
 
-ChosenPlan plan_chosen(int mode, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t rows, int64_t head_dim,
+ChosenPlan plan_chosen(int mode, bool bf16, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t rows, int64_t head_dim,
                        int64_t page_tokens, int64_t keys, int32_t requested) {
     ChosenPlan plan{};
     const int64_t columns = batch * rows * q_heads;
     plan.mfma = (head_dim == 64 || head_dim == 128) && page_tokens == kPageTok;
     const int64_t units = batch * kv_heads * (mode == kChosenSparse ? rows : 1);
-    const int64_t base = plan.mfma ? units * ((columns / units + 15) / 16) : columns;
+    const int64_t cols = columns / units;
+    plan.tiles = mode == kChosenTree && plan.mfma && bf16 && cols > kTreeTileCols;
+    const int64_t base = plan.tiles ? units * tree_tiles(cols).chunks : plan.mfma ? units * ((cols + 15) / 16) : columns;
     const int64_t most = plan.mfma ? (keys + kPageTok - 1) / kPageTok : keys;
     int64_t s = 1;
     if (requested > 0) s = std::min<int64_t>(requested, std::max<int64_t>(most, 1));
     // matrix cores: two workgroups per CU while a split keeps 8 pages (two per wave);
     // else >= 1024 waves while a split keeps >= 256 tokens
+    else if (plan.tiles)
+        // tiles of 64 tokens: two workgroups per CU while a split keeps 4
+        while (base * s < 512 && most / (s * 2) >= 16) s *= 2;
     else
         while (base * s < (plan.mfma ? 512 : 1024) && most / (s * 2) >= (plan.mfma ? 8 : 256)) s *= 2;
     plan.splits = static_cast<int>(std::min<int64_t>(s, 65535));

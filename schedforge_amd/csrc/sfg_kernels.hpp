@@ -165,12 +165,14 @@ struct ChosenLaunch {
 // for the weights the scaled scores.
 struct ChosenPlan {
     int splits;
-    bool mfma;                                      // the matrix-core kernel's head_dim and page size
+    bool mfma;                                      // the matrix-core kernels' head_dim and page size
+    bool tiles;                                     // the tree's tile kernel
     size_t ml_bytes, acc_bytes, scores_bytes;
     int64_t scores_ld;
     size_t bytes() const { return ml_bytes + acc_bytes + scores_bytes; }
 };
-ChosenPlan plan_chosen(int mode, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t rows, int64_t head_dim,
+// bf16: queries, pools and output all are.
+ChosenPlan plan_chosen(int mode, bool bf16, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t rows, int64_t head_dim,
                        int64_t page_tokens, int64_t keys, int32_t requested);
 void launch_chosen(const ChosenLaunch& a, const ChosenPlan& plan, void* workspace, hipStream_t stream);
 

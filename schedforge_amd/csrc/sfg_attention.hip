@@ -1800,6 +1800,56 @@ __global__ __launch_bounds__(64) void kv_append_kernel(KvAppendArgs a) {
         vdst[static_cast<int64_t>(d) * pt] = to_pool<KvT>(load_src(a.values, a.src_f32, src + d));
 }
 
+// Several tokens without RoPE into 16-token pages: a workgroup per (sequence, kv head)
+// and page that the call touches.  A wave of the kernel above stores one token's values
+// two bytes at a time into 32-byte runs that other compute units' waves share (64 x 8
+// heads x 64 tokens at D 128: 22 us); here a thread gathers a dim's tokens of the page
+// and stores the run, whole where the call covers it.
+template <typename KvT, typename SrcT>
+__global__ __launch_bounds__(256) void kv_append_pages_kernel(KvAppendArgs a, int tokens) {
+    const int h = blockIdx.x % a.kv_heads, b = blockIdx.x / a.kv_heads;
+    const int D = a.head_dim;
+    const int64_t start = a.seq_lens ? a.seq_lens[b] : a.start;  // (a length may be anything)
+    const int64_t lp = (start >> 4) + static_cast<int64_t>(blockIdx.y);
+    if (lp < 0 || lp >= a.pages_per_seq) return;
+    const int phys = a.page_table[static_cast<int64_t>(b) * a.pages_per_seq + lp];
+    if (phys < 0 || phys >= a.num_pages) return;
+    const int t0 = static_cast<int>(lp * kPageTok - start);   // call token of the page's first slot
+    const int lo = max(-t0, 0), hi = min(kPageTok, tokens - t0);  // slots written
+    if (lo >= hi) return;
+    const int64_t src = b * a.sb + h * a.sh;
+    const int64_t blk = static_cast<int64_t>(phys) * a.kv_heads + h;
+    const SrcT* ks = static_cast<const SrcT*>(a.keys) + src;
+    const SrcT* vs = static_cast<const SrcT*>(a.values) + src;
+    KvT* kdst = static_cast<KvT*>(a.k_pool) + blk * kPageTok * D;
+    KvT* vdst = static_cast<KvT*>(a.v_pool) + blk * D * kPageTok;
+    auto load = [](const SrcT* p) {
+        if constexpr (sizeof(KvT) == sizeof(SrcT)) return *p;
+        else if constexpr (sizeof(SrcT) == 4) return f32_to_bf16(*p);
+        else return bf16_to_f32(*p);
+    };
+    for (int e = threadIdx.x; e < (hi - lo) * D; e += 256) {
+        const int t = lo + e / D, d = e % D;
+        kdst[t * D + d] = load(ks + (t0 + t) * a.st + d);
+    }
+    for (int d = threadIdx.x; d < D; d += 256) {
+        KvT v[kPageTok];
+#pragma unroll
+        for (int t = 0; t < kPageTok; ++t) v[t] = load(vs + (t0 + min(max(t, lo), hi - 1)) * a.st + d);
+        if (lo == 0 && hi == kPageTok) {
+            constexpr int kRun = kPageTok * sizeof(KvT) / 16;
+            uint4 w[kRun];
+            __builtin_memcpy(w, v, sizeof w);
+#pragma unroll
+            for (int i = 0; i < kRun; ++i) reinterpret_cast<uint4*>(vdst + static_cast<int64_t>(d) * kPageTok)[i] = w[i];
+        } else {
+#pragma unroll
+            for (int t = 0; t < kPageTok; ++t)
+                if (t >= lo && t < hi) vdst[static_cast<int64_t>(d) * kPageTok + t] = v[t];
+        }
+    }
+}
+
 // Lengths advance by the appended tokens and saturate at the capacity: tokens
 // past it were not written (kv_append_kernel skips them), so they are not
 // counted either.
@@ -1850,7 +1900,19 @@ int launch_kv_append(const void* keys, const void* values, int src_dtype, int64_
     a.page_tokens = static_cast<int>(page_tokens); a.pages_per_seq = static_cast<int>(pages_per_seq);
     a.num_pages = static_cast<int>(num_pages);
     const dim3 grid(static_cast<unsigned>(tokens), static_cast<unsigned>(kv_heads), static_cast<unsigned>(batch));
-    if (pool_dtype == SFG_F32) kv_append_kernel<float><<<grid, 64, 0, stream>>>(a);
+    const int64_t spans = (tokens + 2 * kPageTok - 2) / kPageTok;  // pages that a run of tokens can touch
+    if (!rope && tokens > 1 && page_tokens == kPageTok && spans <= 65535 &&
+        (reinterpret_cast<uintptr_t>(v_pool) & 15) == 0) {
+        const dim3 pgrid(static_cast<unsigned>(batch * kv_heads), static_cast<unsigned>(spans));
+        const int n = static_cast<int>(tokens);
+        if (pool_dtype == SFG_F32) {
+            if (a.src_f32) kv_append_pages_kernel<float, float><<<pgrid, 256, 0, stream>>>(a, n);
+            else kv_append_pages_kernel<float, uint16_t><<<pgrid, 256, 0, stream>>>(a, n);
+        } else {
+            if (a.src_f32) kv_append_pages_kernel<uint16_t, float><<<pgrid, 256, 0, stream>>>(a, n);
+            else kv_append_pages_kernel<uint16_t, uint16_t><<<pgrid, 256, 0, stream>>>(a, n);
+        }
+    } else if (pool_dtype == SFG_F32) kv_append_kernel<float><<<grid, 64, 0, stream>>>(a);
     else kv_append_kernel<uint16_t><<<grid, 64, 0, stream>>>(a);
     if (advance && seq_lens)
         kv_advance_kernel<<<dim3(static_cast<unsigned>((batch + 255) / 256)), 256, 0, stream>>>(

@@ -454,86 +454,148 @@ __global__ __launch_bounds__(256, sizeof(KvT) == 4 ? 1 : 2) void chosen_mfma_ker
 // ===========================================================================
 // The splits of a column merged: weights 2^(m_s - M), output sum / L.
 // ===========================================================================
-// A column's maximum and sum over its splits, by the whole wave.
-__device__ __forceinline__ void merge_ml(const float* ml, int splits, int lane, float& M, float& L) {
-    float m = -INFINITY;
-    for (int s = lane; s < splits; s += 64) m = fmaxf(m, ml[2 * s]);
-    M = wave_max(m);
-    float l = 0.f;
-    for (int s = lane; s < splits; s += 64) l = fmaf(ml[2 * s + 1], split_weight(ml[2 * s], M), l);
-    L = wave_sum(l);
-}
-
-// By `lanes` threads (whole waves), thread t the dims t, t + lanes, ...
-template <int MODE>
-__device__ __forceinline__ void merge_column(const ChosenArgs& p, const Unit<MODE>& u, int col, int t, int lanes) {
+// One wave a column.  kV: dims a lane holds side by side (head_dim 64 kV), 0: any head_dim.
+template <int MODE, int kV>
+__device__ __forceinline__ void merge_dims(const ChosenArgs& p, const Unit<MODE>& u, int col, int lane) {
+    constexpr int kW = kV ? kV : 1;
     const int64_t slot = u.id * u.cols + col;
-    const float* ml = p.part_ml + 2 * slot * p.splits;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot * p.splits;
     const float* pa = p.part_acc + slot * p.splits * p.head_dim;
-    float M, L;
-    merge_ml(ml, p.splits, t & 63, M, L);
     int row, head;
     column_of<MODE>(p, u, col, row, head);
     const int64_t o0 = column_offset(p, u.b, row, head);
     // eight splits at a time, their loads all issued before the ordered sum (slots past
     // the count re-read the last split and are left out)
     constexpr int kBatch = 8;
-    for (int d = t; d < p.head_dim; d += lanes) {
-        float o = 0.f;
+    for (int d = lane * kW; d < p.head_dim; d += 64 * kW) {
+        float M = -INFINITY, L = 0.f, o[kW];
+#pragma unroll
+        for (int i = 0; i < kW; ++i) o[i] = 0.f;
         for (int s0 = 0; s0 < p.splits; s0 += kBatch) {
-            float ms[kBatch], av[kBatch];
+            float2 x[kBatch];
+            float av[kBatch][kW];
 #pragma unroll
             for (int e = 0; e < kBatch; ++e) {
                 const int64_t sc = min(s0 + e, p.splits - 1);
-                ms[e] = ml[2 * sc];
-                av[e] = pa[sc * p.head_dim + d];
+                x[e] = ml[sc];
+                const float* at = pa + sc * p.head_dim + d;
+                if constexpr (kV == 2) {
+                    const float2 v = *reinterpret_cast<const float2*>(at);
+                    av[e][0] = v.x;
+                    av[e][kW - 1] = v.y;
+                } else {
+                    av[e][0] = *at;
+                }
             }
+            float m = M;
 #pragma unroll
-            for (int e = 0; e < kBatch; ++e)
-                if (s0 + e < p.splits) o = fmaf(split_weight(ms[e], M), av[e], o);
+            for (int e = 0; e < kBatch; ++e) m = fmaxf(m, x[e].x);
+            const float f = split_weight(M, m);
+            L *= f;
+#pragma unroll
+            for (int i = 0; i < kW; ++i) o[i] *= f;
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+                if (s0 + e >= p.splits) continue;
+                const float w = split_weight(x[e].x, m);
+                L = fmaf(x[e].y, w, L);
+#pragma unroll
+                for (int i = 0; i < kW; ++i) o[i] = fmaf(w, av[e][i], o[i]);
+            }
+            M = m;
         }
-        const float v = o / L;  // nothing visible: 0 / 0
-        if (p.out_f32) static_cast<float*>(p.out)[o0 + d] = v;
-        else static_cast<uint16_t*>(p.out)[o0 + d] = f32_to_bf16(v);
+#pragma unroll
+        for (int i = 0; i < kW; ++i) {
+            const float v = o[i] / L;  // nothing visible: 0 / 0
+            if (p.out_f32) static_cast<float*>(p.out)[o0 + d + i] = v;
+            else static_cast<uint16_t*>(p.out)[o0 + d + i] = f32_to_bf16(v);
+        }
     }
 }
 
 template <int MODE>
-__global__ __launch_bounds__(128) void chosen_combine_kernel(ChosenArgs p) {
-    int col;
-    const Unit<MODE> u = unit_of_slot<MODE>(p, blockIdx.x, col);
-    merge_column<MODE>(p, u, col, threadIdx.x, blockDim.x);
+__device__ __forceinline__ void merge_column(const ChosenArgs& p, const Unit<MODE>& u, int col, int lane) {
+    if (p.head_dim == 128) merge_dims<MODE, 2>(p, u, col, lane);
+    else merge_dims<MODE, 0>(p, u, col, lane);
 }
 
-// The weights' end: every workgroup merges the columns' (m, l) of its (sequence,
-// kv head), adds sum_columns 2^(s - M) / L to its 256 tokens' accumulators, and
-// takes its share of the output columns.  A column that sees nothing adds nothing.
-__global__ __launch_bounds__(256) void chosen_weights_kernel(ChosenArgs p, float* weights, int64_t ld) {
-    constexpr int kCols = 64;
-    __shared__ float sM[kCols], sR[kCols];
+// Four columns a workgroup, one a wave.
+template <int MODE>
+__global__ __launch_bounds__(256) void chosen_combine_kernel(ChosenArgs p, int columns) {
+    const int slot = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (slot >= columns) return;
+    int col;
+    const Unit<MODE> u = unit_of_slot<MODE>(p, slot, col);
+    merge_column<MODE>(p, u, col, threadIdx.x & 63);
+}
+
+// The weights' end, one wave per 256 tokens of a (sequence, kv head): lane c merges
+// (m, l) of column c, 64 columns at a time; the wave adds sum_columns 2^(s - M) / L to
+// its tokens' accumulators and takes its share of the output columns.  A column that
+// sees nothing adds nothing.  Latency, not bytes, bounds it (4 G bytes of scores and 8
+// of accumulator a token): the first columns' scores are loaded before (m, l).
+__global__ __launch_bounds__(64) void chosen_weights_kernel(ChosenArgs p, float* weights, int64_t ld) {
+    constexpr int kTok = 4, kEarly = 4, kBatch = 8;  // tokens a lane, columns loaded early, splits a batch
     const Unit<kChosenWeights> u = unit_of<kChosenWeights>(p, blockIdx.x / p.kv_heads, blockIdx.x % p.kv_heads);
-    const int tok = blockIdx.y * 256 + threadIdx.x;
-    float sum = 0.f;
-    for (int c0 = 0; c0 < u.cols; c0 += kCols) {
-        const int n = min(kCols, u.cols - c0);
-        __syncthreads();
-        for (int c = threadIdx.x >> 6; c < n; c += 4) {
-            float M, L;
-            merge_ml(p.part_ml + 2 * (u.id * u.cols + c0 + c) * p.splits, p.splits, threadIdx.x & 63, M, L);
-            if ((threadIdx.x & 63) == 0) {
-                sM[c] = M;
-                sR[c] = L == 0.f ? 0.f : 1.f / L;
+    const int lane = threadIdx.x, tok0 = blockIdx.y * 256 + lane;
+    const float* scores = p.scores + u.id * u.cols * p.scores_ld;
+    if (static_cast<int>(blockIdx.y) * 256 < u.total) {
+        int at[kTok];
+        float early[kEarly][kTok], sum[kTok], was[kTok];
+#pragma unroll
+        for (int t = 0; t < kTok; ++t) {
+            at[t] = min(tok0 + 64 * t, u.total - 1);
+            sum[t] = 0.f;
+            was[t] = weights[u.id * ld + at[t]];
+        }
+#pragma unroll
+        for (int c = 0; c < kEarly; ++c)
+#pragma unroll
+            for (int t = 0; t < kTok; ++t) early[c][t] = scores[min(c, u.cols - 1) * p.scores_ld + at[t]];
+        for (int c0 = 0; c0 < u.cols; c0 += 64) {
+            const int n = min(64, u.cols - c0);
+            const float* ml = p.part_ml + 2 * (u.id * u.cols + c0 + min(lane, n - 1)) * p.splits;
+            float M = -INFINITY, L = 0.f;
+            for (int s0 = 0; s0 < p.splits; s0 += kBatch) {
+                float2 x[kBatch];
+#pragma unroll
+                for (int e = 0; e < kBatch; ++e) x[e] = reinterpret_cast<const float2*>(ml)[min(s0 + e, p.splits - 1)];
+                float m = M;
+#pragma unroll
+                for (int e = 0; e < kBatch; ++e) m = fmaxf(m, x[e].x);
+                L *= split_weight(M, m);
+#pragma unroll
+                for (int e = 0; e < kBatch; ++e)
+                    if (s0 + e < p.splits) L = fmaf(x[e].y, split_weight(x[e].x, m), L);
+                M = m;
+            }
+            const float R = L == 0.f ? 0.f : 1.f / L;
+            auto add = [&](int c, const float* s) __attribute__((always_inline)) {
+                const float m = lane_bcast(M, c), r = lane_bcast(R, c);
+#pragma unroll
+                for (int t = 0; t < kTok; ++t)
+                    if (s[t] != -INFINITY) sum[t] = fmaf(fast_exp2(s[t] - m), r, sum[t]);
+            };
+            int c = 0;
+            if (c0 == 0)
+#pragma unroll
+                for (int e = 0; e < kEarly; ++e)
+                    if (e < n) {
+                        add(e, early[e]);
+                        c = e + 1;
+                    }
+            for (; c < n; ++c) {
+                float s[kTok];
+#pragma unroll
+                for (int t = 0; t < kTok; ++t) s[t] = scores[(c0 + c) * p.scores_ld + at[t]];
+                add(c, s);
             }
         }
-        __syncthreads();
-        if (tok < u.total)
-            for (int c = 0; c < n; ++c) {
-                const float s = p.scores[(u.id * u.cols + c0 + c) * p.scores_ld + tok];
-                if (s != -INFINITY) sum = fmaf(fast_exp2(s - sM[c]), sR[c], sum);
-            }
+#pragma unroll
+        for (int t = 0; t < kTok; ++t)
+            if (tok0 + 64 * t < u.total) weights[u.id * ld + at[t]] = was[t] + sum[t];
     }
-    if (tok < u.total) weights[u.id * ld + tok] += sum;
-    for (int c = blockIdx.y; c < u.cols; c += gridDim.y) merge_column<kChosenWeights>(p, u, c, threadIdx.x, 256);
+    for (int c = blockIdx.y; c < u.cols; c += gridDim.y) merge_column<kChosenWeights>(p, u, c, lane);
 }
 
 constexpr int64_t kTreeTileCols = 32;    // more columns than these run the tree's tile kernel
@@ -570,8 +632,8 @@ void launch_mode(const ChosenLaunch& a, const ChosenArgs& p, const ChosenPlan& p
     }
     if constexpr (MODE == kChosenWeights)
         chosen_weights_kernel<<<dim3(static_cast<unsigned>(a.batch * a.kv_heads), static_cast<unsigned>((a.max_context + 255) / 256)),
-                                256, 0, stream>>>(p, a.weights, a.weights_ld);
-    else if (plan.splits > 1) chosen_combine_kernel<MODE><<<columns, a.head_dim > 64 ? 128 : 64, 0, stream>>>(p);
+                                64, 0, stream>>>(p, a.weights, a.weights_ld);
+    else if (plan.splits > 1) chosen_combine_kernel<MODE><<<(columns + 3) / 4, 256, 0, stream>>>(p, static_cast<int>(columns));
 }
 
 }  // namespace

@@ -39,10 +39,10 @@ struct BoundsArgs {
     int kv_heads, head_dim, page_tokens, pages_per_seq, num_pages;
 };
 
-// One wave per (sequence, kv head) and page, from the newest page back, lane d owning
+// Any head_dim and page size: one wave per (sequence, kv head) and page, from the newest page back, lane d owning
 // dims d, d + 64, ...; a page is read whole, up to the sequence's end.
 template <typename KvT>
-__global__ __launch_bounds__(64) void page_bounds_kernel(BoundsArgs a) {
+__global__ __launch_bounds__(64) void page_bounds_any_kernel(BoundsArgs a) {
     const int b = blockIdx.x / a.kv_heads, h = blockIdx.x % a.kv_heads;
     const int pt = a.page_tokens, D = a.head_dim;
     const int len = a.seq_lens ? min(max(a.seq_lens[b], 0), a.max_len) : a.max_len;
@@ -68,6 +68,69 @@ __global__ __launch_bounds__(64) void page_bounds_kernel(BoundsArgs a) {
                 out[d] = f32_to_bf16(lo);
                 out[D + d] = f32_to_bf16(hi);
             }
+        }
+    }
+}
+
+// head_dim 64 / 128, 16-token pages: a row is read as 16-byte vectors, 64 of them a load of
+// the wave, all of the page's loads before the first comparison (slots past the end
+// re-read the last token); lanes of the same vector and other tokens meet by shuffles.
+template <typename KvT, int kD>
+__global__ __launch_bounds__(64) void page_bounds_kernel(BoundsArgs a) {
+    constexpr int kEl = 16 / sizeof(KvT), kVecs = kD / kEl, kTok = 64 / kVecs, kLoads = kPageTok / kTok;
+    const int b = blockIdx.x / a.kv_heads, h = blockIdx.x % a.kv_heads;
+    const int len = a.seq_lens ? min(max(a.seq_lens[b], 0), a.max_len) : a.max_len;
+    const int lane = threadIdx.x, vec = lane % kVecs, tok = lane / kVecs;
+    for (int page = (len + kPageTok - 1) / kPageTok - 1 - static_cast<int>(blockIdx.y);
+         page >= 0 && static_cast<int64_t>(page + 1) * kPageTok > len - a.fresh; page -= static_cast<int>(gridDim.y)) {
+        const int id = a.page_table[static_cast<int64_t>(b) * a.pages_per_seq + page];
+        if (id < 0 || id >= a.num_pages) continue;
+        const int last = min(kPageTok, len - page * kPageTok) - 1;
+        const int64_t blk = static_cast<int64_t>(id) * a.kv_heads + h;
+        const uint4* k = reinterpret_cast<const uint4*>(static_cast<const KvT*>(a.k_pool) + blk * kPageTok * kD);
+        uint4 w[kLoads];
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) w[i] = k[min(kTok * i + tok, last) * kVecs + vec];
+        float lo[kEl], hi[kEl];
+#pragma unroll
+        for (int e = 0; e < kEl; ++e) {
+            lo[e] = INFINITY;
+            hi[e] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            KvT v[kEl];
+            __builtin_memcpy(v, &w[i], sizeof v);
+#pragma unroll
+            for (int e = 0; e < kEl; ++e) {
+                lo[e] = fminf(lo[e], kv_f32(v, e));
+                hi[e] = fmaxf(hi[e], kv_f32(v, e));
+            }
+        }
+#pragma unroll
+        for (int o = kVecs; o < 64; o <<= 1)
+#pragma unroll
+            for (int e = 0; e < kEl; ++e) {
+                lo[e] = fminf(lo[e], __shfl_xor(lo[e], o, 64));
+                hi[e] = fmaxf(hi[e], __shfl_xor(hi[e], o, 64));
+            }
+        if (tok == 0) {
+            KvT v[2][kEl];
+#pragma unroll
+            for (int e = 0; e < kEl; ++e) {
+                if constexpr (sizeof(KvT) == 4) {
+                    v[0][e] = lo[e];
+                    v[1][e] = hi[e];
+                } else {  // values of the pool: exact
+                    v[0][e] = f32_to_bf16(lo[e]);
+                    v[1][e] = f32_to_bf16(hi[e]);
+                }
+            }
+            uint4* out = reinterpret_cast<uint4*>(static_cast<KvT*>(a.bounds) + blk * 2 * kD);
+            uint4 x[2];
+            __builtin_memcpy(x, v, sizeof x);
+            out[vec] = x[0];
+            out[kVecs + vec] = x[1];
         }
     }
 }
@@ -693,8 +756,19 @@ void launch_page_bounds(const void* k_pool, int pool_dtype, const int32_t* page_
     const int64_t newest = std::min(fresh, max_context);
     const int64_t pages = std::min((max_context + page_tokens - 1) / page_tokens, (newest + page_tokens - 2) / page_tokens + 1);
     const dim3 grid(static_cast<unsigned>(batch * kv_heads), static_cast<unsigned>(std::min<int64_t>(pages, 65535)));
-    if (pool_dtype == SFG_F32) page_bounds_kernel<float><<<grid, 64, 0, stream>>>(a);
-    else page_bounds_kernel<uint16_t><<<grid, 64, 0, stream>>>(a);
+    const bool fast = (head_dim == 64 || head_dim == 128) && page_tokens == kPageTok &&
+                      ((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(bounds)) & 15) == 0;
+    if (fast && pool_dtype == SFG_F32) {
+        if (head_dim == 128) page_bounds_kernel<float, 128><<<grid, 64, 0, stream>>>(a);
+        else page_bounds_kernel<float, 64><<<grid, 64, 0, stream>>>(a);
+    } else if (fast) {
+        if (head_dim == 128) page_bounds_kernel<uint16_t, 128><<<grid, 64, 0, stream>>>(a);
+        else page_bounds_kernel<uint16_t, 64><<<grid, 64, 0, stream>>>(a);
+    } else if (pool_dtype == SFG_F32) {
+        page_bounds_any_kernel<float><<<grid, 64, 0, stream>>>(a);
+    } else {
+        page_bounds_any_kernel<uint16_t><<<grid, 64, 0, stream>>>(a);
+    }
 }
 
 size_t page_select_workspace_bytes(int64_t batch, int64_t kv_heads, int64_t rows, int64_t max_pages) {

@@ -529,3 +529,34 @@ def test_two_streams_with_workspaces_of_their_own():
     torch.cuda.synchronize()
     for o, w in zip(outs, alone):
         assert torch.equal(o.view(torch.int16), w.view(torch.int16))
+
+
+@pytest.mark.parametrize("src", ["bf16", "f32"])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [128, 24])
+def test_several_tokens_appended_by_pages(d, dtype, src):
+    """Runs of tokens that start and end inside pages, at lengths of their own (a negative and a full one
+    among them); slots that the call does not cover and tokens past the capacity are not written."""
+    lib = _abi.load()
+    rng = np.random.default_rng(d)
+    for tokens in (2, 15, 16, 17, 40):
+        starts = np.array([0, 5, 16, 31, 64, 80, -3, 79], np.int32)
+        c = Cache(rng, starts, 80, 3, d, 16, dtype, poison=False).upload(starts)
+        table = c.table.copy()
+        table[1, 1] = -1
+        c.td = dev(table)
+        k, v = (rng.standard_normal((8, 3, tokens, d)).astype(np.float32) for _ in range(2))
+        if src == "bf16":
+            k, v = oracle.round_bf16(k), oracle.round_bf16(v)
+        to = (lambda x: dev(oracle.to_bf16_bits(x).view(np.int16))) if src == "bf16" else dev
+        _abi.check(lib.sfg_hip_kv_append_pool_v1(
+            to(k).data_ptr(), to(v).data_ptr(), BF16 if src == "bf16" else F32, c.kd.data_ptr(), c.vd.data_ptr(),
+            BF16 if dtype == "bf16" else F32, c.td.data_ptr(), c.ld.data_ptr(), 0, 0, 8, 3, tokens, d, 16, c.per, c.pages, stream()))
+        for got, was, new in zip(c.logical(c.kd, c.vd), (c.k, c.v), (k, v)):
+            want = was.copy()
+            for n in range(8):
+                for t in range(tokens):
+                    at = starts[n] + t
+                    if 0 <= at < 80 and table[n, at // 16] >= 0:
+                        want[n, :, at] = c.round(new[n, :, t])
+            np.testing.assert_array_equal(got, want)

@@ -136,8 +136,8 @@ int sfg_hip_attn_weights_v1(const sfg_paged_attn_args* a, float* weights, int64_
         return fail(SFG_ERR_INVALID_CONFIG, "attn_weights: %lld rows over %lld tokens", (long long)a->rows,
                     (long long)a->max_context);
     if ((rc = check_context("attn_weights", a->max_context, a->pages_per_seq * a->page_tokens)) != SFG_OK) return rc;
-    if (a->max_context > (1 << 24))
-        return fail(SFG_ERR_UNSUPPORTED, "attn_weights: more than 2^24 tokens");
+    if (a->max_context > (1 << 23))
+        return fail(SFG_ERR_UNSUPPORTED, "attn_weights: more than 2^23 tokens");
     if (!weights || weights_ld < a->max_context)
         return fail(SFG_ERR_SHAPE, "attn_weights: weights of %lld tokens for sequences up to %lld", (long long)weights_ld,
                     (long long)a->max_context);

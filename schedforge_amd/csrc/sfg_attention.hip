@@ -1806,7 +1806,7 @@ __global__ __launch_bounds__(64) void kv_append_kernel(KvAppendArgs a) {
 // heads x 64 tokens at D 128: 22 us); here a thread gathers a dim's tokens of the page
 // and stores the run, whole where the call covers it.
 template <typename KvT, typename SrcT>
-__global__ __launch_bounds__(256) void kv_append_pages_kernel(KvAppendArgs a, int tokens) {
+__global__ __launch_bounds__(256) void kv_append_pages_kernel(KvAppendArgs a, int tokens, int vector) {
     const int h = blockIdx.x % a.kv_heads, b = blockIdx.x / a.kv_heads;
     const int D = a.head_dim;
     const int64_t start = a.seq_lens ? a.seq_lens[b] : a.start;  // (a length may be anything)
@@ -1828,11 +1828,24 @@ __global__ __launch_bounds__(256) void kv_append_pages_kernel(KvAppendArgs a, in
         else if constexpr (sizeof(SrcT) == 4) return f32_to_bf16(*p);
         else return bf16_to_f32(*p);
     };
-    for (int e = threadIdx.x; e < (hi - lo) * D; e += 256) {
-        const int t = lo + e / D, d = e % D;
-        kdst[t * D + d] = load(ks + (t0 + t) * a.st + d);
+    // half of the waves take K, half V
+    const int tid = threadIdx.x & 127;
+    if (threadIdx.x < 128) {
+        const int row = D * static_cast<int>(sizeof(KvT)) / 16;  // vectors of a row
+        if (vector) {
+            for (int e = tid; e < (hi - lo) * row; e += 128) {
+                const int t = lo + e / row, x = e % row;
+                reinterpret_cast<uint4*>(kdst + t * D)[x] = reinterpret_cast<const uint4*>(ks + (t0 + t) * a.st)[x];
+            }
+        } else {
+            for (int e = tid; e < (hi - lo) * D; e += 128) {
+                const int t = lo + e / D, d = e % D;
+                kdst[t * D + d] = load(ks + (t0 + t) * a.st + d);
+            }
+        }
+        return;
     }
-    for (int d = threadIdx.x; d < D; d += 256) {
+    for (int d = tid; d < D; d += 128) {
         KvT v[kPageTok];
 #pragma unroll
         for (int t = 0; t < kPageTok; ++t) v[t] = load(vs + (t0 + min(max(t, lo), hi - 1)) * a.st + d);
@@ -1905,12 +1918,16 @@ int launch_kv_append(const void* keys, const void* values, int src_dtype, int64_
         (reinterpret_cast<uintptr_t>(v_pool) & 15) == 0) {
         const dim3 pgrid(static_cast<unsigned>(batch * kv_heads), static_cast<unsigned>(spans));
         const int n = static_cast<int>(tokens);
+        // rows of the pool's type that start and end on 16-byte boundaries move as vectors
+        const int64_t per = pool_dtype == SFG_F32 ? 4 : 8;
+        const int vec = src_dtype == pool_dtype && head_dim % per == 0 && sb % per == 0 && sh % per == 0 && st % per == 0 &&
+                        ((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(k_pool)) & 15) == 0;
         if (pool_dtype == SFG_F32) {
-            if (a.src_f32) kv_append_pages_kernel<float, float><<<pgrid, 256, 0, stream>>>(a, n);
-            else kv_append_pages_kernel<float, uint16_t><<<pgrid, 256, 0, stream>>>(a, n);
+            if (a.src_f32) kv_append_pages_kernel<float, float><<<pgrid, 256, 0, stream>>>(a, n, vec);
+            else kv_append_pages_kernel<float, uint16_t><<<pgrid, 256, 0, stream>>>(a, n, vec);
         } else {
-            if (a.src_f32) kv_append_pages_kernel<uint16_t, float><<<pgrid, 256, 0, stream>>>(a, n);
-            else kv_append_pages_kernel<uint16_t, uint16_t><<<pgrid, 256, 0, stream>>>(a, n);
+            if (a.src_f32) kv_append_pages_kernel<uint16_t, float><<<pgrid, 256, 0, stream>>>(a, n, vec);
+            else kv_append_pages_kernel<uint16_t, uint16_t><<<pgrid, 256, 0, stream>>>(a, n, vec);
         }
     } else if (pool_dtype == SFG_F32) kv_append_kernel<float><<<grid, 64, 0, stream>>>(a);
     else kv_append_kernel<uint16_t><<<grid, 64, 0, stream>>>(a);

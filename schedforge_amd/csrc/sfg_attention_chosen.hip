@@ -531,13 +531,17 @@ __global__ __launch_bounds__(256) void chosen_combine_kernel(ChosenArgs p, int c
 
 // The weights' end, one wave per 256 tokens of a (sequence, kv head): lane c merges
 // (m, l) of column c, 64 columns at a time; the wave adds sum_columns 2^(s - M) / L to
-// its tokens' accumulators and takes its share of the output columns.  A column that
-// sees nothing adds nothing.  Latency, not bytes, bounds it (4 G bytes of scores and 8
+// its tokens' accumulators.  The workgroups past the tokens merge the output columns.  A
+// column that sees nothing adds nothing.  Latency, not bytes, bounds it (4 G bytes of scores and 8
 // of accumulator a token): the first columns' scores are loaded before (m, l).
-__global__ __launch_bounds__(64) void chosen_weights_kernel(ChosenArgs p, float* weights, int64_t ld) {
-    constexpr int kTok = 4, kEarly = 4, kBatch = 8;  // tokens a lane, columns loaded early, splits a batch
+__global__ __launch_bounds__(64) void chosen_weights_kernel(ChosenArgs p, float* weights, int64_t ld, int chunks) {
+    constexpr int kTok = 4, kEarly = 4, kBatch = 32;  // tokens a lane, columns loaded early, splits a batch
     const Unit<kChosenWeights> u = unit_of<kChosenWeights>(p, blockIdx.x / p.kv_heads, blockIdx.x % p.kv_heads);
     const int lane = threadIdx.x, tok0 = blockIdx.y * 256 + lane;
+    if (static_cast<int>(blockIdx.y) >= chunks) {
+        for (int c = blockIdx.y - chunks; c < u.cols; c += gridDim.y - chunks) merge_column<kChosenWeights>(p, u, c, lane);
+        return;
+    }
     const float* scores = p.scores + u.id * u.cols * p.scores_ld;
     if (static_cast<int>(blockIdx.y) * 256 < u.total) {
         int at[kTok];
@@ -595,7 +599,6 @@ __global__ __launch_bounds__(64) void chosen_weights_kernel(ChosenArgs p, float*
         for (int t = 0; t < kTok; ++t)
             if (tok0 + 64 * t < u.total) weights[u.id * ld + at[t]] = was[t] + sum[t];
     }
-    for (int c = blockIdx.y; c < u.cols; c += gridDim.y) merge_column<kChosenWeights>(p, u, c, lane);
 }
 
 constexpr int64_t kTreeTileCols = 32;    // more columns than these run the tree's tile kernel
@@ -630,9 +633,11 @@ void launch_mode(const ChosenLaunch& a, const ChosenArgs& p, const ChosenPlan& p
         if (a.kv_dtype == SFG_F32) chosen_any_kernel<float, MODE><<<grid, 64, 0, stream>>>(p);
         else chosen_any_kernel<uint16_t, MODE><<<grid, 64, 0, stream>>>(p);
     }
-    if constexpr (MODE == kChosenWeights)
-        chosen_weights_kernel<<<dim3(static_cast<unsigned>(a.batch * a.kv_heads), static_cast<unsigned>((a.max_context + 255) / 256)),
-                                64, 0, stream>>>(p, a.weights, a.weights_ld);
+    if constexpr (MODE == kChosenWeights) {
+        const int tokens = static_cast<int>((a.max_context + 255) / 256);
+        const unsigned merges = static_cast<unsigned>(std::min<int64_t>(columns / units, 64));
+        chosen_weights_kernel<<<dim3(static_cast<unsigned>(units), tokens + merges), 64, 0, stream>>>(p, a.weights, a.weights_ld, tokens);
+    }
     else if (plan.splits > 1) chosen_combine_kernel<MODE><<<(columns + 3) / 4, 256, 0, stream>>>(p, static_cast<int>(columns));
 }
 

@@ -73,6 +73,7 @@ sfg::ChosenLaunch launch_of(int mode, const sfg_paged_attn_args& a) {
     c.batch = a.batch; c.q_heads = a.q_heads; c.kv_heads = a.kv_heads; c.rows = a.rows; c.head_dim = a.head_dim;
     c.page_tokens = a.page_tokens; c.pages_per_seq = a.pages_per_seq; c.num_pages = a.num_pages;
     c.max_context = a.max_context;
+    c.kv_splits = a.kv_splits;
     c.scale = a.scale > 0.0f ? a.scale : 1.0f / sqrtf(static_cast<float>(a.head_dim));
     return c;
 }

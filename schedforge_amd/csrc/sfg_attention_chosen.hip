@@ -601,7 +601,6 @@ __global__ __launch_bounds__(64) void chosen_weights_kernel(ChosenArgs p, float*
     }
 }
 
-constexpr int64_t kTreeTileCols = 32;    // more columns than these run the tree's tile kernel
 constexpr int64_t kMaxGroups = 1 << 23;  // workgroups of 256 threads in a launch
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
@@ -615,16 +614,18 @@ void launch_mfma(const ChosenLaunch& a, const ChosenArgs& p, unsigned grid, int 
 }
 
 template <int MODE>
-void launch_mode(const ChosenLaunch& a, const ChosenArgs& p, const ChosenPlan& plan, hipStream_t stream) {
+void launch_mode(const ChosenLaunch& a, const ChosenArgs& p, const ChosenPlan& plan, void* workspace, hipStream_t stream) {
     const unsigned columns = static_cast<unsigned>(a.batch * a.rows * a.q_heads);
     const int64_t units = a.batch * a.kv_heads * (MODE == kChosenSparse ? a.rows : 1);
     const int64_t chunks = (columns / units + 15) / 16;
     // Q, K and V are read as 16-byte vectors; rows of 64 or 128 elements keep a base's boundary
     const bool aligned = ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k_pool) | reinterpret_cast<uintptr_t>(a.v_pool)) & 15) == 0;
-    const TreeTiles tiles = tree_tiles(columns / units);
-    if (plan.tiles && aligned && units * tiles.chunks * plan.splits <= kMaxGroups) {
-        launch_tree_tiles(p, tiles, units, stream);
-    } else if (plan.mfma && aligned && units * chunks * plan.splits <= kMaxGroups) {
+    if (plan.tiles && aligned) {
+        launch_tree_tiles(p, plan_tree_tiles(a.batch, a.kv_heads, columns / units, a.head_dim, a.max_context + a.rows, a.kv_splits),
+                          a.batch, workspace, stream);
+        return;
+    }
+    if (plan.mfma && aligned && units * chunks * plan.splits <= kMaxGroups) {
         const unsigned grid = static_cast<unsigned>(units * chunks * plan.splits);
         if (a.head_dim == 128) launch_mfma<MODE, 128>(a, p, grid, static_cast<int>(chunks), stream);
         else launch_mfma<MODE, 64>(a, p, grid, static_cast<int>(chunks), stream);
@@ -650,16 +651,12 @@ ChosenPlan plan_chosen(int mode, bool bf16, int64_t batch, int64_t q_heads, int6
     plan.mfma = (head_dim == 64 || head_dim == 128) && page_tokens == kPageTok;
     const int64_t units = batch * kv_heads * (mode == kChosenSparse ? rows : 1);
     const int64_t cols = columns / units;
-    plan.tiles = mode == kChosenTree && plan.mfma && bf16 && cols > kTreeTileCols;
-    const int64_t base = plan.tiles ? units * tree_tiles(cols).chunks : plan.mfma ? units * ((cols + 15) / 16) : columns;
+    const int64_t base = plan.mfma ? units * ((cols + 15) / 16) : columns;
     const int64_t most = plan.mfma ? (keys + kPageTok - 1) / kPageTok : keys;
     int64_t s = 1;
     if (requested > 0) s = std::min<int64_t>(requested, std::max<int64_t>(most, 1));
     // matrix cores: two workgroups per CU while a split keeps 8 pages (two per wave);
     // else >= 1024 waves while a split keeps >= 256 tokens
-    else if (plan.tiles)
-        // tiles of 64 tokens: two workgroups per CU while a split keeps 4
-        while (base * s < 512 && most / (s * 2) >= 16) s *= 2;
     else
         while (base * s < (plan.mfma ? 512 : 1024) && most / (s * 2) >= (plan.mfma ? 8 : 256)) s *= 2;
     plan.splits = static_cast<int>(std::min<int64_t>(s, 65535));
@@ -671,6 +668,11 @@ ChosenPlan plan_chosen(int mode, bool bf16, int64_t batch, int64_t q_heads, int6
     if (mode == kChosenWeights) {
         plan.scores_ld = (keys + 15) / 16 * 16;
         plan.scores_bytes = up256(static_cast<size_t>(columns) * plan.scores_ld * sizeof(float));
+    }
+    if (mode == kChosenTree && plan.mfma && bf16) {
+        const TreeTiles t = plan_tree_tiles(batch, kv_heads, cols, head_dim, keys, requested);
+        plan.tiles = t.groups > 0;
+        plan.tile_bytes = t.bytes();
     }
     return plan;
 }
@@ -693,9 +695,9 @@ void launch_chosen(const ChosenLaunch& a, const ChosenPlan& plan, void* workspac
     p.scale_log2 = a.scale * kLog2e;
     p.mask = a.mask; p.mask_stride = a.mask_stride; p.mask_words = static_cast<int>((a.rows + 31) / 32);
     p.selected = a.selected; p.top = static_cast<int>(a.top);
-    if (a.mode == kChosenTree) launch_mode<kChosenTree>(a, p, plan, stream);
-    else if (a.mode == kChosenWeights) launch_mode<kChosenWeights>(a, p, plan, stream);
-    else launch_mode<kChosenSparse>(a, p, plan, stream);
+    if (a.mode == kChosenTree) launch_mode<kChosenTree>(a, p, plan, workspace, stream);
+    else if (a.mode == kChosenWeights) launch_mode<kChosenWeights>(a, p, plan, workspace, stream);
+    else launch_mode<kChosenSparse>(a, p, plan, workspace, stream);
 }
 
 }  // namespace sfg

@@ -156,6 +156,7 @@ struct ChosenLaunch {
     void* out; int out_dtype;
     int64_t batch, q_heads, kv_heads, rows, head_dim, page_tokens, pages_per_seq, num_pages;
     int64_t max_context;                            // no sequence is longer (tree: committed tokens)
+    int32_t kv_splits;
     float scale;
     const uint32_t* mask; int64_t mask_stride;      // tree
     float* weights; int64_t weights_ld;             // weights
@@ -169,7 +170,11 @@ struct ChosenPlan {
     bool tiles;                                     // the tree's tile kernel
     size_t ml_bytes, acc_bytes, scores_bytes;
     int64_t scores_ld;
-    size_t bytes() const { return ml_bytes + acc_bytes + scores_bytes; }
+    size_t tile_bytes;                              // what the tile kernel takes instead of the partials
+    size_t bytes() const {
+        const size_t n = ml_bytes + acc_bytes + scores_bytes;
+        return n > tile_bytes ? n : tile_bytes;
+    }
 };
 // bf16: queries, pools and output all are.
 ChosenPlan plan_chosen(int mode, bool bf16, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t rows, int64_t head_dim,

@@ -153,16 +153,6 @@ struct SelShared {
     Key found; int ties;
 };
 
-// Sum of the lanes up to this one, by DPP: row shifts, then the rows' totals broadcast.
-__device__ __forceinline__ int wave_inclusive(int x) {
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr:1
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15 to rows 1, 3
-    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast:31 to rows 2, 3
-    return x;
-}
 // OR over the wave, in every lane (an AND is the complement of the complements' OR).
 __device__ __forceinline__ uint32_t wave_or(uint32_t v) {
     int x = static_cast<int>(v);

@@ -30,6 +30,16 @@ __device__ __forceinline__ uint32_t finite_bf16x2(uint32_t w) {
     return w & ~((bad >> 15) * 0xFFFFu);
 }
 
+// Sum of the lanes up to this one, by DPP: row shifts, then the rows' totals broadcast.
+__device__ __forceinline__ int wave_inclusive(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr:1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15 to rows 1, 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast:31 to rows 2, 3
+    return x;
+}
 template <typename KvT>
 __device__ __forceinline__ float kv_f32(const KvT* p, int64_t i) {
     if constexpr (sizeof(KvT) == 4) return p[i];

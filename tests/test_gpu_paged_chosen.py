@@ -560,3 +560,58 @@ def test_several_tokens_appended_by_pages(d, dtype, src):
                     if 0 <= at < 80 and table[n, at // 16] >= 0:
                         want[n, :, at] = c.round(new[n, :, t])
             np.testing.assert_array_equal(got, want)
+
+
+# (q heads, kv heads, D, nodes, lengths, splits): more than 32 columns in bf16
+TILES = [(16, 4, 128, 24, (1500, 0, 64, 63, 65, 130), 0), (8, 2, 64, 30, (1000, 1, 700), 0), (8, 2, 128, 70, (900, 40, 0), 0),
+         (12, 2, 128, 9, (300, 2000, 128), 3), (16, 4, 64, 100, (600, 33), 7), (8, 1, 128, 5, (4096, 17), 0),
+         (4, 4, 128, 200, (190, 0, 500), 0), (64, 1, 64, 3, (250,), 1), (4, 2, 128, 64, tuple(range(0, 700, 10)), 0)]
+
+
+@pytest.mark.parametrize("hq,hkv,d,t,lens,splits", TILES)
+def test_trees_of_many_columns(hq, hkv, d, t, lens, splits):
+    """The tile kernel: every number of columns a wave and a workgroup, runs that begin and end anywhere in a
+    sequence, masks of up to seven words, poison where nothing may look, twice over the same workspace."""
+    lib = _abi.load()
+    rng = np.random.default_rng(hq + d + t)
+    longest = max(lens)
+    c = Cache(rng, lens, longest + t, hkv, d)
+    c.upload(c.lens + t)
+    for _ in range(2):
+        bits = ancestors(random_tree(rng, c.b, t))
+        q, qd, qdt = queries(rng, c.b, hq, t, d, "bf16")
+        out, odt = output(q.shape, "bf16")
+        run_tree(lib, c, qd, qdt, dev(words(bits)), t * -(-t // 32), out, odt, longest, splits)
+        got = value(out)
+        pick = rng.permutation(c.b * hq * t)[:400]  # (every column is computed; some are compared)
+        for x in pick:
+            n, h, i = x // (hq * t), x // t % hq, x % t
+            s = np.arange(c.per * 16) < c.lens[n]
+            s[c.lens[n]: c.lens[n] + t] = bits[n, i]
+            ref, _, err, _ = attend(q[n, h, i], c.k[n, h // (hq // hkv)], c.v[n, h // (hq // hkv)], s, True, True)
+            close(got[n, h, i], ref, err, f"column {n} {h} {i}")
+
+
+@pytest.mark.parametrize("longest", [70, 3000])
+def test_visible_infinities_in_trees_of_many_columns(longest):
+    """Infinite drafted values reach the rows that see them, and no others; infinite committed values reach all:
+    where one workgroup walks a sequence, and where several do."""
+    lib = _abi.load()
+    rng = np.random.default_rng(longest)
+    t = 20
+    c = Cache(rng, (longest, 60), longest + t, 2, 128)
+    at = longest + 11
+    c.v[0, 1, at, 5], c.v[0, 1, at, 100] = np.inf, np.nan
+    c.v[0, 0, 33, 7] = -np.inf
+    c.upload(c.lens + t)
+    bits = ancestors(random_tree(rng, 2, t))
+    q, qd, qdt = queries(rng, 2, 8, t, 128, "bf16")
+    out, odt = output(q.shape, "bf16")
+    run_tree(lib, c, qd, qdt, dev(words(bits)), t, out, odt, longest)
+    got = value(out)
+    for i in range(t):
+        sees = bits[0, i, 11]
+        assert ((got[0, 4:, i, 5] == np.inf) == sees).all() and (np.isnan(got[0, 4:, i, 100]) == sees).all()
+    assert (got[0, :4, :, 7] == -np.inf).all()
+    got[0, 4:, :, 5] = got[0, 4:, :, 100] = got[0, :4, :, 7] = 0.0
+    assert np.isfinite(got).all()

@@ -85,9 +85,9 @@ int64_t walked(int mode, const sfg_paged_attn_args& a, int64_t top) {
     return std::min((a.max_context + a.page_tokens - 1) / a.page_tokens, top) * a.page_tokens;
 }
 
-sfg::ChosenPlan plan_of(int mode, const sfg_paged_attn_args& a, int64_t top) {
+sfg::ChosenPlan plan_of(int mode, const sfg_paged_attn_args& a, int64_t top, bool ragged) {
     const bool bf16 = a.q_dtype == SFG_BF16 && a.kv_dtype == SFG_BF16 && a.out_dtype == SFG_BF16;
-    return sfg::plan_chosen(mode, bf16, a.batch, a.q_heads, a.kv_heads, a.rows, a.head_dim, a.page_tokens,
+    return sfg::plan_chosen(mode, bf16, ragged, a.batch, a.q_heads, a.kv_heads, a.rows, a.head_dim, a.page_tokens,
                             walked(mode, a, top), a.kv_splits);
 }
 
@@ -95,7 +95,8 @@ size_t page_keys_bytes(const sfg_paged_attn_args& a) {
     return sfg::page_select_workspace_bytes(a.batch, a.kv_heads, a.rows, (a.max_context + a.page_tokens - 1) / a.page_tokens);
 }
 
-// What a workspace query goes by (its pointers may be null).
+// What a workspace query goes by (its pointers may be null: it covers a call with lengths
+// and one without).
 bool sized(const sfg_paged_attn_args* a) {
     return a && a->batch > 0 && a->q_heads > 0 && a->kv_heads > 0 && a->q_heads % a->kv_heads == 0 && a->rows > 0 &&
            a->head_dim > 0 && a->head_dim <= 256 && a->page_tokens > 0 && a->max_context >= 0;
@@ -106,7 +107,7 @@ bool sized(const sfg_paged_attn_args* a) {
 extern "C" {
 
 size_t sfg_hip_attn_tree_workspace_v1(const sfg_paged_attn_args* a) {
-    return sized(a) ? plan_of(sfg::kChosenTree, *a, 0).bytes() : 0;
+    return sized(a) ? plan_of(sfg::kChosenTree, *a, 0, true).bytes() : 0;
 }
 
 int sfg_hip_attn_tree_v1(const sfg_paged_attn_args* a, const uint32_t* tree_mask, int64_t mask_stride, void* workspace,
@@ -116,7 +117,7 @@ int sfg_hip_attn_tree_v1(const sfg_paged_attn_args* a, const uint32_t* tree_mask
     if (!tree_mask || (mask_stride != 0 && mask_stride < a->rows * ((a->rows + 31) / 32)))
         return fail(SFG_ERR_SHAPE, "attn_tree: no mask, or sequences' masks overlap");
     if ((rc = check_context("attn_tree", a->max_context + a->rows, a->pages_per_seq * a->page_tokens)) != SFG_OK) return rc;
-    const sfg::ChosenPlan plan = plan_of(sfg::kChosenTree, *a, 0);
+    const sfg::ChosenPlan plan = plan_of(sfg::kChosenTree, *a, 0, a->seq_lens != nullptr);
     if ((rc = check_workspace("attn_tree", plan.bytes(), workspace, workspace_bytes)) != SFG_OK) return rc;
     sfg::ChosenLaunch c = launch_of(sfg::kChosenTree, *a);
     c.mask = tree_mask;
@@ -126,7 +127,7 @@ int sfg_hip_attn_tree_v1(const sfg_paged_attn_args* a, const uint32_t* tree_mask
 }
 
 size_t sfg_hip_attn_weights_workspace_v1(const sfg_paged_attn_args* a) {
-    return sized(a) ? plan_of(sfg::kChosenWeights, *a, 0).bytes() : 0;
+    return sized(a) ? plan_of(sfg::kChosenWeights, *a, 0, true).bytes() : 0;
 }
 
 int sfg_hip_attn_weights_v1(const sfg_paged_attn_args* a, float* weights, int64_t weights_ld, void* workspace,
@@ -142,7 +143,7 @@ int sfg_hip_attn_weights_v1(const sfg_paged_attn_args* a, float* weights, int64_
     if (!weights || weights_ld < a->max_context)
         return fail(SFG_ERR_SHAPE, "attn_weights: weights of %lld tokens for sequences up to %lld", (long long)weights_ld,
                     (long long)a->max_context);
-    const sfg::ChosenPlan plan = plan_of(sfg::kChosenWeights, *a, 0);
+    const sfg::ChosenPlan plan = plan_of(sfg::kChosenWeights, *a, 0, a->seq_lens != nullptr);
     if ((rc = check_workspace("attn_weights", plan.bytes(), workspace, workspace_bytes)) != SFG_OK) return rc;
     sfg::ChosenLaunch c = launch_of(sfg::kChosenWeights, *a);
     c.weights = weights;
@@ -152,7 +153,7 @@ int sfg_hip_attn_weights_v1(const sfg_paged_attn_args* a, float* weights, int64_
 }
 
 size_t sfg_hip_attn_sparse_workspace_v1(const sfg_paged_attn_args* a, int64_t top_pages) {
-    return sized(a) && top_pages > 0 ? page_keys_bytes(*a) + plan_of(sfg::kChosenSparse, *a, top_pages).bytes() : 0;
+    return sized(a) && top_pages > 0 ? page_keys_bytes(*a) + plan_of(sfg::kChosenSparse, *a, top_pages, true).bytes() : 0;
 }
 
 int sfg_hip_attn_sparse_v1(const sfg_paged_attn_args* a, const void* bounds, int64_t top_pages, int64_t sink_pages,
@@ -167,7 +168,7 @@ int sfg_hip_attn_sparse_v1(const sfg_paged_attn_args* a, const void* bounds, int
         return fail(SFG_ERR_SHAPE, "attn_sparse: %lld pages with %lld first and %lld newest ones", (long long)top_pages,
                     (long long)sink_pages, (long long)recent_pages);
     if ((rc = check_context("attn_sparse", a->max_context, a->pages_per_seq * a->page_tokens)) != SFG_OK) return rc;
-    const sfg::ChosenPlan plan = plan_of(sfg::kChosenSparse, *a, top_pages);
+    const sfg::ChosenPlan plan = plan_of(sfg::kChosenSparse, *a, top_pages, a->seq_lens != nullptr);
     const size_t keys = page_keys_bytes(*a);
     if ((rc = check_workspace("attn_sparse", keys + plan.bytes(), workspace, workspace_bytes)) != SFG_OK) return rc;
     sfg::ChosenLaunch c = launch_of(sfg::kChosenSparse, *a);

@@ -115,8 +115,8 @@ __global__ __launch_bounds__(64) void chosen_any_kernel(ChosenArgs p) {
 
 // ===========================================================================
 // head_dim 64 / 128 and 16-token pages on the matrix cores.  A workgroup owns 16
-// columns of a unit and one split; its four waves take a quarter of the pages each,
-// with the next page's K and V loads behind the current page's products:
+// columns of a unit and one split; its four (or eight) waves take an equal part of the
+// pages each, with the next page's K and V loads behind the current page's products:
 //   S^T[16 tok][16 col] = K[16 tok][D] Q^T[D][16 col]
 //   O^T[D][16 col]     += V^T[D][16 tok] P^T[16 tok][16 col]
 // The S^T accumulator (lane: column l & 15, tokens 4 (l >> 4) + r) is the P^T
@@ -134,8 +134,8 @@ __global__ __launch_bounds__(64) void chosen_any_kernel(ChosenArgs p) {
 // zero, so a wave whose sums are not finite walks its pages once more: keys'
 // non-finite elements meet the leading term only, values go token by token.
 // ===========================================================================
-template <typename KvT, int kD, int MODE, bool FAST>
-__global__ __launch_bounds__(256, sizeof(KvT) == 4 ? 1 : 2) void chosen_mfma_kernel(ChosenArgs p, int chunks) {
+template <typename KvT, int kD, int MODE, bool FAST, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, sizeof(KvT) == 4 && WAVES == 4 ? 1 : 2) void chosen_mfma_kernel(ChosenArgs p, int chunks) {
     constexpr bool kF32 = sizeof(KvT) == 4;
     static_assert(!(FAST && kF32), "fp32 pools keep fp32 precision");
     constexpr int kTerms = FAST ? 1 : 3;
@@ -156,8 +156,8 @@ __global__ __launch_bounds__(256, sizeof(KvT) == 4 ? 1 : 2) void chosen_mfma_ker
     const int sp_begin = static_cast<int>(static_cast<int64_t>(pages) * split / p.splits);
     const int sp_end = static_cast<int>(static_cast<int64_t>(pages) * (split + 1) / p.splits);
     const int n_sp = sp_end - sp_begin;
-    const int w_begin = sp_begin + n_sp * wave / 4;
-    const int w_end = sp_begin + n_sp * (wave + 1) / 4;
+    const int w_begin = sp_begin + n_sp * wave / WAVES;
+    const int w_end = sp_begin + n_sp * (wave + 1) / WAVES;
 
     // Q^T operand: this lane's column, dims kStep s + kLane lg + [0, kLane)
     const bool has = col0 + lr < u.cols;
@@ -410,9 +410,9 @@ __global__ __launch_bounds__(256, sizeof(KvT) == 4 ? 1 : 2) void chosen_mfma_ker
             for (int r = 0; r < 4; ++r) t = fmaf(acc[dt][r], 0.f, t);
         if (__any(has && t != 0.f)) walk_pages(std::true_type{});
     }
-    // the four waves merged in LDS: acc[dt][r] = O^T[dim 16 dt + 4 lg + r][column lr]
-    __shared__ float s_m[4][16], s_l[4][16];
-    __shared__ float s_acc[4][16][kD];
+    // the waves merged in LDS: acc[dt][r] = O^T[dim 16 dt + 4 lg + r][column lr]
+    __shared__ float s_m[WAVES][16], s_l[WAVES][16];
+    __shared__ float s_acc[WAVES][16][kD];
     const float l_sum = xor32_sum(xor16_sum(l_run));
 #pragma unroll
     for (int dt = 0; dt < kDt; ++dt) *reinterpret_cast<floatx4*>(&s_acc[wave][lr][16 * dt + 4 * lg]) = acc[dt];
@@ -421,14 +421,14 @@ __global__ __launch_bounds__(256, sizeof(KvT) == 4 ? 1 : 2) void chosen_mfma_ker
         s_l[wave][lr] = l_sum;
     }
     __syncthreads();
-    for (int o = threadIdx.x; o < min(16, u.cols - col0) * kD; o += 256) {
+    for (int o = threadIdx.x; o < min(16, u.cols - col0) * kD; o += WAVES * 64) {
         const int c = o / kD, d = o % kD;
         float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, s_m[w][c]);
+        for (int w = 0; w < WAVES; ++w) M = fmaxf(M, s_m[w][c]);
         float L = 0.f, a = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             const float f = split_weight(s_m[w][c], M);
             L = fmaf(s_l[w][c], f, L);
             a = fmaf(s_acc[w][c][d], f, a);
@@ -605,12 +605,12 @@ constexpr int64_t kMaxGroups = 1 << 23;  // workgroups of 256 threads in a launc
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
-template <int MODE, int kD>
+template <int MODE, int kD, int WAVES>
 void launch_mfma(const ChosenLaunch& a, const ChosenArgs& p, unsigned grid, int chunks, hipStream_t stream) {
-    if (a.kv_dtype == SFG_F32) chosen_mfma_kernel<float, kD, MODE, false><<<grid, 256, 0, stream>>>(p, chunks);
+    if (a.kv_dtype == SFG_F32) chosen_mfma_kernel<float, kD, MODE, false, WAVES><<<grid, WAVES * 64, 0, stream>>>(p, chunks);
     else if (a.q_dtype == SFG_BF16 && a.out_dtype == SFG_BF16)
-        chosen_mfma_kernel<uint16_t, kD, MODE, true><<<grid, 256, 0, stream>>>(p, chunks);
-    else chosen_mfma_kernel<uint16_t, kD, MODE, false><<<grid, 256, 0, stream>>>(p, chunks);
+        chosen_mfma_kernel<uint16_t, kD, MODE, true, WAVES><<<grid, WAVES * 64, 0, stream>>>(p, chunks);
+    else chosen_mfma_kernel<uint16_t, kD, MODE, false, WAVES><<<grid, WAVES * 64, 0, stream>>>(p, chunks);
 }
 
 template <int MODE>
@@ -627,8 +627,17 @@ void launch_mode(const ChosenLaunch& a, const ChosenArgs& p, const ChosenPlan& p
     }
     if (plan.mfma && aligned && units * chunks * plan.splits <= kMaxGroups) {
         const unsigned grid = static_cast<unsigned>(units * chunks * plan.splits);
-        if (a.head_dim == 128) launch_mfma<MODE, 128>(a, p, grid, static_cast<int>(chunks), stream);
-        else launch_mfma<MODE, 64>(a, p, grid, static_cast<int>(chunks), stream);
+        const int n = static_cast<int>(chunks);
+        if constexpr (MODE == kChosenWeights) {
+            if (a.head_dim == 128) launch_mfma<MODE, 128, 4>(a, p, grid, n, stream);
+            else launch_mfma<MODE, 64, 4>(a, p, grid, n, stream);
+        } else if (plan.waves == 8) {
+            if (a.head_dim == 128) launch_mfma<MODE, 128, 8>(a, p, grid, n, stream);
+            else launch_mfma<MODE, 64, 8>(a, p, grid, n, stream);
+        } else {
+            if (a.head_dim == 128) launch_mfma<MODE, 128, 4>(a, p, grid, n, stream);
+            else launch_mfma<MODE, 64, 4>(a, p, grid, n, stream);
+        }
     } else {
         const dim3 grid(columns, static_cast<unsigned>(plan.splits));
         if (a.kv_dtype == SFG_F32) chosen_any_kernel<float, MODE><<<grid, 64, 0, stream>>>(p);
@@ -644,7 +653,7 @@ void launch_mode(const ChosenLaunch& a, const ChosenArgs& p, const ChosenPlan& p
 
 }  // namespace
 
-ChosenPlan plan_chosen(int mode, bool bf16, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t rows, int64_t head_dim,
+ChosenPlan plan_chosen(int mode, bool bf16, bool ragged, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t rows, int64_t head_dim,
                        int64_t page_tokens, int64_t keys, int32_t requested) {
     ChosenPlan plan{};
     const int64_t columns = batch * rows * q_heads;
@@ -654,11 +663,25 @@ ChosenPlan plan_chosen(int mode, bool bf16, int64_t batch, int64_t q_heads, int6
     const int64_t base = plan.mfma ? units * ((cols + 15) / 16) : columns;
     const int64_t most = plan.mfma ? (keys + kPageTok - 1) / kPageTok : keys;
     int64_t s = 1;
-    if (requested > 0) s = std::min<int64_t>(requested, std::max<int64_t>(most, 1));
-    // matrix cores: two workgroups per CU while a split keeps 8 pages (two per wave);
-    // else >= 1024 waves while a split keeps >= 256 tokens
-    else
-        while (base * s < (plan.mfma ? 512 : 1024) && most / (s * 2) >= (plan.mfma ? 8 : 256)) s *= 2;
+    plan.waves = 4;
+    if (requested > 0) {
+        s = std::min<int64_t>(requested, std::max<int64_t>(most, 1));
+    } else if (!plan.mfma) {
+        // >= 1024 waves while a split keeps >= 256 tokens
+        while (base * s < 1024 && most / (s * 2) >= 256) s *= 2;
+    } else if (mode != kChosenWeights && most <= 64 && base >= 128) {
+        // half of the CUs busy and up to eight pages a wave: no splits to merge, one launch
+        // less (16 x 8 kv heads x 64 selected pages: 19.5 us with four splits and their merge,
+        // 16.6 so; 16 units of 57 pages: 11.2 us with eight splits, 16.6 so)
+        plan.waves = 8;
+    } else {
+        // two workgroups per CU while a split keeps 8 pages, two per wave (tree: 4; 1 x 8 kv
+        // heads x 900 tokens 12.3 us at 4 splits, 11.2 at 8); sequences with lengths of their
+        // own leave their last splits short or empty, so up to eight per CU while a split
+        // keeps 32 (32 x 4 kv heads x up to 8192 tokens: 65 us at 4 splits, 58 at 16)
+        while (base * s < 512 && most / (s * 2) >= (mode == kChosenTree ? 4 : 8)) s *= 2;
+        while (ragged && mode != kChosenSparse && base * s < 2048 && most / (s * 2) >= 32) s *= 2;
+    }
     plan.splits = static_cast<int>(std::min<int64_t>(s, 65535));
     if (mode == kChosenWeights || plan.splits > 1) {
         const size_t parts = static_cast<size_t>(columns) * plan.splits;

@@ -39,6 +39,9 @@ constexpr int kTileTok = 64;
 // What starting a (sequence, kv head, chunk) costs, in tiles: its queries, mask and first
 // tiles are waited for, the sums before it are written.
 constexpr int kStart = 6;
+// The least length of a workgroup's range: shorter ones cost more in starts, and in parts
+// to join, than they give.
+constexpr int kLeast = 5;
 
 __device__ __forceinline__ int swap_bits23(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
 
@@ -124,7 +127,7 @@ void tree_tile_kernel(ChosenArgs p, TreeRuns runs, int xcds) {
     if (blockIdx.x == 0 && threadIdx.x == 0) runs.before[0] = 0;
     const int per_seq = p.kv_heads * runs.chunks;  // (kv head, chunk) pairs
     const int64_t total = static_cast<int64_t>(total_seq) * per_seq;
-    const int groups = static_cast<int>(min<int64_t>(runs.groups, total));
+    const int groups = static_cast<int>(min<int64_t>(runs.groups, max<int64_t>(total / runs.least, 1)));
     // consecutive workgroup ids go to the XCDs in turn: each XCD gets consecutive runs, so
     // that the chunks of a (sequence, kv head) read K and V through one L2
     const int grid = static_cast<int>(gridDim.x), bid = static_cast<int>(blockIdx.x);
@@ -455,7 +458,7 @@ __device__ __forceinline__ float2 add_non_finite(const ChosenArgs& p, const Unit
 // flight), lane l the dims kD / 64 l + [0, kD / 64).
 template <int kD>
 __global__ __launch_bounds__(256) void tree_join_kernel(ChosenArgs p, TreeRuns runs, int col_groups) {
-    constexpr int kW = kD / 64, kCols = 4, kBatch = 4;
+    constexpr int kW = kD / 64, kCols = 4, kBatch = 8;
     const int lane = threadIdx.x & 63;
     const int item = blockIdx.x * 4 + (threadIdx.x >> 6);  // (sequence, kv head, four columns)
     if (item >= col_groups * p.kv_heads * runs.batch) return;
@@ -464,7 +467,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(ChosenArgs p, TreeRuns r
     const Unit<kChosenTree> u = unit_of<kChosenTree>(p, uid / p.kv_heads, uid % p.kv_heads);
     const int chunk = col0 / runs.cols;  // (a chunk is a multiple of four columns)
     const int64_t total = static_cast<int64_t>(runs.before[runs.batch]) * per_seq;
-    const int groups = static_cast<int>(min<int64_t>(runs.groups, total));
+    const int groups = static_cast<int>(min<int64_t>(runs.groups, max<int64_t>(total / runs.least, 1)));
     const int before = runs.before[u.b], n = runs.before[u.b + 1] - before;
     const int64_t first = static_cast<int64_t>(before) * per_seq + static_cast<int64_t>(u.kvh * runs.chunks + chunk) * n;
     // the workgroup of position x: the last whose range begins at or before it
@@ -541,8 +544,16 @@ TreeTiles plan_tree_tiles(int64_t batch, int64_t kv_heads, int64_t cols, int64_t
     t.cols = 32 * t.col_waves;
     t.chunks = (cols + t.cols - 1) / t.cols;
     const int64_t units = batch * kv_heads * t.chunks, tiles = (keys + kTileTok - 1) / kTileTok;
-    if (cols <= kTreeTileCols || (tiles + kStart) * batch > 0x7FFFFFFF || units * tiles > (int64_t{1} << 40)) return t;  // 64-bit products with groups
+    // Against the 16-column kernel, which reads K and V once per 16 columns but starts sooner:
+    // by the bytes that one reads.  64 columns: 1 x 8 kv heads x 8000 tokens 22.5 us there,
+    // 35 here; 16 x 8 x 900 31 and 27; 128 columns: 4 x 8 x 2000 32 and 28, 16 x 4 heads of
+    // 64 dims x 900 19 and 21, 16 x 8 x 8000 345 and 82.
+    if (cols < 8) return t;
+    const int64_t reads = (cols + 15) / 16 * batch * kv_heads * tiles * head_dim;
+    if (requested <= 0 && reads < 960 * 1024) return t;
+    if ((tiles + kStart) * batch > 0x7FFFFFFF || units * tiles > (int64_t{1} << 40)) return t;  // 64-bit products with groups
     // eight waves fill a CU (two a SIMD), four half of one; a requested count is that many a unit
+    t.least = requested > 0 ? 1 : kLeast;
     t.groups = std::min<int64_t>(requested > 0 ? std::min<int64_t>(units * requested, 1 << 16) : t.waves == 8 ? 256 : 512, units * tiles);
     const size_t parts = 2 * static_cast<size_t>(t.groups) * t.cols;
     // the length before each sequence; marks of the whole units and of the parts
@@ -562,6 +573,7 @@ void launch_tree_tiles(ChosenArgs p, const TreeTiles& t, int64_t batch, void* wo
     r.chunks = static_cast<int>(t.chunks);
     r.cols = t.cols;
     r.groups = static_cast<int>(t.groups);
+    r.least = t.least;
     p.part_ml = reinterpret_cast<float*>(ws + t.before_bytes);
     p.part_acc = reinterpret_cast<float*>(ws + t.before_bytes + t.ml_bytes);
     const unsigned grid = static_cast<unsigned>(t.groups);

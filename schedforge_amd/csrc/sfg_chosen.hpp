@@ -110,13 +110,12 @@ __device__ __forceinline__ int64_t column_offset(const ChosenArgs& p, int b, int
 __device__ __forceinline__ float split_weight(float m, float M) { return m == -INFINITY ? 1.f : fast_exp2(m - M); }
 
 // The tree's tile kernel (sfg_attention_tree.hip): bf16 queries, pools and output,
-// head_dim 64 / 128, 16-token pages, more than kTreeTileCols columns a unit.
-// groups == 0: not for this shape.
-constexpr int64_t kTreeTileCols = 32;
+// head_dim 64 / 128, 16-token pages.  groups == 0: the kernels here take the call.
 struct TreeTiles {
     int waves, col_waves, cols;  // waves of a workgroup, those that split its columns, and the columns
     int64_t chunks;        // column chunks of a unit
-    int64_t groups;        // workgroups that the tiles are dealt to
+    int64_t groups;        // workgroups that the tiles are dealt to, at most
+    int least;             // and the least that one takes
     size_t before_bytes, ml_bytes, acc_bytes;
     size_t bytes() const { return before_bytes + ml_bytes + acc_bytes; }
 };
@@ -124,7 +123,7 @@ struct TreeRuns {
     int32_t* before;       // [batch + 1] tiles before each sequence
     int32_t* unit_flags;   // [unit][chunk] and [group][2]: non-finite values among those that
     int32_t* part_flags;   // not every column sees, left out of a whole unit or of a part
-    int batch, chunks, cols, groups;
+    int batch, chunks, cols, groups, least;
 };
 TreeTiles plan_tree_tiles(int64_t batch, int64_t kv_heads, int64_t cols, int64_t head_dim, int64_t keys, int32_t requested);
 void launch_tree_tiles(ChosenArgs p, const TreeTiles& t, int64_t batch, void* workspace, hipStream_t stream);

@@ -165,7 +165,7 @@ struct ChosenLaunch {
 // keys: the tokens a unit walks at most.  The workspace holds the splits' partials and
 // for the weights the scaled scores.
 struct ChosenPlan {
-    int splits;
+    int splits, waves;
     bool mfma;                                      // the matrix-core kernels' head_dim and page size
     bool tiles;                                     // the tree's tile kernel
     size_t ml_bytes, acc_bytes, scores_bytes;
@@ -176,8 +176,9 @@ struct ChosenPlan {
         return n > tile_bytes ? n : tile_bytes;
     }
 };
-// bf16: queries, pools and output all are.
-ChosenPlan plan_chosen(int mode, bool bf16, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t rows, int64_t head_dim,
+// bf16: queries, pools and output all are.  ragged: the sequences have lengths of their
+// own (never fewer splits than without).
+ChosenPlan plan_chosen(int mode, bool bf16, bool ragged, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t rows, int64_t head_dim,
                        int64_t page_tokens, int64_t keys, int32_t requested);
 void launch_chosen(const ChosenLaunch& a, const ChosenPlan& plan, void* workspace, hipStream_t stream);
 

@@ -44,9 +44,9 @@ int check_args(const char* what, const sfg_paged_attn_args* a) {
         return fail(SFG_ERR_INVALID_CONFIG, "%s: invalid configuration", what);
     if (!float_dtype(a->q_dtype)) return fail(SFG_ERR_UNSUPPORTED, "%s: query dtype %d", what, a->q_dtype);
     if (!float_dtype(a->out_dtype)) return fail(SFG_ERR_UNSUPPORTED, "%s: output dtype %d", what, a->out_dtype);
-    if (a->q_heads > (1 << 24) || a->rows > (1 << 24) || a->batch * a->q_heads > (1 << 25) ||
-        a->batch * a->q_heads * a->rows > (1 << 25))
-        return fail(SFG_ERR_UNSUPPORTED, "%s: more than 2^25 query columns", what);
+    constexpr int64_t kMost = (1 << 22) - 1;  // 1024 threads each
+    if (a->q_heads > kMost || a->rows > kMost || a->batch * a->q_heads > kMost || a->batch * a->q_heads * a->rows > kMost)
+        return fail(SFG_ERR_UNSUPPORTED, "%s: 2^22 query columns or more", what);
     return SFG_OK;
 }
 

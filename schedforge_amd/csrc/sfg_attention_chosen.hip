@@ -620,7 +620,7 @@ void launch_mode(const ChosenLaunch& a, const ChosenArgs& p, const ChosenPlan& p
     const int64_t chunks = (columns / units + 15) / 16;
     // Q, K and V are read as 16-byte vectors; rows of 64 or 128 elements keep a base's boundary
     const bool aligned = ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k_pool) | reinterpret_cast<uintptr_t>(a.v_pool)) & 15) == 0;
-    if (plan.tiles && aligned) {
+    if (plan.tiles && aligned && (reinterpret_cast<uintptr_t>(a.out) & 7) == 0) {
         launch_tree_tiles(p, plan_tree_tiles(a.batch, a.kv_heads, columns / units, a.head_dim, a.max_context + a.rows, a.kv_splits),
                           a.batch, workspace, stream);
         return;

@@ -615,3 +615,41 @@ def test_visible_infinities_in_trees_of_many_columns(longest):
     assert (got[0, :4, :, 7] == -np.inf).all()
     got[0, 4:, :, 5] = got[0, 4:, :, 100] = got[0, :4, :, 7] = 0.0
     assert np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("t,d", [(64, 128), (12, 64), (24, 128)])
+def test_captured_trees_of_many_columns(t, d):
+    """Replays with other lengths, masks and queries in the same buffers: nothing of a capture is kept but its
+    addresses; an output off an 8-byte boundary gives what an aligned one gives, within rounding."""
+    lib = _abi.load()
+    rng = np.random.default_rng(t)
+    b, hq, hkv, longest = 3, 8, 2, 6000
+    c = Cache(rng, (6000, 17, 2500), longest + t, hkv, d, poison=False).upload((0, 0, 0))
+    q, qd, qdt = queries(rng, b, hq, t, d, "bf16")
+    mask = dev(words(ancestors(random_tree(rng, b, t))))
+    out, odt = output(q.shape, "bf16")
+    off, _ = output((q.size + 1,), "bf16")
+    a = c.args(qd, out, qdt, odt, longest)
+    ws = workspace(lib.sfg_hip_attn_tree_workspace_v1(ctypes.byref(a)))
+    run_tree(lib, c, qd, qdt, mask, t * -(-t // 32), out, odt, longest, ws=ws)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            run_tree(lib, c, qd, qdt, mask, t * -(-t // 32), out, odt, longest, ws=ws)
+    torch.cuda.synchronize()
+    for lens in ((6000, 17, 2500), (1, 5999, 64), (0, 0, 0)):
+        c.ld.copy_(torch.tensor(lens, dtype=torch.int32))
+        qd.copy_(torch.from_numpy(rng.standard_normal(q.shape).astype(np.float32)))
+        mask.copy_(torch.from_numpy(words(ancestors(random_tree(rng, b, t)))))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = out.clone()
+        run_tree(lib, c, qd, qdt, mask, t * -(-t // 32), out, odt, longest)
+        view = off[1:].view(q.shape)
+        run_tree(lib, c, qd, qdt, mask, t * -(-t // 32), view, odt, longest)
+        torch.cuda.synchronize()
+        assert torch.equal(replayed.view(torch.int16), out.view(torch.int16))
+        # both within 2^-7 of the values they round, whose size the values' bound gives
+        assert (view.float() - out.float()).abs().max() <= 2.0 ** -6 * np.abs(c.v).max()

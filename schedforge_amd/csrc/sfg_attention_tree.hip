@@ -458,7 +458,7 @@ __device__ __forceinline__ float2 add_non_finite(const ChosenArgs& p, const Unit
 // flight), lane l the dims kD / 64 l + [0, kD / 64).
 template <int kD>
 __global__ __launch_bounds__(256) void tree_join_kernel(ChosenArgs p, TreeRuns runs, int col_groups) {
-    constexpr int kW = kD / 64, kCols = 4, kBatch = 8;
+    constexpr int kW = kD / 64, kCols = 4, kBatch = 4;
     const int lane = threadIdx.x & 63;
     const int item = blockIdx.x * 4 + (threadIdx.x >> 6);  // (sequence, kv head, four columns)
     if (item >= col_groups * p.kv_heads * runs.batch) return;

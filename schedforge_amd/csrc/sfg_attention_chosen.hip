@@ -529,76 +529,59 @@ __global__ __launch_bounds__(256) void chosen_combine_kernel(ChosenArgs p, int c
     merge_column<MODE>(p, u, col, threadIdx.x & 63);
 }
 
-// The weights' end, one wave per 256 tokens of a (sequence, kv head): lane c merges
-// (m, l) of column c, 64 columns at a time; the wave adds sum_columns 2^(s - M) / L to
-// its tokens' accumulators.  The workgroups past the tokens merge the output columns.  A
-// column that sees nothing adds nothing.  Latency, not bytes, bounds it (4 G bytes of scores and 8
-// of accumulator a token): the first columns' scores are loaded before (m, l).
+// The weights' end, one wave per 256 tokens of a (sequence, kv head): four columns at a
+// time, their scores and (m, l) loaded together, lane s merging split s (and s + 64, ...);
+// the wave adds sum_columns 2^(s - M) / L to its tokens' accumulators.  The workgroups past
+// the tokens merge the output columns.  A column that sees nothing adds nothing.  Latency,
+// not bytes (4 G of scores and 8 of accumulator a token), bounds it.
 __global__ __launch_bounds__(64) void chosen_weights_kernel(ChosenArgs p, float* weights, int64_t ld, int chunks) {
-    constexpr int kTok = 4, kEarly = 4, kBatch = 32;  // tokens a lane, columns loaded early, splits a batch
+    constexpr int kTok = 4, kCols = 4;  // tokens a lane, columns at a time
     const Unit<kChosenWeights> u = unit_of<kChosenWeights>(p, blockIdx.x / p.kv_heads, blockIdx.x % p.kv_heads);
     const int lane = threadIdx.x, tok0 = blockIdx.y * 256 + lane;
     if (static_cast<int>(blockIdx.y) >= chunks) {
         for (int c = blockIdx.y - chunks; c < u.cols; c += gridDim.y - chunks) merge_column<kChosenWeights>(p, u, c, lane);
         return;
     }
+    if (static_cast<int>(blockIdx.y) * 256 >= u.total) return;
     const float* scores = p.scores + u.id * u.cols * p.scores_ld;
-    if (static_cast<int>(blockIdx.y) * 256 < u.total) {
-        int at[kTok];
-        float early[kEarly][kTok], sum[kTok], was[kTok];
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + u.id * u.cols * p.splits;
+    int at[kTok];
+    float sum[kTok], was[kTok];
 #pragma unroll
-        for (int t = 0; t < kTok; ++t) {
-            at[t] = min(tok0 + 64 * t, u.total - 1);
-            sum[t] = 0.f;
-            was[t] = weights[u.id * ld + at[t]];
-        }
-#pragma unroll
-        for (int c = 0; c < kEarly; ++c)
-#pragma unroll
-            for (int t = 0; t < kTok; ++t) early[c][t] = scores[min(c, u.cols - 1) * p.scores_ld + at[t]];
-        for (int c0 = 0; c0 < u.cols; c0 += 64) {
-            const int n = min(64, u.cols - c0);
-            const float* ml = p.part_ml + 2 * (u.id * u.cols + c0 + min(lane, n - 1)) * p.splits;
-            float M = -INFINITY, L = 0.f;
-            for (int s0 = 0; s0 < p.splits; s0 += kBatch) {
-                float2 x[kBatch];
-#pragma unroll
-                for (int e = 0; e < kBatch; ++e) x[e] = reinterpret_cast<const float2*>(ml)[min(s0 + e, p.splits - 1)];
-                float m = M;
-#pragma unroll
-                for (int e = 0; e < kBatch; ++e) m = fmaxf(m, x[e].x);
-                L *= split_weight(M, m);
-#pragma unroll
-                for (int e = 0; e < kBatch; ++e)
-                    if (s0 + e < p.splits) L = fmaf(x[e].y, split_weight(x[e].x, m), L);
-                M = m;
-            }
-            const float R = L == 0.f ? 0.f : 1.f / L;
-            auto add = [&](int c, const float* s) __attribute__((always_inline)) {
-                const float m = lane_bcast(M, c), r = lane_bcast(R, c);
-#pragma unroll
-                for (int t = 0; t < kTok; ++t)
-                    if (s[t] != -INFINITY) sum[t] = fmaf(fast_exp2(s[t] - m), r, sum[t]);
-            };
-            int c = 0;
-            if (c0 == 0)
-#pragma unroll
-                for (int e = 0; e < kEarly; ++e)
-                    if (e < n) {
-                        add(e, early[e]);
-                        c = e + 1;
-                    }
-            for (; c < n; ++c) {
-                float s[kTok];
-#pragma unroll
-                for (int t = 0; t < kTok; ++t) s[t] = scores[(c0 + c) * p.scores_ld + at[t]];
-                add(c, s);
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < kTok; ++t)
-            if (tok0 + 64 * t < u.total) weights[u.id * ld + at[t]] = was[t] + sum[t];
+    for (int t = 0; t < kTok; ++t) {
+        at[t] = min(tok0 + 64 * t, u.total - 1);
+        sum[t] = 0.f;
+        was[t] = weights[u.id * ld + at[t]];
     }
+    for (int c0 = 0; c0 < u.cols; c0 += kCols) {
+        float2 x[kCols];
+        float s[kCols][kTok];
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+            const int64_t col = min(c0 + c, u.cols - 1);
+            x[c] = ml[col * p.splits + min(lane, p.splits - 1)];
+            if (lane >= p.splits) x[c] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int t = 0; t < kTok; ++t) s[c][t] = scores[col * p.scores_ld + at[t]];
+        }
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+            if (c0 + c >= u.cols) continue;
+            for (int i = lane + 64; i < p.splits; i += 64) {
+                const float2 y = ml[static_cast<int64_t>(c0 + c) * p.splits + i];
+                const float m = fmaxf(x[c].x, y.x);
+                x[c] = make_float2(m, x[c].y * split_weight(x[c].x, m) + y.y * split_weight(y.x, m));
+            }
+            const float M = wave_max(x[c].x), L = wave_sum(x[c].y * split_weight(x[c].x, M));
+            const float R = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+            for (int t = 0; t < kTok; ++t)
+                if (s[c][t] != -INFINITY) sum[t] = fmaf(fast_exp2(s[c][t] - M), R, sum[t]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < kTok; ++t)
+        if (tok0 + 64 * t < u.total) weights[u.id * ld + at[t]] = was[t] + sum[t];
 }
 
 constexpr int64_t kMaxGroups = 1 << 23;  // workgroups of 256 threads in a launch

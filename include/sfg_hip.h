@@ -395,7 +395,8 @@ typedef struct {
  * ceil(rows / 32), is set: for a tree, u is t or one of its ancestors.  The mask is
  * taken as it is (a row does not see itself unless its bit says so).  mask_stride
  * 0: one mask for all sequences, else at least rows * W words.  The tables must
- * cover max_context + rows tokens. */
+ * cover max_context + rows tokens.  Trees of many query columns over many tokens
+ * take up to 70 MB of workspace. */
 size_t sfg_hip_attn_tree_workspace_v1(const sfg_paged_attn_args* args);
 int sfg_hip_attn_tree_v1(const sfg_paged_attn_args* args, const uint32_t* tree_mask,
                          int64_t mask_stride, void* workspace, size_t workspace_bytes,

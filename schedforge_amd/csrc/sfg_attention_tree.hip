@@ -1,9 +1,9 @@
 // sfg_attention_tree.hip -- tree attention of many columns over a paged bf16 cache.
 //
 // The rows x group query columns of a (sequence, kv head) read the same K and V.  A
-// workgroup of four waves takes up to 128 of them (32 a wave) through tiles of 64
-// tokens -- four pages -- which its waves bring into LDS by DMA, one page's K and V
-// each, the next tile in flight while the current one is multiplied:
+// workgroup takes up to 256 of them (32 a wave) through tiles of 64 tokens -- four pages
+// -- which its waves bring into LDS by DMA, the next tiles in flight while the current
+// one is multiplied:
 //   S^T[64 tok][32 col] = K Q^T     2 x D/16 mfma_f32_32x32x16_bf16 (Q in registers)
 //   O^T[D][32 col]     += V^T P^T   4 x D/32 of them
 // K row order inside a 32-token block (bits 2 and 3 of the row exchanged) makes the
@@ -11,8 +11,9 @@
 // + r % 8, so a V^T fragment is eight consecutive tokens of one page's dim -- 16 bytes of
 // the page as it lies in the pool.  LDS 16-byte slots are XOR-swizzled so that 16
 // consecutive lanes read 16 distinct ones.
-// Four waves for up to 128 columns, eight (256) beyond; up to 64 and from 65 to 128 columns
-// two waves share each 32 and take every other 32-token block.
+// Up to 64 columns four waves and two LDS stages, two workgroups a CU; else eight waves and
+// three stages.  With up to 64, and with 65 to 128, columns two waves share each 32 and take
+// every other 32-token block.
 // The running maximum moves only when a tile exceeds it by more than 8 (p <= 2^8): the
 // rescale of O^T runs only then.  P is rounded to bf16 once (2^-8 of each weight).
 //
@@ -21,6 +22,10 @@
 // chunk) as long as its tiles and kStart more for its start, workgroup w of W takes the
 // range [N w / W, N (w + 1) / W), at most two of whose runs are parts of a longer one;
 // those leave (m, l, acc) partials, and a second kernel joins them in tile order.
+// 64 drafts x 4 heads a kv head, 16 x 8 kv heads x up to 8192 tokens: 123 us and 19 of the
+// join (174 and 43 with two equal splits a sequence); the matrix pipe is 32% busy there,
+// fragment reads take LDS 2048 of a tile's 5000 cycles, and starts and partials cost the
+// rest.  32 drafts, 8 x 8 x up to 4096: 28 and 9 us.
 //
 // Tokens that some column does not see (drafts, the end, pages of no id) sit in the
 // last tiles: there each lane builds the 64 bits of what its column sees, and non-finite
@@ -37,10 +42,12 @@ namespace {
 
 constexpr int kTileTok = 64;
 // What starting a (sequence, kv head, chunk) costs, in tiles: its queries, mask and first
-// tiles are waited for, the sums before it are written.
+// tiles are waited for, the sums before it are written (at 0, 16 x 8 heads x up to 8192
+// tokens with 64 drafts took 160 us, where one workgroup had five short sequences; 126 so).
 constexpr int kStart = 6;
 // The least length of a workgroup's range: shorter ones cost more in starts, and in parts
-// to join, than they give.
+// to join, than they give (8 heads x 8000 tokens, 64 columns: 45 us at 2, 37 at 4, 34 at 6,
+// 36 at 8; 8 heads x 900: 18, 19, 21, 23).
 constexpr int kLeast = 5;
 
 __device__ __forceinline__ int swap_bits23(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
@@ -455,7 +462,8 @@ __device__ __forceinline__ float2 add_non_finite(const ChosenArgs& p, const Unit
 
 // Joins the parts of the (sequence, kv head, chunk)s that more than one workgroup
 // walked, in tile order: a wave takes four columns side by side (their loads together in
-// flight), lane l the dims kD / 64 l + [0, kD / 64).
+// flight), lane l the dims kD / 64 l + [0, kD / 64).  Four parts a batch: eight load more
+// than the usual two or three (30 us against 19 on the shape above).
 template <int kD>
 __global__ __launch_bounds__(256) void tree_join_kernel(ChosenArgs p, TreeRuns runs, int col_groups) {
     constexpr int kW = kD / 64, kCols = 4, kBatch = 4;

@@ -140,7 +140,7 @@ __global__ __launch_bounds__(64) void chosen_any_kernel(ChosenArgs p) {
 // non-finite elements meet the leading term only, values go token by token.
 // ===========================================================================
 template <typename KvT, int kD, int MODE, bool FAST, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, sizeof(KvT) == 4 && WAVES == 4 ? 1 : 2) void chosen_mfma_kernel(ChosenArgs p, int chunks) {
+__global__ __launch_bounds__(WAVES * 64, 2) void chosen_mfma_kernel(ChosenArgs p, int chunks, int xcds) {
     constexpr bool kF32 = sizeof(KvT) == 4;
     static_assert(!(FAST && kF32), "fp32 pools keep fp32 precision");
     constexpr int kTerms = FAST ? 1 : 3;
@@ -150,10 +150,15 @@ __global__ __launch_bounds__(WAVES * 64, sizeof(KvT) == 4 && WAVES == 4 ? 1 : 2)
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lr = lane & 15, lg = lane >> 4;
-    const int split = blockIdx.x % p.splits;
-    const int64_t uc = blockIdx.x / p.splits;
-    const int chunk = static_cast<int>(uc % chunks);
-    const int uid = static_cast<int>(uc / chunks);
+    // consecutive workgroup ids go to the XCDs in turn: the chunks of a (unit, split) lie one
+    // round of XCDs apart, so that they read its K and V through one L2 at about one time
+    const int bid = static_cast<int>(blockIdx.x), pairs = static_cast<int>(gridDim.x) / chunks;
+    const int full = pairs - pairs % xcds;
+    const int in = bid < full * chunks ? bid % (xcds * chunks) : bid - full * chunks;
+    const int lanes = bid < full * chunks ? xcds : pairs - full;  // (unit, split)s side by side
+    const int chunk = in / lanes;
+    const int pair = (bid < full * chunks ? bid / (xcds * chunks) * xcds : full) + in % lanes;
+    const int split = pair % p.splits, uid = pair / p.splits;
     const int per_b = MODE == kChosenSparse ? p.rows * p.kv_heads : p.kv_heads;
     const Unit<MODE> u = unit_of<MODE>(p, uid / per_b, uid % per_b);
     const int col0 = 16 * chunk;
@@ -597,10 +602,11 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 template <int MODE, int kD, int WAVES>
 void launch_mfma(const ChosenLaunch& a, const ChosenArgs& p, unsigned grid, int chunks, hipStream_t stream) {
-    if (a.kv_dtype == SFG_F32) chosen_mfma_kernel<float, kD, MODE, false, WAVES><<<grid, WAVES * 64, 0, stream>>>(p, chunks);
+    const int xcds = device_xcds(stream);
+    if (a.kv_dtype == SFG_F32) chosen_mfma_kernel<float, kD, MODE, false, WAVES><<<grid, WAVES * 64, 0, stream>>>(p, chunks, xcds);
     else if (a.q_dtype == SFG_BF16 && a.out_dtype == SFG_BF16)
-        chosen_mfma_kernel<uint16_t, kD, MODE, true, WAVES><<<grid, WAVES * 64, 0, stream>>>(p, chunks);
-    else chosen_mfma_kernel<uint16_t, kD, MODE, false, WAVES><<<grid, WAVES * 64, 0, stream>>>(p, chunks);
+        chosen_mfma_kernel<uint16_t, kD, MODE, true, WAVES><<<grid, WAVES * 64, 0, stream>>>(p, chunks, xcds);
+    else chosen_mfma_kernel<uint16_t, kD, MODE, false, WAVES><<<grid, WAVES * 64, 0, stream>>>(p, chunks, xcds);
 }
 
 template <int MODE>

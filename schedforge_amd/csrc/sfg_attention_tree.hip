@@ -562,7 +562,7 @@ TreeTiles plan_tree_tiles(int64_t batch, int64_t kv_heads, int64_t cols, int64_t
     if ((tiles + kStart) * batch > 0x7FFFFFFF || units * tiles > (int64_t{1} << 40)) return t;  // 64-bit products with groups
     // eight waves fill a CU (two a SIMD), four half of one; a requested count is that many a unit
     t.least = requested > 0 ? 1 : kLeast;
-    t.groups = std::min<int64_t>(requested > 0 ? std::min<int64_t>(units * requested, 1 << 16) : t.waves == 8 ? 256 : 512, units * tiles);
+    t.groups = std::min<int64_t>(requested > 0 ? std::min<int64_t>(units * requested, 1024) : t.waves == 8 ? 256 : 512, units * tiles);
     const size_t parts = 2 * static_cast<size_t>(t.groups) * t.cols;
     // the length before each sequence; marks of the whole units and of the parts
     t.before_bytes = (static_cast<size_t>(batch + 1 + units + 2 * t.groups) * sizeof(int32_t) + 255) / 256 * 256;

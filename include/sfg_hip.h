@@ -432,9 +432,11 @@ int sfg_hip_kv_select_v1(const float* weights, int64_t weights_ld, const int32_t
  * to the capacity).  keep is [B][keep_heads][keep_ld], keep_heads 1 (one list for
  * all heads: an accepted path of drafted tokens, base the committed lengths) or
  * kv_heads (evictions, base NULL), ascending; an entry below its index or past the
- * capacity moves nothing.  Tokens are rotated already: they keep their original
- * positions' RoPE.  new_lens may be base or counts.  No page may be in two
- * tables.  Page bounds of moved tokens must be made anew. */
+ * capacity moves nothing.  A page that receives tokens is written as a whole, with
+ * its unmoved elements as they were: nothing else may write to it meanwhile.
+ * Tokens are rotated already: they keep their original positions' RoPE.  new_lens
+ * may be base or counts.  No page may be in two tables.  Page bounds of moved
+ * tokens must be made anew. */
 int sfg_hip_kv_compact_v1(void* k_pool, void* v_pool, int pool_dtype, const int32_t* page_table,
                           const int32_t* base, const int32_t* keep, int64_t keep_heads,
                           int64_t keep_ld, const int32_t* counts, int32_t* new_lens,

@@ -25,9 +25,9 @@ namespace {
 // Any head_dim up to kRowMaxD, any page size, any alignment: one wave per
 // (unit column, split).  Lane j scores token j of each 64-token chunk with one
 // fp32 FMA chain over the head dimension, then the wave accumulates p V, lane d
-// owning dims d, d + 64, ...  Bound by its loads, K and V once per column and a
-// lane's elements apart: head_dim 80, 8 x 8 kv heads x up to 4096 tokens, 32
-// columns 1.5 ms, 4 columns with weights 0.38 ms.
+// owning dims d, d + 64, ...  Bound by its loads, K and V once per column: head_dim
+// 80, 8 x 8 kv heads x up to 4096 tokens, 32 columns 0.74 ms, 4 columns with weights
+// 0.205 ms (an element a load 1.53 and 0.38 ms).
 // ===========================================================================
 template <typename KvT, int MODE>
 __global__ __launch_bounds__(64) void chosen_any_kernel(ChosenArgs p) {
@@ -38,8 +38,13 @@ __global__ __launch_bounds__(64) void chosen_any_kernel(ChosenArgs p) {
     const Unit<MODE> u = unit_of_slot<MODE>(p, slot, col);
     column_of<MODE>(p, u, col, row, head);
     const int D = p.head_dim, pt = p.page_tokens;
-    const int k0 = static_cast<int>(static_cast<int64_t>(u.walk) * split / p.splits);
-    const int k1 = static_cast<int>(static_cast<int64_t>(u.walk) * (split + 1) / p.splits);
+    // splits begin at multiples of four tokens
+    const int k0 = static_cast<int>(static_cast<int64_t>(u.walk) * split / p.splits) & ~3;
+    const int k1 = split + 1 == p.splits ? u.walk : static_cast<int>(static_cast<int64_t>(u.walk) * (split + 1) / p.splits) & ~3;
+    // K rows as 16-byte vectors, V four tokens of a dim at a time, where they lie so
+    constexpr int kVec = 16 / sizeof(KvT);
+    const bool k_vec = D % kVec == 0 && (reinterpret_cast<uintptr_t>(p.k_pool) & 15) == 0;
+    const bool v_vec = pt % 4 == 0 && (reinterpret_cast<uintptr_t>(p.v_pool) & 15) == 0;
 
     __shared__ float sq[kRowMaxD];
     const int64_t qo = column_offset(p, u.b, row, head);
@@ -66,7 +71,18 @@ __global__ __launch_bounds__(64) void chosen_any_kernel(ChosenArgs p) {
                     page = id;
                     const KvT* kr = kpool + ((static_cast<int64_t>(id) * p.kv_heads + u.kvh) * pt + at) * D;
                     float dot = 0.f;
-                    for (int d = 0; d < D; ++d) dot = fmaf(sq[d], kv_f32(kr, d), dot);
+                    if (k_vec) {
+#pragma unroll 4
+                        for (int d = 0; d < D; d += kVec) {
+                            KvT v[kVec];
+                            const uint4 w = *reinterpret_cast<const uint4*>(kr + d);
+                            __builtin_memcpy(v, &w, sizeof v);
+#pragma unroll
+                            for (int e = 0; e < kVec; ++e) dot = fmaf(sq[d + e], kv_f32(v, e), dot);
+                        }
+                    } else {
+                        for (int d = 0; d < D; ++d) dot = fmaf(sq[d], kv_f32(kr, d), dot);
+                    }
                     s = dot * p.scale_log2;
                 }
             }
@@ -79,6 +95,30 @@ __global__ __launch_bounds__(64) void chosen_any_kernel(ChosenArgs p) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[r] *= alpha;
         const int count = min(64, k1 - base);
+        if (v_vec) {
+            for (int t = 0; t < count; t += 4) {  // tokens of one page
+                int seen[4], pg = -1;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    seen[e] = lane_bcast(page, t + e);  // (lanes past the chunk hold -1)
+                    pg = max(pg, seen[e]);
+                }
+                if (pg < 0) continue;  // wave-uniform
+                const KvT* vb = vpool + (static_cast<int64_t>(pg) * p.kv_heads + u.kvh) * D * pt + lane_bcast(at, t);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int d = lane + 64 * r;
+                    if (d >= D) continue;
+                    KvT v[4];
+                    __builtin_memcpy(v, __builtin_assume_aligned(vb + static_cast<int64_t>(d) * pt, 4 * sizeof(KvT)), sizeof v);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (seen[e] >= 0) acc[r] = fmaf(lane_bcast(pr, t + e), kv_f32(v, e), acc[r]);
+                }
+            }
+            m = m_new;
+            continue;
+        }
         for (int t = 0; t < count; ++t) {
             const float pt_t = lane_bcast(pr, t);
             const int pg = lane_bcast(page, t);
@@ -138,6 +178,10 @@ __global__ __launch_bounds__(64) void chosen_any_kernel(ChosenArgs p) {
 // is taken token by token.  With three terms a visible infinity would meet terms of
 // zero, so a wave whose sums are not finite walks its pages once more: keys'
 // non-finite elements meet the leading term only, values go token by token.
+//
+// Two waves a SIMD (at most 256 registers) for every variant: over fp32 pools of head_dim
+// 128 the compiler would take more and leave one (8 x 8 kv heads x up to 4096 tokens, 128
+// columns: 213 us so, 185 with two).
 // ===========================================================================
 template <typename KvT, int kD, int MODE, bool FAST, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void chosen_mfma_kernel(ChosenArgs p, int chunks, int xcds) {
@@ -152,6 +196,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void chosen_mfma_kernel(ChosenArgs p
     const int lr = lane & 15, lg = lane >> 4;
     // consecutive workgroup ids go to the XCDs in turn: the chunks of a (unit, split) lie one
     // round of XCDs apart, so that they read its K and V through one L2 at about one time
+    // (16 x 8 kv heads x 900 tokens, 32 columns: 22.8 us in plain order, 17.3 so)
     const int bid = static_cast<int>(blockIdx.x), pairs = static_cast<int>(gridDim.x) / chunks;
     const int full = pairs - pairs % xcds;
     const int in = bid < full * chunks ? bid % (xcds * chunks) : bid - full * chunks;

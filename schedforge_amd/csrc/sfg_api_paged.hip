@@ -15,6 +15,8 @@ using sfg::check_launch;
 using sfg::fail;
 
 constexpr int64_t kMaxInt = 0x7FFFFFFF;
+constexpr int64_t kMostUnits = (1 << 21) - 1;    // (sequence, kv head)s: up to 2048 threads each
+constexpr int64_t kMostColumns = (1 << 22) - 1;  // 1024 threads each
 
 hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
 
@@ -29,9 +31,15 @@ int check_pool(const char* what, const void* table, int pool_dtype, int64_t batc
     if (!float_dtype(pool_dtype)) return fail(SFG_ERR_UNSUPPORTED, "%s: pool dtype %d", what, pool_dtype);
     if (head_dim > 256) return fail(SFG_ERR_UNSUPPORTED, "%s: head_dim %lld > 256", what, (long long)head_dim);
     if (page_tokens > kMaxInt / 2 || pages_per_seq > kMaxInt / 2 / page_tokens || num_pages > kMaxInt || batch > (1 << 20) ||
-        kv_heads > (1 << 20) || batch * kv_heads > (1 << 21))
+        kv_heads > (1 << 20) || batch * kv_heads > kMostUnits)
         return fail(SFG_ERR_UNSUPPORTED, "%s: sizes beyond 32-bit positions", what);
     return SFG_OK;
+}
+
+// Whether the query columns can be counted (batch and kv_heads are positive).
+bool countable(const sfg_paged_attn_args& a) {
+    return a.batch <= kMostColumns && a.q_heads <= kMostColumns && a.rows <= kMostColumns &&
+           a.batch * a.q_heads <= kMostColumns && a.batch * a.q_heads * a.rows <= kMostColumns;
 }
 
 int check_args(const char* what, const sfg_paged_attn_args* a) {
@@ -44,8 +52,7 @@ int check_args(const char* what, const sfg_paged_attn_args* a) {
         return fail(SFG_ERR_INVALID_CONFIG, "%s: invalid configuration", what);
     if (!float_dtype(a->q_dtype)) return fail(SFG_ERR_UNSUPPORTED, "%s: query dtype %d", what, a->q_dtype);
     if (!float_dtype(a->out_dtype)) return fail(SFG_ERR_UNSUPPORTED, "%s: output dtype %d", what, a->out_dtype);
-    constexpr int64_t kMost = (1 << 22) - 1;  // 1024 threads each
-    if (a->q_heads > kMost || a->rows > kMost || a->batch * a->q_heads > kMost || a->batch * a->q_heads * a->rows > kMost)
+    if (!countable(*a))
         return fail(SFG_ERR_UNSUPPORTED, "%s: 2^22 query columns or more", what);
     return SFG_OK;
 }
@@ -99,7 +106,8 @@ size_t page_keys_bytes(const sfg_paged_attn_args& a) {
 // and one without).
 bool sized(const sfg_paged_attn_args* a) {
     return a && a->batch > 0 && a->q_heads > 0 && a->kv_heads > 0 && a->q_heads % a->kv_heads == 0 && a->rows > 0 &&
-           a->head_dim > 0 && a->head_dim <= 256 && a->page_tokens > 0 && a->max_context >= 0;
+           a->head_dim > 0 && a->head_dim <= 256 && a->page_tokens > 0 && a->page_tokens <= kMaxInt / 2 &&
+           a->max_context >= 0 && a->max_context <= kMaxInt / 2 && countable(*a);
 }
 
 }  // namespace
@@ -116,7 +124,9 @@ int sfg_hip_attn_tree_v1(const sfg_paged_attn_args* a, const uint32_t* tree_mask
     if (rc != SFG_OK) return rc;
     if (!tree_mask || (mask_stride != 0 && mask_stride < a->rows * ((a->rows + 31) / 32)))
         return fail(SFG_ERR_SHAPE, "attn_tree: no mask, or sequences' masks overlap");
-    if ((rc = check_context("attn_tree", a->max_context + a->rows, a->pages_per_seq * a->page_tokens)) != SFG_OK) return rc;
+    const int64_t capacity = a->pages_per_seq * a->page_tokens;  // (the sum below is taken only of lengths within it)
+    if ((rc = check_context("attn_tree", a->max_context, capacity)) != SFG_OK) return rc;
+    if ((rc = check_context("attn_tree", a->max_context + a->rows, capacity)) != SFG_OK) return rc;
     const sfg::ChosenPlan plan = plan_of(sfg::kChosenTree, *a, 0, a->seq_lens != nullptr);
     if ((rc = check_workspace("attn_tree", plan.bytes(), workspace, workspace_bytes)) != SFG_OK) return rc;
     sfg::ChosenLaunch c = launch_of(sfg::kChosenTree, *a);
@@ -204,7 +214,7 @@ int sfg_hip_kv_select_v1(const float* weights, int64_t weights_ld, const int32_t
         return fail(SFG_ERR_INVALID_CONFIG, "kv_select: a budget of %lld tokens with the newest %lld", (long long)budget,
                     (long long)recent);
     if (max_context > kMaxInt / 2 || budget > kMaxInt / 2 || batch > (1 << 20) || kv_heads > (1 << 20) ||
-        batch * kv_heads > (1 << 21))
+        batch * kv_heads > kMostUnits)
         return fail(SFG_ERR_UNSUPPORTED, "kv_select: sizes beyond 32-bit positions");
     sfg::launch_kv_select(weights, weights_ld, seq_lens, max_context, budget, recent, keep, kept_lens, kept_weights, batch,
                           kv_heads, as_stream(stream));

@@ -88,6 +88,25 @@ def test_workspace_queries_of_bad_sizes_are_zero(lib):
     assert lib.sfg_hip_attn_sparse_workspace_v1(ctypes.byref(args()), 0) == 0
 
 
+def test_sizes_past_counting(lib):
+    """Sizes whose products or sums leave 64 bits: queries say 0, calls refuse."""
+    far = (1 << 63) - 1
+    for bad in (dict(batch=1 << 32, kv_heads=1 << 32, q_heads=1 << 32), dict(rows=1 << 62), dict(q_heads=1 << 40), dict(page_tokens=far),
+                dict(batch=1 << 12, rows=1 << 10)):
+        r = ctypes.byref(args(**bad))
+        assert lib.sfg_hip_attn_tree_workspace_v1(r) == 0, bad
+        assert lib.sfg_hip_attn_weights_workspace_v1(r) == 0, bad
+        assert lib.sfg_hip_attn_sparse_workspace_v1(r, 4) == 0, bad
+    for longest in (far, far - 3, 1 << 31):
+        r = ctypes.byref(args(max_context=longest))
+        assert lib.sfg_hip_attn_tree_workspace_v1(r) == lib.sfg_hip_attn_sparse_workspace_v1(r, 4) == 0
+        for rc in calls(lib, args(max_context=longest)):
+            assert rc == GUARD, longest
+    wide = args(batch=1 << 20, q_heads=2, kv_heads=2, rows=1)
+    for rc in calls(lib, wide):
+        assert rc == UNSUPPORTED
+
+
 def test_token_selection(lib):
     def call(weights=64, ld=100, lens=None, longest=100, budget=10, recent=2, keep=64, counts=128, kept=None, b=2, h=2):
         return lib.sfg_hip_kv_select_v1(weights, ld, lens, longest, budget, recent, keep, counts, kept, b, h, None)

@@ -169,9 +169,10 @@ __global__ __launch_bounds__(64) void chosen_any_kernel(ChosenArgs p) {
 // pages in flight instead of one were no faster (53 and 17 us).
 //
 // FAST (bf16 queries and output over bf16 pools): Q is exact in one bf16 operand; P
-// is rounded to bf16 once, half a step (2^-8) of each weight, whose sum is as far off
-// as the rounding of the result itself.  Otherwise Q and P keep 24 bits: three bf16
-// terms over bf16 pools, fp32 matrix instructions over fp32 pools.
+// keeps 16 bits in two terms, so that what reaches the result is its own rounding (one
+// rounded term made as large an error of its own, and was no faster: the loads bound
+// the walk).  Otherwise Q and P keep 24 bits: three bf16 terms over bf16 pools, fp32
+// matrix instructions over fp32 pools.
 //
 // What a column does not see reaches it neither as a score (replaced by -inf) nor as
 // 0 * inf: V past the unit's end is zeroed, and a page with a hidden non-finite value
@@ -407,10 +408,15 @@ __global__ __launch_bounds__(WAVES * 64, 2) void chosen_mfma_kernel(ChosenArgs p
                             acc[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vt, pv[t], acc[dt], 0, 0, 0);
                         }
                 } else if constexpr (FAST) {
-                    const short4v pb = as_short4(make_uint2(cvt_pk_bf16(pv[0], pv[1]), cvt_pk_bf16(pv[2], pv[3])));
+                    uint2 hi, lo;
+                    split2_weights(pv[0], pv[1], hi.x, lo.x);
+                    split2_weights(pv[2], pv[3], hi.y, lo.y);
 #pragma unroll
                     for (int dt = 0; dt < kDt; ++dt)
-                        acc[dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(as_short4(vc[dt]), pb, acc[dt], 0, 0, 0);
+                        acc[dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(as_short4(vc[dt]), as_short4(lo), acc[dt], 0, 0, 0);
+#pragma unroll
+                    for (int dt = 0; dt < kDt; ++dt)
+                        acc[dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(as_short4(vc[dt]), as_short4(hi), acc[dt], 0, 0, 0);
                 } else {
                     uint16_t w[3][4];
 #pragma unroll

@@ -24,6 +24,15 @@ __device__ __forceinline__ void split3(float v, uint16_t& hi, uint16_t& mid, uin
     mid = static_cast<uint16_t>(__float_as_uint(r) >> 16);
     lo = static_cast<uint16_t>(__float_as_uint(r - bf16_to_f32(mid)) >> 16);
 }
+// Two softmax weights as two bf16 terms each, packed: the leading one truncated, the second
+// what is left of p (1 + 2^-23), rounded (2^-15 of p at most, and the 2^-23).  Both terms are
+// positive wherever p is, so that an infinity times them keeps its sign and is not 0 * inf.
+__device__ __forceinline__ void split2_weights(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+    const uint32_t u0 = __float_as_uint(p0), u1 = __float_as_uint(p1);
+    hi = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
+    lo = cvt_pk_bf16(fmaf(p0, 1.0f + 0x1p-23f, -__uint_as_float(u0 & 0xFFFF0000u)),
+                     fmaf(p1, 1.0f + 0x1p-23f, -__uint_as_float(u1 & 0xFFFF0000u)));
+}
 // two bf16 values, the infinite and NaN ones replaced by zero
 __device__ __forceinline__ uint32_t finite_bf16x2(uint32_t w) {
     const uint32_t bad = ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;  // exponent all ones

@@ -371,9 +371,11 @@ int sfg_hip_kv_gather_paged_v1(const uint16_t* k_pool, const uint16_t* v_pool,
 /* Arguments shared by the three attentions: q and out head-major
  * [B][Hq][rows][D] in q_dtype and out_dtype (SFG_F32 or SFG_BF16), group
  * Hq / Hkv of any size.  kv_splits <= 0 picks a split count, scale <= 0 means
- * 1 / sqrt(D).  bf16 queries with a bf16 output run with probabilities rounded to
- * bf16 once before the value product; every other combination keeps queries and
- * probabilities at fp32 precision. */
+ * 1 / sqrt(D).  bf16 queries with a bf16 output over bf16 pools run with
+ * probabilities of 16 bits (2^-15 of each lost at most); every other combination
+ * keeps queries and probabilities at fp32 precision.  Infinities and NaN among the
+ * keys and values that a row sees give what the formula gives; where an infinite
+ * value's weight is under 2^-100 of the row's largest it may count as 0 (NaN). */
 typedef struct {
     const void* q; int32_t q_dtype;
     const void* k_pool; const void* v_pool; int32_t kv_dtype;

@@ -449,7 +449,8 @@ int sfg_hip_kv_compact_v1(void* k_pool, void* v_pool, int pool_dtype, const int3
 /* The smallest and largest value of each key dim over a page's cached tokens:
  * bounds [num_pages][Hkv][2][D] (lowest, then highest) in the pool's dtype, exact.
  * Refreshes the pages that hold the newest `fresh` tokens of each sequence (fresh
- * >= max_context: all its pages); other entries stay.  NaN keys are passed over. */
+ * >= max_context: all its pages); other entries stay.  NaN keys are passed over; a dim
+ * whose keys are all NaN has NaN bounds. */
 int sfg_hip_kv_page_bounds_v1(const void* k_pool, int pool_dtype, const int32_t* page_table,
                               const int32_t* seq_lens, int64_t max_context, int64_t fresh,
                               void* bounds, int64_t batch, int64_t kv_heads, int64_t head_dim,
@@ -461,8 +462,8 @@ int sfg_hip_kv_page_bounds_v1(const void* k_pool, int pool_dtype, const int32_t*
  * sees, the first sink_pages, the newest recent_pages and the others of the
  * highest score, the sum over the group's query heads and the dims of
  * max(q lo, q hi) -- a bound of the group's summed q.k on the page -- taken in 64
- * bits; ties go to the lower page, NaN scores and pages outside the pool come
- * last.  selected [B][rows][Hkv][top_pages] receives the logical pages ascending,
+ * bits, with infinite bounds and NaN as they are; ties go to the lower page, NaN
+ * scores and pages outside the pool come last.  selected [B][rows][Hkv][top_pages] receives the logical pages ascending,
  * -1 behind.  Rows see the bounds of whole pages, later rows' tokens included.
  * sink_pages + recent_pages <= top_pages. */
 size_t sfg_hip_attn_sparse_workspace_v1(const sfg_paged_attn_args* args, int64_t top_pages);

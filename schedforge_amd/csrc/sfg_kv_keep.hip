@@ -61,6 +61,7 @@ __global__ __launch_bounds__(64) void page_bounds_any_kernel(BoundsArgs a) {
                 lo = fminf(lo, v);
                 hi = fmaxf(hi, v);
             }
+            if (!(lo <= hi)) lo = hi = NAN;  // no key but NaN
             if constexpr (sizeof(KvT) == 4) {
                 out[d] = lo;
                 out[D + d] = hi;
@@ -120,6 +121,7 @@ __global__ __launch_bounds__(64) void page_bounds_kernel(BoundsArgs a) {
             KvT v[2][kEl];
 #pragma unroll
             for (int e = 0; e < kEl; ++e) {
+                if (!(lo[e] <= hi[e])) lo[e] = hi[e] = NAN;  // no key but NaN
                 if constexpr (sizeof(KvT) == 4) {
                     v[0][e] = lo[e];
                     v[1][e] = hi[e];
@@ -407,23 +409,42 @@ __device__ __forceinline__ int row_pages(const PageScoreArgs& a, int b, int row)
     return (max(len - a.rows + row + 1, 0) + a.page_tokens - 1) / a.page_tokens;
 }
 
-// score = sum_d P_d hi_d + N_d lo_d, P and N the group's sums of max(q, 0) and min(q, 0)
-// (which makes the work per page independent of the group's size): P and N to LDS.
+__device__ __forceinline__ double query_at(const PageScoreArgs& a, int b, int head, int row, int d) {
+    const int64_t at = ((static_cast<int64_t>(b) * a.q_heads + head) * a.rows + row) * a.head_dim + d;
+    return a.q_f32 ? static_cast<const float*>(a.q)[at] : bf16_to_f32(static_cast<const uint16_t*>(a.q)[at]);
+}
+
+// The score is the sum over the group's heads and the dims of max(q lo, q hi).  Of numbers that
+// is sum_d P_d hi_d + N_d lo_d, P and N the group's sums of max(q, 0) and min(q, 0), which
+// makes the work per page independent of the group's size: P and N to LDS.  An infinite or
+// NaN bound or query leaves that sum infinite or NaN (P or N times it is, 0 * inf included),
+// and the page is then summed term by term.
 __device__ __forceinline__ void group_query(const PageScoreArgs& a, int b, int h, int row, double* up, double* down) {
     const int D = a.head_dim, G = a.q_heads / a.kv_heads;
     for (int d = threadIdx.x; d < D; d += 256) {
         double hi = 0.0, lo = 0.0;
         for (int g = 0; g < G; ++g) {
-            const int64_t at = ((static_cast<int64_t>(b) * a.q_heads + h * G + g) * a.rows + row) * D + d;
-            const float v = a.q_f32 ? static_cast<const float*>(a.q)[at] : bf16_to_f32(static_cast<const uint16_t*>(a.q)[at]);
-            hi += v > 0.f ? v : 0.f;
-            lo += v < 0.f ? v : 0.f;
+            const double v = query_at(a, b, h * G + g, row, d);
+            hi += v < 0.0 ? 0.0 : v;  // (NaN too)
+            lo += v < 0.0 ? v : 0.0;
         }
         up[d] = hi;
         down[d] = lo;
     }
     __syncthreads();
 }
+
+// The terms of one dim: the larger of q lo and q hi of each head, NaN if either is.
+__device__ __forceinline__ double dim_score(const PageScoreArgs& a, int b, int h, int row, int d, double lo, double hi) {
+    const int G = a.q_heads / a.kv_heads;
+    double s = 0.0;
+    for (int g = 0; g < G; ++g) {
+        const double v = query_at(a, b, h * G + g, row, d), x = v * lo, y = v * hi;
+        s += x != x || x > y ? x : y;
+    }
+    return s;
+}
+__device__ __forceinline__ bool is_number(double s) { return fabs(s) < INFINITY; }
 
 // Any head_dim: workgroups of a (sequence, row, kv head) walk its pages, one wave a page.
 template <typename KvT>
@@ -446,6 +467,11 @@ __global__ __launch_bounds__(256) void page_score_any_kernel(PageScoreArgs a) {
                 s = fma(down[d], static_cast<double>(kv_f32(lo, d)), s);
             }
             s = wave_sum(s);
+            if (!is_number(s)) {
+                s = 0.0;
+                for (int d = lane; d < D; d += 64) s += dim_score(a, b, h, row, d, kv_f32(lo, d), kv_f32(lo, D + d));
+                s = wave_sum(s);
+            }
         } else {
             s = -INFINITY;
         }
@@ -492,10 +518,18 @@ __global__ __launch_bounds__(256) void page_score_kernel(PageScoreArgs a) {
     // pages_per_wave is at most 64: the wave's page ids, one a lane
     const int mine = begin + lane < end ? a.page_table[static_cast<int64_t>(b) * a.pages_per_seq + begin + lane] : -1;
     uint64_t* keys = a.keys + unit * a.max_pages;
+    auto page_sum = [](double s) __attribute__((always_inline)) {  // over the lanes of a page
+        s += lane_xor_f64<1>(s);
+        s += lane_xor_f64<2>(s);
+        s += lane_xor_f64<4>(s);
+        if constexpr (kLanes == 16) s += lane_xor_f64<8>(s);
+        return s;
+    };
     for (int p0 = begin; p0 < end; p0 += kPer * kGroups) {
         constexpr int kV = 8 * sizeof(KvT) / 16;  // vectors of eight dims
         uint4 lo[kGroups][kV], hi[kGroups][kV];
         bool ok[kGroups];
+        int odd = 0;  // bit g: the lane's page of group g has no number as its score
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
             const int page = p0 + g * kPer + sub;
@@ -519,12 +553,24 @@ __global__ __launch_bounds__(256) void page_score_kernel(PageScoreArgs a) {
                 s = fma(P[e], static_cast<double>(kv_f32(u, e)), s);
                 s = fma(N[e], static_cast<double>(kv_f32(l, e)), s);
             }
-            s += lane_xor_f64<1>(s);
-            s += lane_xor_f64<2>(s);
-            s += lane_xor_f64<4>(s);
-            if constexpr (kLanes == 16) s += lane_xor_f64<8>(s);
+            s = page_sum(s);
+            odd |= ok[g] && !is_number(s) ? 1 << g : 0;
             const int page = p0 + g * kPer + sub;
             if (lane % kLanes == 0 && page < end) keys[page] = order_key(ok[g] ? s : -INFINITY);
+        }
+        if (!__any(odd)) continue;
+#pragma unroll 1
+        for (int g = 0; g < kGroups; ++g) {  // (only those: a sum in another order would part equal pages)
+            const int page = p0 + g * kPer + sub;
+            const int id = __shfl(mine, (page - begin) & 63, 64);
+            double s = 0.0;
+            if ((odd >> g) & 1) {
+                const KvT* at = static_cast<const KvT*>(a.bounds) + (static_cast<int64_t>(id) * a.kv_heads + h) * 2 * kD + d0;
+#pragma unroll 1
+                for (int e = 0; e < 8; ++e) s += dim_score(a, b, h, row, d0 + e, kv_f32(at, e), kv_f32(at, kD + e));
+            }
+            s = page_sum(s);
+            if (((odd >> g) & 1) && lane % kLanes == 0) keys[page] = order_key(s);
         }
     }
 }

@@ -407,10 +407,11 @@ int sfg_hip_attn_tree_v1(const sfg_paged_attn_args* args, const uint32_t* tree_m
 /* Causal attention of the newest `rows` tokens (row i sees token j iff
  * j <= L_b - rows + i, as sfg_hip_attn_paged_v1) that also adds to
  * weights[b][g][j], fp32 [B][Hkv][weights_ld], the softmax weight that token j
- * drew, summed over the rows and the query heads of kv head g.  weights_ld >=
- * max_context; entries from L_b on are not touched.  The same call gives the same
- * bits (no atomics).  The workspace holds the scores, 4 bytes per query column
- * and token. */
+ * drew, summed over the rows and the query heads of kv head g (a row that sees
+ * nothing adds nothing; one whose softmax is NaN adds NaN to what it sees).
+ * weights_ld >= max_context; entries from L_b on are not touched.  The same call
+ * gives the same bits (no atomics).  The workspace holds the scores, 4 bytes per
+ * query column and token. */
 size_t sfg_hip_attn_weights_workspace_v1(const sfg_paged_attn_args* args);
 int sfg_hip_attn_weights_v1(const sfg_paged_attn_args* args, float* weights, int64_t weights_ld,
                             void* workspace, size_t workspace_bytes, void* stream);

@@ -12,6 +12,8 @@
 // unit is a (sequence, kv head) with rows x group columns, or for the selected
 // pages a (sequence, row, kv head) with group columns.  Splits of a unit's tokens
 // leave (m, l, acc) partials, merged in split order.
+#include <cfloat>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -20,6 +22,10 @@
 namespace sfg {
 
 namespace {
+
+// A score as the weights' end reads it: -inf is a token that the column does not see, so
+// that one it does see whose score is -inf (weight 0, or NaN where all are) is the lowest number.
+__device__ __forceinline__ float kept_score(float s, bool seen) { return seen && s == -INFINITY ? -FLT_MAX : s; }
 
 // ===========================================================================
 // Any head_dim up to kRowMaxD, any page size, any alignment: one wave per
@@ -86,7 +92,7 @@ __global__ __launch_bounds__(64) void chosen_any_kernel(ChosenArgs p) {
                     s = dot * p.scale_log2;
                 }
             }
-            if constexpr (MODE == kChosenWeights) p.scores[slot * p.scores_ld + j] = s;
+            if constexpr (MODE == kChosenWeights) p.scores[slot * p.scores_ld + j] = kept_score(s, page >= 0);
         }
         const float m_new = fmaxf(m, wave_max(s));
         const float pr = page < 0 ? 0.f : m_new == -INFINITY ? (s == -INFINITY ? 0.f : s) : fast_exp2(s - m_new);
@@ -385,7 +391,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void chosen_mfma_kernel(ChosenArgs p
                 mx = fmaxf(mx, sv[r]);
             }
             if constexpr (MODE == kChosenWeights)
-                if (has) *reinterpret_cast<float4*>(scores + tok0) = make_float4(sv[0], sv[1], sv[2], sv[3]);
+                if (has)
+                    *reinterpret_cast<float4*>(scores + tok0) =
+                        make_float4(kept_score(sv[0], vis & 1u), kept_score(sv[1], vis & 2u), kept_score(sv[2], vis & 4u), kept_score(sv[3], vis & 8u));
             mx = xor16_max(mx);
             mx = xor32_max(mx);
             const float m_new = fmaxf(m_run, mx);
@@ -636,7 +644,7 @@ __global__ __launch_bounds__(64) void chosen_weights_kernel(ChosenArgs p, float*
                 x[c] = make_float2(m, x[c].y * split_weight(x[c].x, m) + y.y * split_weight(y.x, m));
             }
             const float M = wave_max(x[c].x), L = wave_sum(x[c].y * split_weight(x[c].x, M));
-            const float R = L == 0.f ? 0.f : 1.f / L;
+            const float R = L == 0.f ? NAN : 1.f / L;  // (0: every score it sees is -inf)
 #pragma unroll
             for (int t = 0; t < kTok; ++t)
                 if (s[c][t] != -INFINITY) sum[t] = fmaf(fast_exp2(s[c][t] - M), R, sum[t]);

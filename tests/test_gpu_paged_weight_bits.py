@@ -111,3 +111,46 @@ def test_visible_infinite_keys_and_values(d, types):
     compare(lambda n, h, i: sees(c.per * 16, c.lens[n], bits[n, i]))
     weights(lib, c, qd, qdt, out, odt, torch.zeros((2, hkv, 160), device="cuda"))
     compare(lambda n, h, i: np.arange(c.per * 16) < c.lens[n] - t + i + 1)
+
+
+@pytest.mark.parametrize("types", ["bf16/bf16/bf16", "f32/bf16/f32", "f32/f32/f32"])
+@pytest.mark.parametrize("d,pt", [(128, 16), (64, 16), (80, 16), (33, 5)])
+def test_accumulated_weights_of_infinite_scores(d, pt, types):
+    """A token whose score is -inf draws nothing beside others, and NaN where every score that the row sees is -inf
+    (as its output); a row with a score of +inf draws NaN; a row that sees nothing, its length past its place or
+    its pages outside the pool, adds nothing."""
+    lib = _abi.load()
+    qt, kt, ot = types.split("/")
+    rng = np.random.default_rng(d)
+    hq, hkv, rows, lens = 4, 2, 2, (1, 40, 40, 33, 40)
+    c = Cache(rng, lens, 40, hkv, d, pt, kt)
+    c.k[0, 0, 0, 3] = -np.inf        # its only token
+    c.k[1, 1, :, 3] = -np.inf        # every token
+    c.k[2, 0, 7, 3] = -np.inf        # one of many
+    c.k[2, 1, 39, 3] = np.inf        # the newest: only the second row sees it
+    c.upload(c.lens)
+    table = c.table.copy()
+    table[4] = -1
+    c.td = dev(table)
+    q, qd, qdt = queries(rng, c.b, hq, rows, d, qt)
+    q[..., 3] = np.abs(q[..., 3])
+    qd.copy_(torch.from_numpy(q))
+    out, odt = output(q.shape, ot)
+    wd = torch.ones((c.b, hkv, 43), device="cuda")
+    weights(lib, c, qd, qdt, out, odt, wd, 2)
+    got, res = host(wd).astype(np.float64), value(out)
+    for n in range(c.b):
+        for h in range(hkv):
+            want = np.ones(43)
+            for head in (2 * h, 2 * h + 1):
+                for i in range(rows):
+                    s = np.arange(c.per * pt) < lens[n] - rows + i + 1
+                    if not s.any() or n == 4:
+                        assert np.isnan(res[n, head, i]).all()
+                        continue
+                    o, p = formula(q[n, head, i], c.k[n, h], c.v[n, h], s)
+                    np.testing.assert_array_equal(np.isnan(res[n, head, i]), np.isnan(o))
+                    want[: p.size] += p
+            np.testing.assert_array_equal(np.isnan(got[n, h]), np.isnan(want))
+            # four weights, each off by 2 (D + 4) 2^-24 times c sum |q k| (under 20 here) of itself: 1.3e-3 in all
+            assert np.abs(got[n, h] - want)[~np.isnan(want)].max(initial=0.0) < 2.0 ** -9

@@ -141,7 +141,8 @@ def accept_drafts(cache: PagedKVCache, path: torch.Tensor, counts: torch.Tensor,
                   longest: Optional[int] = None, stream: Optional[torch.cuda.Stream] = None) -> None:
     """Keeps the accepted drafts: draft path[b][i] (int32 [B][n], ascending) becomes the i-th token behind
     sequence b's committed ones for i < counts[b], and seq_lens grows by counts.  longest: the most that any
-    sequence accepts, if the host knows it (default: n); cache.length, the bound on all lengths, grows by it."""
+    sequence accepts, if the host knows it (default: n); counts beyond it are cut to it, and cache.length, the
+    bound on all lengths, grows by it."""
     c = cache.config
     if not isinstance(path, torch.Tensor) or path.dim() != 2 or path.shape[1] == 0:
         raise ValueError("path must be a tensor [batch][nodes]")
@@ -154,10 +155,12 @@ def accept_drafts(cache: PagedKVCache, path: torch.Tensor, counts: torch.Tensor,
     lens = _lens(cache, seq_lens)
     if lens is None:
         raise ValueError("accept_drafts needs the sequences' lengths")
+    if longest == 0:
+        return
     with _on(cache, stream) as s:
         check(cache.lib.sfg_hip_kv_compact_v1(
             cache.k_pool.data_ptr(), cache.v_pool.data_ptr(), cache.pool_dtype, cache.table.data_ptr(), lens,
-            path.data_ptr(), 1, n, counts.data_ptr(), lens, n, c.batch, c.kv_heads, c.head_dim, c.page_tokens,
+            path.data_ptr(), 1, n, counts.data_ptr(), lens, longest, c.batch, c.kv_heads, c.head_dim, c.page_tokens,
             c.pages_per_seq, c.num_pages, s))
     cache.alloc.length += longest
 

@@ -1,0 +1,87 @@
+"""The Python layer over the paged operators on the host (no GPU needed): what it hands to the C ABI, what it refuses
+and what it leaves unchanged when it does.  The pools are CPU tensors and the library records the calls."""
+from __future__ import annotations
+
+import contextlib
+
+import pytest
+
+from schedforge_amd.kvcache import PageAllocator, PagedKVConfig
+
+torch = pytest.importorskip("torch")
+
+from schedforge_amd import paged_ops as po  # noqa: E402
+
+
+class Library:
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return 0
+        return call
+
+
+class Cache:
+    """A PagedKVCache without a device."""
+    device, pool_dtype = torch.device("cpu"), 1
+    length = property(lambda self: self.alloc.length)
+    page_table = property(lambda self: self.alloc.page_table)
+
+    def __init__(self, length=40, batch=2, kv_heads=2, d=64, capacity=128):
+        self.config = PagedKVConfig(batch, kv_heads, d, d, 16, capacity)
+        self.alloc, self.lib, self.uploads = PageAllocator(self.config), Library(), 0
+        n = self.config.num_pages
+        self.k_pool = self.v_pool = torch.zeros((n, kv_heads, 16, d), dtype=torch.int16)
+        self.table = torch.zeros((batch, self.config.pages_per_seq), dtype=torch.int32)
+        self.alloc.reserve(length)
+        self.alloc.length = length
+
+    def _sync_table(self, *_):
+        self.uploads += 1
+
+
+@pytest.fixture(autouse=True)
+def host(monkeypatch):
+    @contextlib.contextmanager
+    def on(cache, stream):
+        yield 0
+    monkeypatch.setattr(po, "_on", on)
+
+
+def ints(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+def drafts(t, b=2, h=2, d=64):
+    return torch.zeros((b, h, t, d), dtype=torch.bfloat16)
+
+
+def test_accepted_counts_are_cut_to_the_longest():
+    """The kernel takes the host's bound on the counts, so that no length passes cache.length."""
+    cache = Cache()
+    po.append_drafts(cache, drafts(6), drafts(6), ints(2))
+    po.accept_drafts(cache, ints(2, 6), ints(2), ints(2), longest=3)
+    name, args = cache.lib.calls[-1]
+    assert name == "sfg_hip_kv_compact_v1" and args[7] == 6 and args[10] == 3
+    assert cache.length == 43
+    po.accept_drafts(cache, ints(2, 5), ints(2), ints(2))
+    assert cache.lib.calls[-1][1][10] == 5 and cache.length == 48
+
+
+def test_nothing_accepted_launches_nothing():
+    cache = Cache()
+    po.append_drafts(cache, drafts(6), drafts(6), ints(2))
+    calls = len(cache.lib.calls)
+    po.accept_drafts(cache, ints(2, 6), ints(2), ints(2), longest=0)
+    assert len(cache.lib.calls) == calls and cache.length == 40
+
+
+def test_counts_beyond_the_path_or_the_capacity_are_refused():
+    cache = Cache()
+    for n, longest in ((30, -1), (30, 31), (100, 89)):
+        with pytest.raises(ValueError):
+            po.accept_drafts(cache, ints(2, n), ints(2), ints(2), longest=longest)
+    assert cache.length == 40 and not cache.lib.calls

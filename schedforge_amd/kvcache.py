@@ -142,9 +142,14 @@ class PagedKVCache:
     def free_pages(self) -> List[int]:
         return self.alloc.free_pages
 
-    def _sync_table(self) -> None:
+    def _sync_table(self, wait: bool = True) -> None:
+        """Uploads the tables on the current stream.  wait=False: from pinned memory, which torch's host
+        allocator keeps until the copy is done, so that the host goes on."""
         import torch
-        self.table.copy_(torch.from_numpy(self.alloc.table_array()))
+        rows = torch.from_numpy(self.alloc.table_array())
+        if not wait:
+            rows = torch.empty_like(rows, pin_memory=True).copy_(rows)
+        self.table.copy_(rows, non_blocking=not wait)
 
     def dump(self) -> str:
         return (f"paged_kv batch={self.config.batch} kv_heads={self.config.kv_heads} "

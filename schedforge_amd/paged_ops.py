@@ -6,9 +6,15 @@
 
 The reference has no counterparts: its caches grow at the end and are read whole.
 Tensors stay on the device and no call waits for it; each runs on `stream`, or the
-current one.  Arguments live on the cache's device and are contiguous; a `workspace`
-(uint8, as large as the *_workspace query of the C ABI says) may be passed to calls that
-are captured or repeated, else it is allocated.
+current one, and the caller orders calls on different streams.  Arguments live on the
+cache's device and are contiguous; a `workspace` (uint8, as large as the *_workspace query
+of the C ABI says) may be passed to calls that are captured or repeated, else it is
+allocated.
+
+Calls can be captured, except where pages change hands (append_drafts into pages that are
+not reserved yet, evict_paged_kv): the tables are uploaded there, and a replay would upload
+them again as they are not any more.  A replay leaves the host's side alone: cache.length,
+the bound on all lengths, is what it was when the call was captured.
 
 Sequences may have lengths of their own: `seq_lens` (int32 [B] on the device), none above
 cache.length.  Without it every sequence holds cache.length tokens.
@@ -79,6 +85,11 @@ def _workspace(cache: PagedKVCache, workspace, size: int) -> torch.Tensor:
     return _tensor(cache, workspace, "workspace", torch.uint8, (workspace.numel(),))
 
 
+def _uncaptured(what: str) -> None:
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what} changes the page tables and cannot be captured")
+
+
 # ---------------------------------------------------------------- speculative decoding
 def tree_mask(parents, device="cuda") -> torch.Tensor:
     """Ancestor-or-self bits of drafted trees, int32 words [B][T][ceil(T / 32)] as tree_attention
@@ -109,10 +120,12 @@ def append_drafts(cache: PagedKVCache, keys: torch.Tensor, values: torch.Tensor,
         _tensor(cache, x, name, keys.dtype if keys.dtype in _DTYPES else tuple(_DTYPES), (c.batch, c.kv_heads, t, c.head_dim))
     lens = _lens(cache, seq_lens)
     with _on(cache, stream) as s:
-        have = sum(len(p) for p in cache.page_table)
+        grows = any(len(p) * c.page_tokens < cache.length + t for p in cache.page_table)
+        if grows:
+            _uncaptured("appending into new pages")
         cache.alloc.reserve(t)
-        if sum(len(p) for p in cache.page_table) != have:
-            cache._sync_table()
+        if grows:
+            cache._sync_table(wait=False)
         dt = _DTYPES[keys.dtype]
         check(cache.lib.sfg_hip_kv_append_pool_v1(
             keys.data_ptr(), values.data_ptr(), dt, cache.k_pool.data_ptr(), cache.v_pool.data_ptr(), cache.pool_dtype,
@@ -206,6 +219,8 @@ def evict_paged_kv(cache: PagedKVCache, weights: torch.Tensor, budget: int, rece
         raise ValueError("invalid eviction budget")
     lens = _lens(cache, seq_lens)
     with _on(cache, stream) as s:
+        if budget < cache.length:
+            _uncaptured("eviction")
         keep = torch.empty((c.batch, c.kv_heads, budget), dtype=torch.int32, device=cache.device)
         counts = torch.empty(c.batch, dtype=torch.int32, device=cache.device)
         check(cache.lib.sfg_hip_kv_select_v1(weights.data_ptr(), weights.shape[2], lens, cache.length, budget, recent,
@@ -216,7 +231,7 @@ def evict_paged_kv(cache: PagedKVCache, weights: torch.Tensor, budget: int, rece
                 keep.data_ptr(), c.kv_heads, budget, counts.data_ptr(), counts.data_ptr() if lens is None else lens, budget,
                 c.batch, c.kv_heads, c.head_dim, c.page_tokens, c.pages_per_seq, c.num_pages, s))
             cache.alloc.truncate(budget)
-            cache._sync_table()
+            cache._sync_table(wait=False)
     return keep
 
 

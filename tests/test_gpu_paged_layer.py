@@ -33,3 +33,33 @@ def test_no_length_passes_the_bound_that_the_host_gave():
     assert lens.tolist() == [44, 35] and cache.length == 44
     po.accept_drafts(cache, path, torch.tensor([9, 2], dtype=torch.int32, device="cuda"), lens, longest=0)
     assert lens.tolist() == [44, 35] and cache.length == 44
+
+
+def test_calls_that_change_the_tables_do_not_wait():
+    """Work that takes a while is queued, then drafts are appended into new pages and tokens evicted: both calls come
+    back while the work still runs, and the tables arrive in order."""
+    rng = np.random.default_rng(3)
+    warm, cache = filled(rng), filled(rng)
+    x = bf16(rng, 2, 2, 60, 64)
+    weights = po.attention_weights(cache)
+    weights.uniform_(0.0, 1.0)
+    for c in (warm, cache):
+        w = weights.clone()
+        a = torch.ones((4096, 4096), device="cuda")
+        torch.cuda.synchronize()
+        if c is cache:
+            for _ in range(200):
+                a = a @ a  # (infinite soon, and as slow)
+        busy = torch.cuda.Event()
+        busy.record()
+        po.append_drafts(c, x, x)
+        appended = busy.query()
+        table = c.table.clone()
+        want_appended = c.alloc.table_array()
+        po.evict_paged_kv(c, w, 20, 4)
+        evicted = busy.query()
+        torch.cuda.synchronize()
+        np.testing.assert_array_equal(table.cpu().numpy(), want_appended)
+        np.testing.assert_array_equal(c.table.cpu().numpy(), c.alloc.table_array())
+        if c is cache:
+            assert not appended and not evicted

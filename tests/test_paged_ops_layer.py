@@ -85,3 +85,18 @@ def test_counts_beyond_the_path_or_the_capacity_are_refused():
         with pytest.raises(ValueError):
             po.accept_drafts(cache, ints(2, n), ints(2), ints(2), longest=longest)
     assert cache.length == 40 and not cache.lib.calls
+
+
+def test_calls_that_change_the_tables_are_not_captured(monkeypatch):
+    """A capture is refused before anything is changed where pages change hands, and let through where none do."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    cache = Cache()  # 40 tokens in three pages
+    po.append_drafts(cache, drafts(8), drafts(8), ints(2))
+    with pytest.raises(RuntimeError, match="captured"):
+        po.append_drafts(cache, drafts(9), drafts(9), ints(2))
+    weights = torch.zeros((2, 2, 128))
+    with pytest.raises(RuntimeError, match="captured"):
+        po.evict_paged_kv(cache, weights, 39, 3)
+    po.evict_paged_kv(cache, weights, 40, 3)  # nothing to evict
+    assert cache.uploads == 0 and cache.length == 40 and [len(p) for p in cache.page_table] == [3, 3]
+    assert [name for name, _ in cache.lib.calls] == ["sfg_hip_kv_append_pool_v1", "sfg_hip_kv_select_v1"]

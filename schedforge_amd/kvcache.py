@@ -121,6 +121,8 @@ class PagedKVCache:
         self.alloc = PageAllocator(config)
         self.config = config
         self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())  # where the pools are, whatever is current later
         self.lib = _abi.load()
         n, h, pt, d = config.num_pages, config.kv_heads, config.page_tokens, config.head_dim
         self.pool_dtype = F32 if config.pool_dtype == "f32" else BF16

@@ -38,6 +38,8 @@ _DTYPES = {torch.float32: F32, torch.bfloat16: BF16}
 @contextlib.contextmanager
 def _on(cache: PagedKVCache, stream: Optional[torch.cuda.Stream]):
     """The cache's device and the call's stream, so that what a call allocates is that stream's."""
+    if stream is not None and (not isinstance(stream, torch.cuda.Stream) or stream.device != cache.device):
+        raise ValueError(f"stream must be a torch.cuda.Stream of {cache.device}")
     with torch.cuda.device(cache.device):
         s = stream if stream is not None else torch.cuda.current_stream()
         with torch.cuda.stream(s):
@@ -48,7 +50,7 @@ def _tensor(cache: PagedKVCache, t, name: str, dtypes, shape) -> torch.Tensor:
     dtypes = dtypes if isinstance(dtypes, tuple) else (dtypes,)
     if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
         raise ValueError(f"{name} must be a tensor of {' or '.join(str(d) for d in dtypes)}")
-    if t.device.type != cache.device.type or (cache.device.index is not None and t.device != cache.device):
+    if t.device != cache.device:
         raise ValueError(f"{name} must be on {cache.device}")
     if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous of shape {tuple(shape)}; got {tuple(t.shape)}")

@@ -63,3 +63,15 @@ def test_calls_that_change_the_tables_do_not_wait():
         np.testing.assert_array_equal(c.table.cpu().numpy(), c.alloc.table_array())
         if c is cache:
             assert not appended and not evicted
+
+
+def test_a_cache_knows_its_device():
+    """The device's index is the pools', also where the cache was made on "cuda"; streams are torch's, of that device."""
+    cache = filled(np.random.default_rng(5))
+    assert cache.device == cache.k_pool.device and cache.device.index is not None
+    x = bf16(np.random.default_rng(6), 2, 2, 3, 64)
+    po.append_drafts(cache, x, x, stream=torch.cuda.Stream())
+    for stream in (torch.cuda.current_stream().cuda_stream, "side"):
+        with pytest.raises(ValueError, match="stream"):
+            po.append_drafts(cache, x, x, stream=stream)
+    torch.cuda.synchronize()

@@ -43,6 +43,9 @@ class Cache:
         self.uploads += 1
 
 
+real_on = po._on
+
+
 @pytest.fixture(autouse=True)
 def host(monkeypatch):
     @contextlib.contextmanager
@@ -100,3 +103,21 @@ def test_calls_that_change_the_tables_are_not_captured(monkeypatch):
     po.evict_paged_kv(cache, weights, 40, 3)  # nothing to evict
     assert cache.uploads == 0 and cache.length == 40 and [len(p) for p in cache.page_table] == [3, 3]
     assert [name for name, _ in cache.lib.calls] == ["sfg_hip_kv_append_pool_v1", "sfg_hip_kv_select_v1"]
+
+
+def test_tensors_and_streams_of_another_device_are_refused(monkeypatch):
+    cache = Cache()
+    cache.device = torch.device("cuda", 1)
+    with pytest.raises(ValueError, match="cuda:1"):
+        po.append_drafts(cache, drafts(3), drafts(3))
+    with pytest.raises(ValueError, match="cuda:1"):
+        po._tensor(cache, torch.empty(2, device="meta"), "query", torch.float32, (2,))
+
+    class Stream:
+        def __init__(self, index):
+            self.device = torch.device("cuda", index)
+    monkeypatch.setattr(torch.cuda, "Stream", Stream)
+    for stream in (Stream(0), 12345, "side"):
+        with pytest.raises(ValueError, match="stream"):
+            with real_on(cache, stream):
+                pass

@@ -61,7 +61,8 @@ def _lens(cache: PagedKVCache, seq_lens) -> Optional[int]:
     return None if seq_lens is None else _tensor(cache, seq_lens, "seq_lens", torch.int32, (cache.config.batch,)).data_ptr()
 
 
-def _args(cache: PagedKVCache, query, out, seq_lens, kv_splits: int, scale: float) -> _abi.PagedAttnArgs:
+def _args(cache: PagedKVCache, query, out, seq_lens, kv_splits: int, scale: float):
+    """The argument block, and the output (made like the query if not given)."""
     c = cache.config
     if not isinstance(query, torch.Tensor) or query.dim() != 4:
         raise ValueError("query must be a tensor [batch][q_heads][rows][head_dim]")
@@ -69,7 +70,7 @@ def _args(cache: PagedKVCache, query, out, seq_lens, kv_splits: int, scale: floa
     if hq <= 0 or hq % c.kv_heads:
         raise ValueError("invalid attention configuration")
     _tensor(cache, query, "query", tuple(_DTYPES), (c.batch, hq, rows, c.head_dim))
-    _tensor(cache, out, "out", tuple(_DTYPES), query.shape)
+    out = torch.empty_like(query) if out is None else _tensor(cache, out, "out", tuple(_DTYPES), query.shape)
     a = _abi.PagedAttnArgs()
     a.q, a.q_dtype = query.data_ptr(), _DTYPES[query.dtype]
     a.k_pool, a.v_pool, a.kv_dtype = cache.k_pool.data_ptr(), cache.v_pool.data_ptr(), cache.pool_dtype
@@ -78,13 +79,13 @@ def _args(cache: PagedKVCache, query, out, seq_lens, kv_splits: int, scale: floa
     a.batch, a.q_heads, a.kv_heads, a.rows, a.head_dim = c.batch, hq, c.kv_heads, rows, c.head_dim
     a.page_tokens, a.pages_per_seq, a.num_pages = c.page_tokens, c.pages_per_seq, c.num_pages
     a.max_context, a.kv_splits, a.scale = cache.length, kv_splits, scale
-    return a
+    return a, out
 
 
 def _workspace(cache: PagedKVCache, workspace, size: int) -> torch.Tensor:
     if workspace is None:
         return torch.empty(max(size, 1), dtype=torch.uint8, device=cache.device)
-    return _tensor(cache, workspace, "workspace", torch.uint8, (workspace.numel(),))
+    return _tensor(cache, workspace, "workspace", torch.uint8, workspace.shape if isinstance(workspace, torch.Tensor) else ())
 
 
 def _uncaptured(what: str) -> None:
@@ -141,8 +142,7 @@ def tree_attention(cache: PagedKVCache, query: torch.Tensor, mask: torch.Tensor,
     """Attention of drafted tokens (append_drafts) over the committed ones and each other: query
     [B][Hq][T][D]; row t sees draft u iff its bit in mask ([B or 1][T][ceil(T / 32)] int32, tree_mask) is set."""
     with _on(cache, stream) as s:
-        out = torch.empty_like(query) if out is None else out
-        a = _args(cache, query, out, seq_lens, kv_splits, scale)
+        a, out = _args(cache, query, out, seq_lens, kv_splits, scale)
         b, w = cache.config.batch, -(-a.rows // 32)
         shared = isinstance(mask, torch.Tensor) and mask.dim() == 3 and mask.shape[0] == 1
         _tensor(cache, mask, "mask", torch.int32, (1 if shared else b, a.rows, w))
@@ -199,8 +199,7 @@ def weighted_decode_attention(cache: PagedKVCache, query: torch.Tensor, weights:
     (attention_weights) what each cached token drew, summed over the rows and the heads of its kv head."""
     _weights(cache, weights)
     with _on(cache, stream) as s:
-        out = torch.empty_like(query) if out is None else out
-        a = _args(cache, query, out, seq_lens, kv_splits, scale)
+        a, out = _args(cache, query, out, seq_lens, kv_splits, scale)
         ws = _workspace(cache, workspace, cache.lib.sfg_hip_attn_weights_workspace_v1(ctypes.byref(a)))
         check(cache.lib.sfg_hip_attn_weights_v1(ctypes.byref(a), weights.data_ptr(), weights.shape[2], ws.data_ptr(),
                                                 ws.numel(), s))
@@ -280,8 +279,7 @@ def sparse_decode_attention(cache: PagedKVCache, query: torch.Tensor, bounds: to
     if top_pages <= 0:
         raise ValueError("sparse attention reads at least one page")
     with _on(cache, stream) as s:
-        out = torch.empty_like(query) if out is None else out
-        a = _args(cache, query, out, seq_lens, kv_splits, scale)
+        a, out = _args(cache, query, out, seq_lens, kv_splits, scale)
         shape = (c.batch, a.rows, c.kv_heads, top_pages)
         selected = torch.empty(shape, dtype=torch.int32, device=cache.device) if selected is None else selected
         _tensor(cache, selected, "selected", torch.int32, shape)

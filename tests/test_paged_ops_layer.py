@@ -6,6 +6,7 @@ import contextlib
 
 import pytest
 
+from schedforge_amd._abi import BF16
 from schedforge_amd.kvcache import PageAllocator, PagedKVConfig
 
 torch = pytest.importorskip("torch")
@@ -26,7 +27,7 @@ class Library:
 
 class Cache:
     """A PagedKVCache without a device."""
-    device, pool_dtype = torch.device("cpu"), 1
+    device, pool_dtype = torch.device("cpu"), BF16
     length = property(lambda self: self.alloc.length)
     page_table = property(lambda self: self.alloc.page_table)
 
@@ -121,3 +122,18 @@ def test_tensors_and_streams_of_another_device_are_refused(monkeypatch):
         with pytest.raises(ValueError, match="stream"):
             with real_on(cache, stream):
                 pass
+
+
+def test_arguments_that_are_no_tensors_are_refused():
+    cache, q = Cache(), torch.zeros((2, 4, 3, 64))
+    mask, weights, bounds = ints(2, 3, 1), torch.zeros((2, 2, 128)), torch.zeros((cache.config.num_pages, 2, 2, 64), dtype=torch.bfloat16)
+    calls = [("query", dict(query=None)), ("query", dict(query=q.numpy())), ("query", dict(query=q[0])), ("query", dict(query=q[..., ::2])),
+             ("out", dict(out=q.numpy())), ("out", dict(out=q[:, :2])), ("workspace", dict(workspace=bytes(8))), ("workspace", dict(workspace=64)),
+             ("workspace", dict(workspace=torch.zeros(8)))]
+    for name, bad in calls:
+        a = dict(query=q, **bad) if name != "query" else bad
+        for call in (lambda: po.tree_attention(cache, mask=mask, **a), lambda: po.weighted_decode_attention(cache, weights=weights, **a),
+                     lambda: po.sparse_decode_attention(cache, bounds=bounds, top_pages=4, **a)):
+            with pytest.raises(ValueError, match=name):
+                call()
+    assert not any("workspace" not in name for name, _ in cache.lib.calls)

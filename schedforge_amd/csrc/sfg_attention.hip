@@ -1914,14 +1914,21 @@ int launch_kv_append(const void* keys, const void* values, int src_dtype, int64_
     a.num_pages = static_cast<int>(num_pages);
     const dim3 grid(static_cast<unsigned>(tokens), static_cast<unsigned>(kv_heads), static_cast<unsigned>(batch));
     const int64_t spans = (tokens + 2 * kPageTok - 2) / kPageTok;  // pages that a run of tokens can touch
-    if (!rope && tokens > 1 && page_tokens == kPageTok && spans <= 65535 &&
+    // rows of the pool's type that start and end on 16-byte boundaries move as vectors
+    const int64_t per = pool_dtype == SFG_F32 ? 4 : 8, units = batch * kv_heads;
+    const int vec = src_dtype == pool_dtype && head_dim % per == 0 && sb % per == 0 && sh % per == 0 && st % per == 0 &&
+                    ((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(k_pool)) & 15) == 0;
+    // By pages from 2048 rows of at least 4 tokens on, 16384 of 8 where rows are converted.
+    // With fewer, a wave a token is sooner done: us by tokens and by pages, bf16 at head_dim
+    // 128, 8 (sequence, head)s x 64 tokens 3.1 and 3.3, 128 x 4 3.2 and 3.2, 128 x 16 4.6 and
+    // 3.8, 1024 x 3 6.2 and 6.5, 1024 x 4 7.2 and 6.8; fp32 into bf16, 128 x 32 6.1 and 6.7,
+    // 128 x 128 13.3 and 12.0 (head_dim 256: 128 x 64 13.4 and 18.0, 128 x 128 23.9 and 21.5).
+    const bool by_pages = tokens >= (vec ? 4 : 8) && units * tokens >= (vec ? 2048 : 16384);
+    // (a launch holds fewer than 2^32 threads a dimension)
+    if (!rope && by_pages && page_tokens == kPageTok && spans <= 65535 && units < (1 << 24) &&
         (reinterpret_cast<uintptr_t>(v_pool) & 15) == 0) {
-        const dim3 pgrid(static_cast<unsigned>(batch * kv_heads), static_cast<unsigned>(spans));
+        const dim3 pgrid(static_cast<unsigned>(units), static_cast<unsigned>(spans));
         const int n = static_cast<int>(tokens);
-        // rows of the pool's type that start and end on 16-byte boundaries move as vectors
-        const int64_t per = pool_dtype == SFG_F32 ? 4 : 8;
-        const int vec = src_dtype == pool_dtype && head_dim % per == 0 && sb % per == 0 && sh % per == 0 && st % per == 0 &&
-                        ((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(k_pool)) & 15) == 0;
         if (pool_dtype == SFG_F32) {
             if (a.src_f32) kv_append_pages_kernel<float, float><<<pgrid, 256, 0, stream>>>(a, n, vec);
             else kv_append_pages_kernel<float, uint16_t><<<pgrid, 256, 0, stream>>>(a, n, vec);

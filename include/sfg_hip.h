@@ -397,8 +397,11 @@ typedef struct {
  * ceil(rows / 32), is set: for a tree, u is t or one of its ancestors.  The mask is
  * taken as it is (a row does not see itself unless its bit says so).  mask_stride
  * 0: one mask for all sequences, else at least rows * W words.  The tables must
- * cover max_context + rows tokens.  Trees of many query columns over many tokens
- * take up to 70 MB of workspace. */
+ * cover max_context + rows tokens.  Keys and queries come rotated, a draft at
+ * seq_lens[b] + its depth: sfg_hip_qkv_split_rope_v1 takes a table with a row per
+ * draft, but the same one for every sequence of its batch.  With kv_splits <= 0
+ * trees of many query columns over many tokens take up to 70 MB of workspace; a
+ * requested count takes what the query says (270 MB and more). */
 size_t sfg_hip_attn_tree_workspace_v1(const sfg_paged_attn_args* args);
 int sfg_hip_attn_tree_v1(const sfg_paged_attn_args* args, const uint32_t* tree_mask,
                          int64_t mask_stride, void* workspace, size_t workspace_bytes,
@@ -409,7 +412,9 @@ int sfg_hip_attn_tree_v1(const sfg_paged_attn_args* args, const uint32_t* tree_m
  * weights[b][g][j], fp32 [B][Hkv][weights_ld], the softmax weight that token j
  * drew, summed over the rows and the query heads of kv head g (a row that sees
  * nothing adds nothing; one whose softmax is NaN adds NaN to what it sees).
- * weights_ld >= max_context; entries from L_b on are not touched.  The same call
+ * weights_ld >= max_context; entries from L_b on are not touched: where a cache is
+ * truncated the caller zeroes those of the tokens that go, or the next ones there
+ * inherit them.  The same call
  * gives the same bits (no atomics).  The workspace holds the scores, 4 bytes per
  * query column and token. */
 size_t sfg_hip_attn_weights_workspace_v1(const sfg_paged_attn_args* args);
@@ -437,8 +442,11 @@ int sfg_hip_kv_select_v1(const float* weights, int64_t weights_ld, const int32_t
  * kv_heads (evictions, base NULL), ascending; an entry below its index or past the
  * capacity moves nothing.  A page that receives tokens is written as a whole, with
  * its unmoved elements as they were: nothing else may write to it meanwhile.
- * Tokens are rotated already: they keep their original positions' RoPE.  new_lens
- * may be base or counts.  No page may be in two tables.  Page bounds of moved
+ * Tokens are rotated already: they keep their original positions' RoPE.  After an
+ * eviction a sequence's length is therefore not its next token's position: the
+ * caller counts positions, rotates new tokens there and appends them
+ * (sfg_hip_kv_append_pool_v1); the layer's kv_append mode, which rotates at the
+ * cached length, is not for such caches.  new_lens may be base or counts.  No page may be in two tables.  Page bounds of moved
  * tokens must be made anew. */
 int sfg_hip_kv_compact_v1(void* k_pool, void* v_pool, int pool_dtype, const int32_t* page_table,
                           const int32_t* base, const int32_t* keep, int64_t keep_heads,

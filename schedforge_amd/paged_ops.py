@@ -18,6 +18,13 @@ the bound on all lengths, is what it was when the call was captured.
 
 Sequences may have lengths of their own: `seq_lens` (int32 [B] on the device), none above
 cache.length.  Without it every sequence holds cache.length tokens.
+
+Keys and queries come rotated (RoPE): drafts at their sequence's length plus their depth in
+the tree.  Tokens that move keep their rotation, so after an eviction a token's position is
+the caller's count, not its place in the cache.
+
+The pools of a compiled layer (DecoderExecutablePlan.t) are no PagedKVCache: its callers use
+the C ABI.
 """
 from __future__ import annotations
 
@@ -182,7 +189,8 @@ def accept_drafts(cache: PagedKVCache, path: torch.Tensor, counts: torch.Tensor,
 
 # ---------------------------------------------------------------- eviction by accumulated weight
 def attention_weights(cache: PagedKVCache) -> torch.Tensor:
-    """Accumulators of the cache's tokens, fp32 [B][Hkv][pages_per_seq * page_tokens], zero."""
+    """Accumulators of the cache's tokens, fp32 [B][Hkv][pages_per_seq * page_tokens], zero.  Entries behind the
+    cached tokens have to be zero: evict_paged_kv leaves them so, after truncate_paged_kv the caller clears them."""
     c = cache.config
     return torch.zeros((c.batch, c.kv_heads, c.pages_per_seq * c.page_tokens), dtype=torch.float32, device=cache.device)
 

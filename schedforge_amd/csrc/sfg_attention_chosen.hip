@@ -603,8 +603,8 @@ __global__ __launch_bounds__(256) void chosen_combine_kernel(ChosenArgs p, int c
 // time, their scores and (m, l) loaded together, lane s merging split s (and s + 64, ...);
 // the wave adds sum_columns 2^(s - M) / L to its tokens' accumulators.  The workgroups past
 // the tokens merge the output columns.  A column that sees nothing adds nothing.  Latency,
-// not bytes (4 G of scores and 8 of accumulator a token), bounds it: 7.2 us for 32 x 4
-// heads x up to 8192 tokens, 5.9 for 8 heads x 4096.
+// not bytes (4 G of scores and 8 of accumulator a token), bounds it: 7.0 us for 32 x 4
+// heads x up to 8192 tokens, 5.8 for 8 heads x 4096.
 __global__ __launch_bounds__(64) void chosen_weights_kernel(ChosenArgs p, float* weights, int64_t ld, int chunks) {
     constexpr int kTok = 4, kCols = 4;  // tokens a lane, columns at a time
     const Unit<kChosenWeights> u = unit_of<kChosenWeights>(p, blockIdx.x / p.kv_heads, blockIdx.x % p.kv_heads);
@@ -726,8 +726,10 @@ ChosenPlan plan_chosen(int mode, bool bf16, bool ragged, int64_t batch, int64_t 
         while (base * s < 1024 && most / (s * 2) >= 256) s *= 2;
     } else if (mode != kChosenWeights && most <= 64 && base >= 128) {
         // half of the CUs busy and up to eight pages a wave: no splits to merge, one launch
-        // less (16 x 8 kv heads x 64 selected pages: 19.5 us with four splits and their merge,
-        // 16.6 so; 16 units of 57 pages: 11.2 us with eight splits, 16.6 so)
+        // less.  Whole sparse calls so and with splits, us: 128 units of 16 pages 16.4 and 18.7,
+        // of 64 26.8 and 29.6, of 128 38.8 and 40.3, of 192 52.3 and 52.1; 96 units of 64 27.0 and
+        // 27.9, 64 units 26.1 and 23.8, 32 units 24.0 and 18.3; 256 units 37.0 and 41.1, 512
+        // units 67.0 and 63.6
         plan.waves = 8;
     } else {
         // two workgroups per CU while a split keeps 8 pages, two per wave (tree: 4; 1 x 8 kv

@@ -24,10 +24,11 @@
 // chunk) as long as its tiles and kStart more for its start, workgroup w of W takes the
 // range [N w / W, N (w + 1) / W), at most two of whose runs are parts of a longer one;
 // those leave (m, l, acc) partials, and a second kernel joins them in tile order.
-// 64 drafts x 4 heads a kv head, 16 x 8 kv heads x up to 8192 tokens: 123 us and 19 of the
-// join (174 and 43 with two equal splits a sequence); the matrix pipe is 32% busy there,
-// fragment reads take LDS 2048 of a tile's 5000 cycles, and starts and partials cost the
-// rest.  32 drafts, 8 x 8 x up to 4096: 28 and 9 us.
+// 64 drafts x 4 heads a kv head, 16 x 8 kv heads x up to 8192 tokens: 121 us and 15 of the
+// join once the clock has settled (up to 170 in the first milliseconds of a run).  That
+// is 260 thousand cycles for 36 tiles a workgroup and its starts: the matrix pipe is 43% busy,
+// and a tile's fragments, 256 KB at 128 bytes a cycle, take LDS 2048 cycles.  32 drafts,
+// 8 x 8 x up to 4096: 29 and 9 us for 80 MB, the starts more of it.
 //
 // Tokens that some column does not see (drafts, the end, pages of no id) sit in the
 // last tiles: there each lane builds the 64 bits of what its column sees, and non-finite
@@ -45,11 +46,13 @@ namespace {
 constexpr int kTileTok = 64;
 // What starting a (sequence, kv head, chunk) costs, in tiles: its queries, mask and first
 // tiles are waited for, the sums before it are written (at 0, 16 x 8 heads x up to 8192
-// tokens with 64 drafts took 160 us, where one workgroup had five short sequences; 126 so).
+// tokens with 64 drafts take 169 us, where one workgroup has five short sequences; 138 so,
+// both with the join).
 constexpr int kStart = 6;
 // The least length of a workgroup's range: shorter ones cost more in starts, and in parts
-// to join, than they give (8 heads x 8000 tokens, 64 columns: 45 us at 2, 37 at 4, 34 at 6,
-// 36 at 8; 8 heads x 900: 18, 19, 21, 23).
+// to join, than they give (us at 2, 4, 5, 6 and 8; 2 x 8 heads x 8000 tokens, 64 columns:
+// 40, 40, 38, 37, 38; 16 x 8 x up to 900: 27.2, 26.2, 26.3, 27.9, 30.5; 4 x 8 x up to 2000, 128
+// columns: 29.3, 28.8, 27.8, 29.1, 30.9).
 constexpr int kLeast = 5;
 
 __device__ __forceinline__ int swap_bits23(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
@@ -565,9 +568,12 @@ TreeTiles plan_tree_tiles(int64_t batch, int64_t kv_heads, int64_t cols, int64_t
     t.chunks = (cols + t.cols - 1) / t.cols;
     const int64_t units = batch * kv_heads * t.chunks, tiles = (keys + kTileTok - 1) / kTileTok;
     // Against the 16-column kernel, which reads K and V once per 16 columns but starts sooner:
-    // by the bytes that one reads.  64 columns: 1 x 8 kv heads x 8000 tokens 22.5 us there,
-    // 35 here; 16 x 8 x 900 31 and 27; 128 columns: 4 x 8 x 2000 32 and 28, 16 x 4 heads of
-    // 64 dims x 900 19 and 21, 16 x 8 x 8000 345 and 82.
+    // by the bytes that one reads.  64 columns: 1 x 8 kv heads x 8000 tokens 23 us there,
+    // 36 here, 2 x 8 x 8000 32 and 38; 16 x 8 x up to 900 31 and 26; 128 columns: 4 x 8 x up to
+    // 2000 33 and 28, 16 x 4 heads of 64 dims x up to 900 17 and 21, 16 x 8 x up to 8000 224 and
+    // 83.  Over 516 random trees of 150 K to 6 M such reads the choice is 4% slower than the
+    // better kernel of each on average (3% from 500 K on), 2.0 times at worst; by the tile
+    // kernel alone 18%, by the other alone 21%.
     if (cols < 8) return t;
     const int64_t reads = (cols + 15) / 16 * batch * kv_heads * tiles * head_dim;
     if (requested <= 0 && reads < 960 * 1024) return t;

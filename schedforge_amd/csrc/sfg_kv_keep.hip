@@ -76,7 +76,7 @@ __global__ __launch_bounds__(64) void page_bounds_any_kernel(BoundsArgs a) {
 // head_dim 64 / 128, 16-token pages: a row is read as 16-byte vectors, 64 of them a load of
 // the wave, all of the page's loads before the first comparison (slots past the end
 // re-read the last token); lanes of the same vector and other tokens meet by shuffles.
-// 3.7 us for the newest page of 16 x 8 heads (12.0 with the loads one by one), 4.3 for all
+// 3.7 us for the newest page of 16 x 8 heads (12.0 with the loads one by one), 4.5 for all
 // of 2 x 4 heads x 6000 tokens.
 template <typename KvT, int kD>
 __global__ __launch_bounds__(64) void page_bounds_kernel(BoundsArgs a) {
@@ -493,8 +493,9 @@ __device__ __forceinline__ double lane_xor_f64(double v) {
 
 // head_dim 64 / 128: 8 or 16 lanes a page, eight dims each, their P and N in registers;
 // a wave takes 8 or 4 pages at a time, four such groups' bounds in flight.  Bound by
-// reading the bounds (4 D bytes a bf16 page and head): 134 MB, 16 x 8 heads x up to 2048
-// pages, in 18 us from a warm cache; the 2 D double-precision FMAs a page stay under it.
+// reading the bounds (4 D bytes a bf16 page and head): 74 MB, 16 x 8 heads x up to 2048
+// pages (lengths of their own), in 18 us from a warm cache, 4.0 TB/s; the 2 D
+// double-precision FMAs a page stay under it.
 template <typename KvT, int kD>
 __global__ __launch_bounds__(256) void page_score_kernel(PageScoreArgs a) {
     constexpr int kLanes = kD / 8, kPer = 64 / kLanes, kGroups = 4;
@@ -681,8 +682,9 @@ __global__ __launch_bounds__(256) void kv_compact_any_kernel(CompactArgs a) {
 // its own -- K by vectors of a row, V by dims -- and a workgroup walks its slice's
 // destinations in order.  The sources of 2048 tokens at a time are looked up first
 // (list, then table) and kept in LDS, so that a chunk's loads wait on nothing else.
-// 16 x 8 heads, 4096 tokens to 2048: 81 us for 201 MB read (the kept K rows, all of V's
-// lines) and 134 written, 104 together with the selection where nothing is cached.  Not
+// 16 x 8 heads, up to 4096 tokens to 2048: 80 us for 178 MB read (the kept K rows, V's
+// lines that hold kept tokens) and 134 written, 104 together with the selection where
+// nothing is cached.  Not
 // faster: finer slices (129 us at 1024 workgroups), the next chunk's loads before this
 // one's stores (110), V as 16-byte vectors shared by a page's tokens (110).
 //   K: a thread moves one vector of each of 8 tokens a chunk.

@@ -61,7 +61,8 @@ enum sfg_status {
     SFG_ERR_WORKSPACE = 17      /* workspace too small                           */
 };
 
-enum sfg_dtype { SFG_F32 = 0, SFG_BF16 = 1, SFG_I8 = 2, SFG_I32 = 3 /* taps only */ };
+enum sfg_dtype { SFG_F32 = 0, SFG_BF16 = 1, SFG_I8 = 2, SFG_I32 = 3 /* taps only */,
+                 SFG_FP8 = 4 /* e4m3, 8-bit caches only */ };
 
 enum sfg_layout { SFG_LAYOUT_NK = 0, SFG_LAYOUT_TILED = 1 };
 
@@ -479,6 +480,148 @@ size_t sfg_hip_attn_sparse_workspace_v1(const sfg_paged_attn_args* args, int64_t
 int sfg_hip_attn_sparse_v1(const sfg_paged_attn_args* args, const void* bounds, int64_t top_pages,
                            int64_t sink_pages, int64_t recent_pages, int32_t* selected,
                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------- a step over a paged cache held in 8 bits ----------------
+ * No counterparts in the reference.  A serving step in four calls, with nothing on
+ * the host: which tokens and pages (kv_plan), queries and keys rotated at their
+ * positions (rope), keys and values stored in 8 bits (kv8_append), attention
+ * (attn_kv8).  Its tokens are packed: T rows, sequence b's from starts[b] to
+ * starts[b + 1].  Common to all:
+ *   - no call allocates, copies to the host, waits for the device or records anything
+ *     but kernels, so a step can be captured into a graph and replayed with other
+ *     lengths and counts;
+ *   - device-side indices are clamped or skipped, never followed out of range;
+ *   - rows behind the last sequence (padding to a captured size) carry position and
+ *     slot -1 and are left as they were.
+ *
+ * The cache: K pool [page][Hkv][page_tokens][D] and V pool [page][Hkv][D][page_tokens] of
+ * one-byte codes, SFG_I8 (-127 .. 127) or SFG_FP8 (e4m3: 4 exponent and 3 mantissa bits,
+ * largest 448), and scales fp32 [page][Hkv][2] (K's, V's).  A stored value is
+ * code * scale. */
+
+/* Pages given back, pages taken, and where each new token goes.  In order:
+ *   release  sequence b keeps its first keep[b] tokens (NULL: all; clamped to
+ *            [0, seq_lens[b]]).  Pages behind them go back on the free list, sequences
+ *            ascending, each one's last page first, and their entries become -1;
+ *   grant    sequence b asks for counts[b] tokens (negative: 0) and the pages they need.
+ *            It gets all of them or none: none past the table's capacity, none that
+ *            would make the rows asked for so far exceed max_tokens, and, where it needs
+ *            pages, none if the pages asked for so far exceed the free ones.  ("So far":
+ *            by sequences 0 .. b, refused ones included, those past their capacity not:
+ *            one that does not fit stops the later ones that need what it waited for.)
+ *            Pages come off the end of the free list, for sequences and pages ascending.
+ * seq_lens becomes the kept plus the granted tokens, starts[b] the rows of the sequences
+ * before b (starts[batch]: of all; a sequence got nothing where starts[b + 1] ==
+ * starts[b]); positions[t] and slots[t] = page * page_tokens + position % page_tokens for
+ * the rows in order, -1 behind the last.  free_pages [num_pages] is a stack of
+ * *free_count entries; those behind stay.  Page ids move as they are; slots on one outside
+ * the pool are -1.  Lists and tables are written in place; none may overlap another. */
+typedef struct {
+    const int32_t* keep;         /* [B] or NULL */
+    const int32_t* counts;       /* [B] */
+    int32_t* seq_lens;           /* [B] */
+    int32_t* page_table;         /* [B][pages_per_seq] */
+    int32_t* free_pages;         /* [num_pages] */
+    int32_t* free_count;         /* [1] */
+    int32_t* starts;             /* [B + 1] */
+    int32_t* positions;          /* [max_tokens] */
+    int64_t* slots;              /* [max_tokens] */
+    int64_t batch, pages_per_seq, num_pages, page_tokens, max_tokens;
+} sfg_kv_plan_args;
+int sfg_hip_kv_plan_v1(const sfg_kv_plan_args* args, void* stream);
+
+/* Angles per position of rotary pairs for scaled contexts: inv_freq [rotary_dim / 2] and the
+ * factor on cosine and sine, computed on the host in 64 bits.  With w_i = theta^(-2 i / R), R
+ * the rotary dim, s the factor and r_i = context w_i / (2 pi) the turns over the context that
+ * the weights were trained on:
+ *   PLAIN   w_i;  LINEAR  w_i / s;  BASE  theta becomes theta s^(R / (R - 2));
+ *   BANDS   w_i (t + (1 - t) / s), t = (r_i - low) / (high - low) in [0, 1];
+ *   RAMP    w_i (1 - t + t / s), t = (i - a) / max(b - a, 0.001) in [0, 1], a the floor (at
+ *           least 0) of d(high) and b the ceiling (at most R - 1) of d(low), d(x) =
+ *           R ln(context / (2 pi x)) / (2 ln theta): the pair that turns x times; the
+ *           factor on cosine and sine is 0.1 ln s + 1. */
+enum sfg_rope_scaling_kind { SFG_ROPE_PLAIN = 0, SFG_ROPE_LINEAR = 1, SFG_ROPE_BASE = 2, SFG_ROPE_BANDS = 3, SFG_ROPE_RAMP = 4 };
+typedef struct {
+    int32_t kind;
+    double theta, factor;        /* factor >= 1 */
+    double context, low, high;   /* BANDS, RAMP: 0 < low < high */
+} sfg_rope_scaling;
+int sfg_hip_rope_inv_freq_host_v1(double* inv_freq, float* magnitude, int64_t rotary_dim,
+                                  const sfg_rope_scaling* scaling);
+/* The same angles as turns per position in 64-bit fixed point, round(inv_freq 2^64 / (2 pi))
+ * modulo 2^64: a position times it wraps as whole turns do, so that the angle of any
+ * position is known to 2^-33 turns. */
+int sfg_hip_rope_turns_host_v1(uint64_t* turns, const double* inv_freq, int64_t pairs);
+
+/* Rotary positions.  Of each head of row t the first rotary_dim values are pairs that are
+ * turned by positions[t] * inv_freq_i and multiplied by `magnitude`; the others are copied.
+ * Pair i is values (i, i + rotary_dim / 2) in the HALF layout, (2 i, 2 i + 1) in the
+ * INTERLEAVED one.  q [T][Hq][D] and k [T][Hkv][D] have strides of their own between
+ * rows (in elements, at least Hq D and Hkv D): parts of a QKV product's rows, say; either may
+ * be absent (NULL, 0 heads).  An output may be its input (same pointer and stride), and
+ * overlaps nothing else.  Rows of negative positions are left as they were. */
+enum sfg_rope_layout { SFG_ROPE_HALF = 0, SFG_ROPE_INTERLEAVED = 1 };
+typedef struct {
+    const void* q; const void* k; void* q_out; void* k_out; int32_t dtype;  /* SFG_F32 or SFG_BF16 */
+    int64_t q_stride, k_stride, q_out_stride, k_out_stride;
+    const int32_t* positions;    /* [T] */
+    const uint64_t* turns;       /* [rotary_dim / 2], device */
+    float magnitude; int32_t layout;
+    int64_t tokens, q_heads, kv_heads, head_dim, rotary_dim;
+} sfg_rope_args;
+int sfg_hip_rope_v1(const sfg_rope_args* args, void* stream);
+
+/* Keys and values [T][Hkv][D] (row strides in elements, at least Hkv D) stored at slots[t]
+ * (outside [0, num_pages page_tokens): the row is skipped).  The rows that a call stores
+ * into one page lie side by side, their slots ascending by one; otherwise that page
+ * holds nothing defined.  For K and V of each page and kv head alone:
+ *   - a run that begins at the page's first slot begins a new scale, any other one goes
+ *     on from the scale that is there;
+ *   - the scale becomes the larger of that and absmax / M over the run's values, M = 127
+ *     or 448, the quotient rounded to fp32.  It never shrinks;
+ *   - where it grew, the page's earlier tokens are coded anew: code * old scale, in fp32, as a
+ *     new value;
+ *   - a value's code is value / scale, rounded to fp32, then to the nearest code (ties to
+ *     even), cut to +-M; 0 under the scale 0.
+ * A NaN or an infinity among a run's values makes the scale NaN, and with it all that the
+ * page and head hold, until a run begins it anew.  Tokens behind the run stay as they are. */
+typedef struct {
+    const void* keys; const void* values; int32_t dtype;                    /* SFG_F32 or SFG_BF16 */
+    int64_t key_stride, value_stride;
+    void* k_pool; void* v_pool; int32_t pool_dtype;                         /* SFG_I8 or SFG_FP8 */
+    float* scales;               /* [num_pages][Hkv][2] */
+    const int64_t* slots;        /* [T] */
+    int64_t tokens, kv_heads, head_dim, page_tokens, num_pages;
+} sfg_kv8_append_args;
+int sfg_hip_kv8_append_v1(const sfg_kv8_append_args* args, void* stream);
+
+/* Causal attention of each sequence's newest rows over its cache: with R = starts[b + 1] -
+ * starts[b] rows and L = seq_lens[b] tokens (clamped to [0, max_context]; the rows' own
+ * tokens included), row i sees token j iff j <= L - R + i.  q and out [T][Hq][D] with row
+ * strides in elements, at least Hq D; out is not q.  starts NULL: every sequence has
+ * max_rows rows, T = batch * max_rows.  max_rows bounds the rows of any sequence: those
+ * past it are not computed.  A row that sees nothing comes out NaN (0 / 0); tokens on a
+ * page whose id is outside the pool are not seen; what no row sees may hold anything.
+ * kv_splits <= 0 picks how far sequences are split, scale <= 0 means 1 / sqrt(D).  Scores,
+ * softmax and sums are fp32; with bf16 queries and a bf16 output the softmax weights times
+ * V's scale enter the product with 16 bits, else with 24.  head_dim up to 256, any group
+ * Hq / Hkv, any page size; head_dim 64 and 128 over pages of whole 16 tokens run on the
+ * matrix cores.  The same call gives the same bits (no atomics). */
+typedef struct {
+    const void* q; int32_t q_dtype; int64_t q_stride;
+    void* out; int32_t out_dtype; int64_t out_stride;                       /* SFG_F32 or SFG_BF16 */
+    const void* k_pool; const void* v_pool; int32_t pool_dtype;             /* SFG_I8 or SFG_FP8 */
+    const float* scales;         /* [num_pages][Hkv][2] */
+    const int32_t* page_table;   /* [B][pages_per_seq] */
+    const int32_t* seq_lens;     /* [B] or NULL: max_context tokens each */
+    const int32_t* starts;       /* [B + 1] or NULL */
+    int64_t batch, tokens, max_rows, q_heads, kv_heads, head_dim;
+    int64_t page_tokens, pages_per_seq, num_pages, max_context;
+    int32_t kv_splits; float scale;
+} sfg_kv8_attn_args;
+size_t sfg_hip_attn_kv8_workspace_v1(const sfg_kv8_attn_args* args);
+int sfg_hip_attn_kv8_v1(const sfg_kv8_attn_args* args, void* workspace, size_t workspace_bytes,
+                        void* stream);
 
 /* MoE routing: Router -> Softmax -> TopK -> Histogram -> PrefixSum -> Dispatch
  * (route_topk, moe_compiler.cpp:412-455; dispatch_tokens, 496-528).

@@ -15,9 +15,11 @@ LIB_PATH = Path(__file__).resolve().parent / "lib" / "libsfg_hip.so"
 
 ABI_VERSION = 1
 
-F32, BF16, I8, I32 = 0, 1, 2, 3
+F32, BF16, I8, I32, FP8 = 0, 1, 2, 3, 4
 EPI_NONE, EPI_RESIDUAL, EPI_SWIGLU, EPI_GLU_SILU_UP = 0, 1, 2, 3
 LAYOUT_NK, LAYOUT_TILED = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_BANDS, ROPE_RAMP = range(5)   # sfg_rope_scaling_kind
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 # sfg_gemm_tile
 TILE_AUTO, TILE_256x256_PP, TILE_256x256_W8, TILE_256x256_W4, TILE_256x128, TILE_128x256, \
     TILE_128x128, TILE_256x256_V, TILE_COUNT = range(9)
@@ -30,8 +32,8 @@ TAP_ATTN, TAP_RESIDUAL1, TAP_NORM2, TAP_ROUTE_INPUT, TAP_ROUTE_IDS, TAP_ROUTE_WE
 ERR_INVALID_CONFIG, ERR_SHAPE, ERR_GUARD, ERR_UNSUPPORTED, ERR_ABI = 1, 2, 3, 4, 5
 ERR_DEVICE, ERR_WORKSPACE = 16, 17
 
-c_i32, c_i64, c_f32, c_vp, c_sz = (ctypes.c_int32, ctypes.c_int64, ctypes.c_float,
-                                    ctypes.c_void_p, ctypes.c_size_t)
+c_i32, c_i64, c_f32, c_f64, c_vp, c_sz = (ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_double,
+                                           ctypes.c_void_p, ctypes.c_size_t)
 
 
 class SfgError(RuntimeError):
@@ -75,6 +77,49 @@ class PagedAttnArgs(ctypes.Structure):
         ("out", c_vp), ("out_dtype", c_i32),
         ("batch", c_i64), ("q_heads", c_i64), ("kv_heads", c_i64), ("rows", c_i64), ("head_dim", c_i64),
         ("page_tokens", c_i64), ("pages_per_seq", c_i64), ("num_pages", c_i64),
+        ("max_context", c_i64), ("kv_splits", c_i32), ("scale", c_f32),
+    ]
+
+
+class KvPlanArgs(ctypes.Structure):
+    _fields_ = [
+        ("keep", c_vp), ("counts", c_vp), ("seq_lens", c_vp), ("page_table", c_vp),
+        ("free_pages", c_vp), ("free_count", c_vp), ("starts", c_vp), ("positions", c_vp), ("slots", c_vp),
+        ("batch", c_i64), ("pages_per_seq", c_i64), ("num_pages", c_i64), ("page_tokens", c_i64),
+        ("max_tokens", c_i64),
+    ]
+
+
+class RopeScaling(ctypes.Structure):
+    _fields_ = [("kind", c_i32), ("theta", c_f64), ("factor", c_f64), ("context", c_f64), ("low", c_f64),
+                ("high", c_f64)]
+
+
+class RopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_vp), ("k", c_vp), ("q_out", c_vp), ("k_out", c_vp), ("dtype", c_i32),
+        ("q_stride", c_i64), ("k_stride", c_i64), ("q_out_stride", c_i64), ("k_out_stride", c_i64),
+        ("positions", c_vp), ("turns", c_vp), ("magnitude", c_f32), ("layout", c_i32),
+        ("tokens", c_i64), ("q_heads", c_i64), ("kv_heads", c_i64), ("head_dim", c_i64), ("rotary_dim", c_i64),
+    ]
+
+
+class Kv8AppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("keys", c_vp), ("values", c_vp), ("dtype", c_i32), ("key_stride", c_i64), ("value_stride", c_i64),
+        ("k_pool", c_vp), ("v_pool", c_vp), ("pool_dtype", c_i32), ("scales", c_vp), ("slots", c_vp),
+        ("tokens", c_i64), ("kv_heads", c_i64), ("head_dim", c_i64), ("page_tokens", c_i64), ("num_pages", c_i64),
+    ]
+
+
+class Kv8AttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_vp), ("q_dtype", c_i32), ("q_stride", c_i64),
+        ("out", c_vp), ("out_dtype", c_i32), ("out_stride", c_i64),
+        ("k_pool", c_vp), ("v_pool", c_vp), ("pool_dtype", c_i32), ("scales", c_vp),
+        ("page_table", c_vp), ("seq_lens", c_vp), ("starts", c_vp),
+        ("batch", c_i64), ("tokens", c_i64), ("max_rows", c_i64), ("q_heads", c_i64), ("kv_heads", c_i64),
+        ("head_dim", c_i64), ("page_tokens", c_i64), ("pages_per_seq", c_i64), ("num_pages", c_i64),
         ("max_context", c_i64), ("kv_splits", c_i32), ("scale", c_f32),
     ]
 
@@ -182,6 +227,13 @@ _SIGNATURES = {
     "sfg_hip_kv_select_v1": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64, c_vp]),
     "sfg_hip_kv_compact_v1": (c_i32, [c_vp, c_vp, ctypes.c_int, c_vp, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64,
                                       c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp]),
+    "sfg_hip_kv_plan_v1": (c_i32, [ctypes.POINTER(KvPlanArgs), c_vp]),
+    "sfg_hip_rope_inv_freq_host_v1": (c_i32, [c_vp, c_vp, c_i64, ctypes.POINTER(RopeScaling)]),
+    "sfg_hip_rope_turns_host_v1": (c_i32, [c_vp, c_vp, c_i64]),
+    "sfg_hip_rope_v1": (c_i32, [ctypes.POINTER(RopeArgs), c_vp]),
+    "sfg_hip_kv8_append_v1": (c_i32, [ctypes.POINTER(Kv8AppendArgs), c_vp]),
+    "sfg_hip_attn_kv8_workspace_v1": (c_sz, [ctypes.POINTER(Kv8AttnArgs)]),
+    "sfg_hip_attn_kv8_v1": (c_i32, [ctypes.POINTER(Kv8AttnArgs), c_vp, c_sz, c_vp]),
     "sfg_hip_moe_route_workspace_v1": (c_sz, [c_i64, c_i64, c_i64]),
     "sfg_hip_moe_route_v1": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp,
                                      c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),

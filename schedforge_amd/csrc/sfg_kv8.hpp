@@ -1,0 +1,51 @@
+// sfg_kv8.hpp -- what the kernels of a step over an 8-bit paged cache share: codes and
+// values, and the launchers that sfg_api_kv8.hip calls with checked arguments.
+#pragma once
+
+#include "../../include/sfg_hip.h"
+#include "sfg_paged.hpp"
+
+namespace sfg {
+
+constexpr float kMostI8 = 127.0f, kMostFp8 = 448.0f;  // the largest codes
+
+// The value of byte b: int8, or e4m3 (hardware conversion, exact).
+template <bool FP8>
+__device__ __forceinline__ float kv8_value(uint8_t b) {
+    if constexpr (FP8) return __builtin_amdgcn_cvt_f32_fp8(b, 0);
+    else return static_cast<float>(static_cast<int8_t>(b));
+}
+
+// The code of v under `scale`: the IEEE quotient in fp32, rounded to the nearest code, ties
+// to even (v_rndne_f32; v_cvt_pk_fp8_f32), cut to the largest one; 0 unless scale > 0.
+template <bool FP8>
+__device__ __forceinline__ uint8_t kv8_code(float v, float scale) {
+    if (!(scale > 0.0f)) return 0;
+    constexpr float most = FP8 ? kMostFp8 : kMostI8;
+    const float y = fminf(fmaxf(__fdiv_rn(v, scale), -most), most);
+    if constexpr (FP8) return static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false));
+    else return static_cast<uint8_t>(static_cast<int>(rintf(y)));
+}
+
+// The scale that holds values up to the one whose magnitude has these bits; NaN for an
+// infinity or a NaN.
+template <bool FP8>
+__device__ __forceinline__ float kv8_scale(uint32_t top) {
+    if (top >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
+    return __fdiv_rn(__uint_as_float(top), FP8 ? kMostFp8 : kMostI8);
+}
+
+// The larger of two scales, NaN if one is.
+__device__ __forceinline__ float kv8_larger(float a, float b) { return a >= b || a != a ? a : b; }
+
+void launch_kv_plan(const sfg_kv_plan_args& a, hipStream_t stream);
+void launch_rope(const sfg_rope_args& a, hipStream_t stream);
+void launch_kv8_append(const sfg_kv8_append_args& a, hipStream_t stream);
+struct Kv8Plan {
+    int splits;
+    size_t bytes;
+};
+Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a);
+void launch_attn_kv8(const sfg_kv8_attn_args& a, const Kv8Plan& plan, void* workspace, hipStream_t stream);
+
+}  // namespace sfg

@@ -18,9 +18,9 @@ struct Kv8Args {
     int batch, tokens, max_rows, q_heads, kv_heads, dim, pt, per, pages, max_context;
     float scale;
     // the matrix-core kernels'
-    int group, slots, share, fixed, least, direct, width;  // (as in Kv8Plan)
+    int group, slots, share, fixed, least, few, width;  // (as in Kv8Plan)
     int vec, out_vec;                                      // rows begin on 16-byte boundaries
-    int2* slot_of; int* sequence_of; float2* part_ml; float* part_acc;
+    int4* slot_of; int* sequence_of; float2* part_ml; float* part_acc;
     // Rows [t0, t0 + rows) of a sequence and its tokens.
     __device__ __forceinline__ void sequence(int b, int& t0, int& rows, int& len) const {
         t0 = b * max_rows;
@@ -167,70 +167,85 @@ __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; 
 __device__ __forceinline__ int ways_of(int cols, int width) { return cols > 2 * width ? 1 : cols > width ? 2 : 4; }
 __device__ __forceinline__ int blocks_of(int cols, int width) { return cols > 4 * width ? ceil_div(cols, 4 * width) : cols > 0; }
 
-// A slot of the grid: block `block` of a sequence's columns, split `split` of its tiles, of which
-// each split has `each`.  Its slots begin at `first`, splits of a block side by side.
-struct Slot {
-    int b, block, split, splits, each, first;
+// A unit of work: a block of a sequence's columns over all its tiles.
+struct Unit {
+    int b, block, blocks, tiles, t0, rows, len;
+    int ord;      // units before it
+    int before;   // tiles of the sequences before (where tiles are dealt), else their splits
+};
+template <int WIDTH>
+__device__ __forceinline__ void load_unit(const Kv8Args& a, int b, Unit& u) {
+    u.tiles = u.blocks = u.t0 = u.rows = u.len = 0;
+    if (b >= a.batch) return;
+    a.sequence(b, u.t0, u.rows, u.len);
+    u.blocks = blocks_of(min(u.rows, a.max_rows) * a.group, WIDTH);
+    u.tiles = max(ceil_div(u.len, kTile), 1);
+}
+
+// How the units' tiles are given to workgroups, which each one works out from the lengths.
+// Dealt (each 0): in units' order, the same number to each of `groups`, across units: with a
+// round of workgroups as long as the work, none waits for another's longer share.  Split: a unit
+// into pieces of `each` tiles, a workgroup a piece, where there are few: a second unit would
+// double a workgroup's time.  64 sequences of up to 8192 tokens: dealt 109 us, split into 1280
+// pieces 117; four of up to 2001 with 5 fp32 rows: 20 and 14.
+struct Shares {
+    int all, groups, each, fixed;
+    __device__ Shares(const Kv8Args& a, int n) : all(n), groups(a.share), each(0), fixed(a.fixed) {
+        if (fixed || n <= a.share * a.few) each = max(ceil_div(n, max(a.share, 1)), a.least);
+    }
+    __device__ int pieces(int tiles) const { return ceil_div(tiles, fixed ? ceil_div(tiles, fixed) : each); }
+    __device__ int begin(int w) const { return static_cast<int>(static_cast<int64_t>(all) * w / groups); }
+    __device__ int of(int tile) const { return static_cast<int>((static_cast<int64_t>(tile + 1) * groups - 1) / all); }
 };
 
-// Sequences are split so that every workgroup has about the same number of tiles: all blocks'
-// tiles over `share`; share and the blocks together bound the slots.  Each wave works it out for
-// itself from the lengths.
+// The unit that tile `at` of all of them belongs to (where units are split: piece `at`), and its
+// place there.  first: the lane's sequence of the first 64.
 template <int WIDTH>
-__device__ bool find_slot(const Kv8Args& a, int slot, Slot& s) {
-    if (a.direct) {  // a slot a sequence
-        int t0, rows, len;
-        a.sequence(slot, t0, rows, len);
-        s = {slot, 0, 0, 1, 0x3FFFFFFF, slot};
-        return rows > 0;
-    }
-    const int lane = threadIdx.x & 63;
-    int tiles = 0, blocks = 0;
-    auto load = [&](int b) {  // a sequence's tiles (at least one) and blocks, none without rows
-        tiles = blocks = 0;
-        if (b < a.batch) {
-            int t0, rows, len;
-            a.sequence(b, t0, rows, len);
-            blocks = blocks_of(min(rows, a.max_rows) * a.group, WIDTH);
-            tiles = max(ceil_div(len, kTile), 1);
-        }
-    };
-    int each = 0x3FFFFFFF;
-    load(lane);
-    if (a.share) {
-        int64_t all = 0;
-        for (int base = 0;;) {
-            // (64 sequences' tiles times blocks may pass 32 bits)
-            int64_t n = static_cast<int64_t>(tiles) * blocks;
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, kWave);
-            all += n;
-            if ((base += kWave) >= a.batch) break;
-            load(base + lane);
-        }
-        each = static_cast<int>(max((all + a.share - 1) / a.share, static_cast<int64_t>(a.least)));
-        if (a.batch > kWave) load(lane);
-    }
-    int before = 0;
+__device__ __forceinline__ bool find_unit(const Kv8Args& a, const Shares& how, const Unit& first, int at, Unit& u, int& place) {
+    int sum = 0, ord = 0;
+    Unit v = first;
     for (int base = 0;;) {
-        const int mine_each = a.fixed ? ceil_div(tiles, a.fixed) : each;
-        const int splits = blocks > 0 ? ceil_div(tiles, mine_each) : 0;
-        const int upto = wave_inclusive(splits * blocks) + before;
-        const uint64_t behind = __ballot(upto > slot);
+        const int mine = v.blocks == 0 ? 0 : (how.each ? how.pieces(v.tiles) : v.tiles) * v.blocks;
+        const int upto = wave_inclusive(mine) + sum, units = wave_inclusive(v.blocks) + ord;
+        const uint64_t behind = __ballot(upto > at);
         if (behind) {
             const int l = __builtin_ctzll(behind);
-            s.b = base + l;
-            s.splits = __builtin_amdgcn_readlane(splits, l);
-            s.each = __builtin_amdgcn_readlane(mine_each, l);
-            s.first = __builtin_amdgcn_readlane(upto - splits * blocks, l);
-            s.block = (slot - s.first) / s.splits;
-            s.split = slot - s.first - s.block * s.splits;
+            u.b = base + l;
+            u.blocks = __builtin_amdgcn_readlane(v.blocks, l);
+            u.tiles = __builtin_amdgcn_readlane(v.tiles, l);
+            u.t0 = __builtin_amdgcn_readlane(v.t0, l);
+            u.rows = __builtin_amdgcn_readlane(v.rows, l);
+            u.len = __builtin_amdgcn_readlane(v.len, l);
+            u.before = __builtin_amdgcn_readlane(upto - mine, l);
+            const int of_block = how.each ? how.pieces(u.tiles) : u.tiles;
+            u.block = (at - u.before) / of_block;
+            place = at - u.before - u.block * of_block;
+            u.ord = __builtin_amdgcn_readlane(units - v.blocks, l) + u.block;
             return true;
         }
-        before = __builtin_amdgcn_readlane(upto, 63);
+        sum = __builtin_amdgcn_readlane(upto, 63);
+        ord = __builtin_amdgcn_readlane(units, 63);
         if ((base += kWave) >= a.batch) return false;
-        load(base + lane);
+        load_unit<WIDTH>(a, base + (threadIdx.x & 63), v);
     }
+}
+
+// (the same in all lanes: kept in scalar registers)
+__device__ __forceinline__ void same(int& x) { x = __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ void same(Unit& u) {
+    same(u.b); same(u.block); same(u.blocks); same(u.tiles); same(u.t0); same(u.rows); same(u.len); same(u.ord); same(u.before);
+}
+
+// The unit behind u, if there is one.
+template <int WIDTH>
+__device__ __forceinline__ void next_unit(const Kv8Args& a, Unit& u) {
+    ++u.ord;
+    if (++u.block < u.blocks) return;
+    u.before += u.tiles * u.blocks;
+    u.block = 0;
+    do {
+        load_unit<WIDTH>(a, ++u.b, u);
+    } while (u.blocks == 0 && u.b < a.batch);
 }
 
 // 8 codes as an MFMA operand.
@@ -249,6 +264,15 @@ __device__ __forceinline__ bf16x8 kv8_operand(uint32_t lo, uint32_t hi) {
     }
 }
 
+// 16 bytes of codes; ONCE: read by this workgroup alone, so not kept in the caches (64
+// sequences of up to 8192 tokens: 112 us -> 109, two of 131072: 76 -> 72).
+typedef uint32_t uint32x4 __attribute__((ext_vector_type(4)));
+template <bool ONCE>
+__device__ __forceinline__ uint4 kv8_fetch(const uint8_t* p) {
+    if constexpr (ONCE) return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const uint32x4*>(p)));
+    else return *reinterpret_cast<const uint4*>(p);
+}
+
 // Two weights as PT bf16 terms, packed (each truncated, the last of two rounded).
 template <int PT>
 __device__ __forceinline__ void weight_terms(float p0, float p1, uint32_t* t) {
@@ -265,283 +289,354 @@ __device__ __forceinline__ void weight_terms(float p0, float p1, uint32_t* t) {
 
 }  // namespace
 
-template <bool FP8, int D, int QT, int PT, int NT>
-__global__ __launch_bounds__(256) void attn_kv8_kernel(Kv8Args a) {
+template <bool FP8, int D, int QT, int PT, int NT, bool P16>
+__global__ __launch_bounds__(256, QT == 3 ? (D == 64 ? 3 : 2) : NT == 2 ? 2 : D == 64 ? 4 : 3) void attn_kv8_kernel(Kv8Args a) {
     static_assert(D == 64 || D == 128, "16 bytes of 4 lanes make a k-step");
     constexpr int kF = D / 32, kDt = D / 16, kLd = D + 4, kCols = 16 * NT;
-    __shared__ float so[4][kCols][kLd];
+    // a wave's queries as operands, which the loop reads again for each tile; then its sums
+    union Wave {
+        uint4 q[NT][kF][QT][kWave];
+        float o[kCols][kLd];
+    };
+    __shared__ Wave sw[4];
     __shared__ float sm[4][kCols], sl[4][kCols];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lg = lane >> 4;
-    const int slot = blockIdx.x / a.kv_heads, kvh = blockIdx.x - slot * a.kv_heads;
-    Slot at;
-    int t0, rows, len;
-    if (!find_slot<kCols>(a, slot, at)) return;
-    a.sequence(at.b, t0, rows, len);
-    const int cols = min(rows, a.max_rows) * a.group;
-    const int ways = ways_of(cols, kCols), groups = 4 / ways, col0 = at.block * groups * kCols;
-    const int wcol = col0 + wave % groups * kCols;  // (may lie behind the columns)
-    // tokens that all of the wave's columns see, and that any does
-    const int seen_all = max(len - rows + wcol / a.group + 1, 0);
-    const int seen_any = wcol < cols ? max(len - rows + min(wcol + kCols - 1, cols - 1) / a.group + 1, 0) : 0;
-    const int64_t from = static_cast<int64_t>(at.split) * at.each;
-    const int tile0 = static_cast<int>(min(from, static_cast<int64_t>(0x3FFFFFFF)));
-    const int span = max(static_cast<int>(min(from + at.each, static_cast<int64_t>(ceil_div(seen_any, kTile)))) - tile0, 0);
-    const int way = wave / groups;
-    const int begin = tile0 + static_cast<int>(static_cast<int64_t>(span) * way / ways), end = tile0 + static_cast<int>(static_cast<int64_t>(span) * (way + 1) / ways);
+    const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = blockIdx.x / a.kv_heads, kvh = blockIdx.x - group * a.kv_heads;
+    const float scale = a.scale * kLog2e;
+    const int pt = P16 ? 16 : a.pt, runs = pt >> 4;  // 16-token runs of a page
 
-    // Q^T: lane (q, g) holds dims 64 (f / 2) + 16 g + 8 (f % 2) + [0, 8) of column q
-    bf16x8 qf[NT][kF][QT];
-    int seen[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int c = wcol + 16 * n + lr, i = c / a.group;
-        const bool live = c < cols;
-        seen[n] = live ? max(len - rows + i + 1, 0) : 0;
-        const int64_t row = static_cast<int64_t>(t0 + (live ? i : 0)) * a.q_stride + static_cast<int64_t>(kvh * a.group + (live ? c - i * a.group : 0)) * D + 16 * lg;
-#pragma unroll
-        for (int f = 0; f < kF; ++f) {
-            const int64_t o = row + 64 * (f >> 1) + 8 * (f & 1);
-            if constexpr (QT == 1) {
-                const uint16_t* p = static_cast<const uint16_t*>(a.q) + o;
-                uint4 w;
-                if (a.vec) w = *reinterpret_cast<const uint4*>(p);
-                else w = make_uint4(p[0] | p[1] << 16, p[2] | p[3] << 16, p[4] | p[5] << 16, p[6] | p[7] << 16);
-                qf[n][f][0] = as_bf16x8(live ? w : make_uint4(0, 0, 0, 0));
-            } else {
-                uint16_t t[3][8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float v = live ? kv8_load(a.q, a.q_f32, o + e) : 0.f;
-                    split3(v, t[0][e], t[1][e], t[2][e]);
-                }
-#pragma unroll
-                for (int s = 0; s < QT; ++s) qf[n][f][s] = __builtin_bit_cast(bf16x8, t[s]);
-            }
+    // what this workgroup walks: a piece of a unit, or tiles of one unit after the other
+    Unit first, u;
+    load_unit<kCols>(a, lane, first);
+    int all = 0;
+    if (!a.fixed) {
+        all = __builtin_amdgcn_readlane(wave_inclusive(first.tiles * first.blocks), 63);
+        for (int base = kWave; base < a.batch; base += kWave) {
+            load_unit<kCols>(a, base + lane, u);
+            all += __builtin_amdgcn_readlane(wave_inclusive(u.tiles * u.blocks), 63);
         }
     }
-    const float scale = a.scale * kLog2e;
-    const int runs = a.pt >> 4;  // 16-token runs of a page
-    const int32_t* table = a.page_table + static_cast<int64_t>(at.b) * a.per;
-    // run s of the sequence (at most the last tile's): its page, and where it lies there
-    auto page_of = [&](int s, int& sub) {
-        const int page = runs == 1 ? s : s / runs;
-        sub = runs == 1 ? 0 : s - page * runs;
-        return table[min(page, a.per - 1)];
-    };
-    uint4 kr[4][D / 64], vr[kDt];
-    float2 sc;
-    bool vok;
-    auto load_k = [&](int page, int sub) {
-        const bool ok = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages);
-        const int64_t u = (static_cast<int64_t>(ok ? page : 0) * a.kv_heads + kvh) * (a.pt * D) + (sub * 16 + (lr & 3)) * D + 16 * lg;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < D / 64; ++j) kr[i][j] = *reinterpret_cast<const uint4*>(a.k_pool + u + i * 4 * D + j * 64);
-    };
-    auto load_v = [&](int page, int sub) {
-        vok = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages);
-        const int64_t u = static_cast<int64_t>(vok ? page : 0) * a.kv_heads + kvh;
-        sc = reinterpret_cast<const float2*>(a.scales)[u];
-        const uint8_t* p = a.v_pool + u * (a.pt * D) + static_cast<int64_t>(lr) * a.pt + sub * 16;
-#pragma unroll
-        for (int i = 0; i < kDt; ++i) vr[i] = *reinterpret_cast<const uint4*>(p + static_cast<int64_t>(i) * 16 * a.pt);
-    };
-    floatx4 o[NT][kDt] = {};
-    float m[NT], l[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        m[n] = -INFINITY;
-        l[n] = 0.f;
+    Shares how(a, all);
+    same(how.each);
+    int tile0, left;
+    if (how.each) {
+        if (!find_unit<kCols>(a, how, first, group, u, tile0)) return;
+        const int each = how.fixed ? ceil_div(u.tiles, how.fixed) : how.each;
+        tile0 *= each;
+        left = min(each, u.tiles - tile0);
+    } else {
+        if (group >= how.groups) return;
+        const int from = how.begin(group);
+        left = how.begin(group + 1) - from;
+        if (!find_unit<kCols>(a, how, first, from, u, tile0)) return;
     }
-    if (begin < end) {
-        int sub_k, sub_v;
-        int page_k = page_of(4 * begin + (lr >> 2), sub_k), page_v = page_of(4 * begin + lg, sub_v);
-        load_k(page_k, sub_k);
-        load_v(page_v, sub_v);
-        // the pages of the tile behind the one in flight
-        int next = min(begin + 1, end - 1);
-        page_k = page_of(4 * next + (lr >> 2), sub_k);
-        page_v = page_of(4 * next + lg, sub_v);
-        for (int t = begin; t < end; ++t) {
-            floatx4 s[NT][4] = {};
+    for (;;) {
+        same(u);
+        same(tile0);
+        same(left);
+        const int count = min(left, u.tiles - tile0);
+        const int cols = min(u.rows, a.max_rows) * a.group;
+        const int ways = ways_of(cols, kCols), groups = 4 / ways, col0 = u.block * groups * kCols;
+        const int wcol = col0 + wave % groups * kCols;  // (may lie behind the columns)
+        // tokens that all of the wave's columns see, and that any does
+        const int seen_all = max(u.len - u.rows + wcol / a.group + 1, 0);
+        const int seen_any = wcol < cols ? max(u.len - u.rows + min(wcol + kCols - 1, cols - 1) / a.group + 1, 0) : 0;
+        const int span = max(min(tile0 + count, ceil_div(seen_any, kTile)) - tile0, 0), way = wave / groups;
+        const int begin = tile0 + static_cast<int>(static_cast<int64_t>(span) * way / ways);
+        const int end = tile0 + static_cast<int>(static_cast<int64_t>(span) * (way + 1) / ways);
+        const int32_t* table = a.page_table + static_cast<int64_t>(u.b) * a.per;
+        // run s of the sequence (at most the last tile's): its page, and where it lies there
+        auto page_of = [&](int s, int& sub) {
+            const int page = P16 ? s : s / runs;
+            sub = P16 ? 0 : s - page * runs;
+            return table[min(page, a.per - 1)];
+        };
+        int sub_k, sub_v, page_k = -1, page_v = -1;
+        if (begin < end) {
+            page_k = page_of(4 * begin + (lr >> 2), sub_k);
+            page_v = page_of(4 * begin + lg, sub_v);
+        }
+        // Q^T: lane (q, g) holds dims 64 (f / 2) + 16 g + 8 (f % 2) + [0, 8) of column q
+        int seen[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int c = wcol + 16 * n + lr, i = c / a.group;
+            const bool live = c < cols;
+            seen[n] = live ? max(u.len - u.rows + i + 1, 0) : 0;
+            const int64_t row = static_cast<int64_t>(u.t0 + (live ? i : 0)) * a.q_stride + static_cast<int64_t>(kvh * a.group + (live ? c - i * a.group : 0)) * D + 16 * lg;
+#pragma unroll
+            for (int f = 0; f < kF; ++f) {
+                const int64_t at = row + 64 * (f >> 1) + 8 * (f & 1);
+                if constexpr (QT == 1) {
+                    const uint16_t* p = static_cast<const uint16_t*>(a.q) + at;
+                    uint4 w;
+                    if (a.vec) w = *reinterpret_cast<const uint4*>(p);
+                    else w = make_uint4(p[0] | p[1] << 16, p[2] | p[3] << 16, p[4] | p[5] << 16, p[6] | p[7] << 16);
+                    sw[wave].q[n][f][0][lane] = live ? w : make_uint4(0, 0, 0, 0);
+                } else {
+                    uint16_t t[3][8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float v = live ? kv8_load(a.q, a.q_f32, at + e) : 0.f;
+                        split3(v, t[0][e], t[1][e], t[2][e]);
+                    }
+#pragma unroll
+                    for (int s = 0; s < QT; ++s) sw[wave].q[n][f][s][lane] = __builtin_bit_cast(uint4, t[s]);
+                }
+            }
+        }
+        uint4 kr[4][D / 64], vr[kDt];
+        float2 sc;
+        bool vok;
+        auto load_k = [&](int page, int sub) {
+            const bool ok = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages);
+            const int64_t at = (static_cast<int64_t>(ok ? page : 0) * a.kv_heads + kvh) * (pt * D) + (sub * 16 + (lr & 3)) * D + 16 * lg;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
+                for (int j = 0; j < D / 64; ++j) kr[i][j] = kv8_fetch<QT == 1 && NT == 1>(a.k_pool + at + i * 4 * D + j * 64);
+        };
+        auto load_v = [&](int page, int sub) {
+            vok = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages);
+            const int64_t at = static_cast<int64_t>(vok ? page : 0) * a.kv_heads + kvh;
+            sc = reinterpret_cast<const float2*>(a.scales)[at];
+            const uint8_t* p = a.v_pool + at * (pt * D) + static_cast<int64_t>(lr) * pt + sub * 16;
+#pragma unroll
+            for (int i = 0; i < kDt; ++i) vr[i] = kv8_fetch<QT == 1 && NT == 1>(p + static_cast<int64_t>(i) * 16 * pt);
+        };
+        floatx4 o[NT][kDt] = {};
+        float m[NT], l[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            m[n] = -INFINITY;
+            l[n] = 0.f;
+        }
+        if (begin < end) {
+            load_k(page_k, sub_k);
+            load_v(page_v, sub_v);
+            // the pages of the tile behind the one in flight
+            int next = min(begin + 1, end - 1);
+            page_k = page_of(4 * next + (lr >> 2), sub_k);
+            page_v = page_of(4 * next + lg, sub_v);
+            for (int t = begin; t < end; ++t) {
+                asm volatile("" ::: "memory");  // (the queries stay in LDS: in registers they cost a wave a SIMD)
+                floatx4 s[NT][4] = {};
+#pragma unroll
                 for (int f = 0; f < kF; ++f) {
-                    const uint4& w = kr[i][f >> 1];
-                    const bf16x8 k = f & 1 ? kv8_operand<FP8>(w.z, w.w) : kv8_operand<FP8>(w.x, w.y);
+                    bf16x8 q[NT][QT];
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int e = QT - 1; e >= 0; --e) s[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qf[n][f][e], s[n][i], 0, 0, 0);
-                }
-            if (t + 1 < end) load_k(page_k, sub_k);
-            const int base = t * kTile + lg * 16;  // the lane's run
-            const float fk = sc.x * scale, fv = sc.y;
-            const bool part = t * kTile + kTile > seen_all || __any(!vok);
-            uint32_t pw[NT][PT][8];
+                        for (int e = 0; e < QT; ++e) q[n][e] = as_bf16x8(sw[wave].q[n][f][e][lane]);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const int live = vok ? min(max(seen[n] - base, 0), 16) : 0;  // tokens of the run that the column sees
-                float top = -INFINITY;
+                    for (int i = 0; i < 4; ++i) {
+                        const uint4& w = kr[i][f >> 1];
+                        const bf16x8 k = f & 1 ? kv8_operand<FP8>(w.z, w.w) : kv8_operand<FP8>(w.x, w.y);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                        for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        s[n][i][r] *= fk;
-                        if (part && 4 * i + r >= live) s[n][i][r] = -INFINITY;
-                        top = fmaxf(top, s[n][i][r]);
+                            for (int e = QT - 1; e >= 0; --e) s[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[n][e], s[n][i], 0, 0, 0);
                     }
-                top = xor32_max(xor16_max(top));
-                // the running maximum moves only when a score is 2^8 above it
-                if (__any(top > m[n] + 8.0f)) {
-                    const float to = fmaxf(m[n], top);
-                    const float alpha = to == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - to);
-                    m[n] = to;
-                    l[n] *= alpha;
-#pragma unroll
-                    for (int d = 0; d < kDt; ++d)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) o[n][d][r] *= alpha;
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                const float ref = m[n] == -INFINITY ? 0.0f : m[n];
-                float w[16];
-                float sum = 0.f;
+                if (t + 1 < end) load_k(page_k, sub_k);
+                const int base = t * kTile + lg * 16;  // the lane's run
+                const float fk = sc.x * scale, fv = sc.y;
+                const bool part = t * kTile + kTile > seen_all || __any(!vok);
+                uint32_t pw[NT][PT][8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int n = 0; n < NT; ++n) {
+                    const int live = vok ? min(max(seen[n] - base, 0), 16) : 0;  // tokens of the run that the column sees
+                    float top = -INFINITY;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float p = __builtin_amdgcn_exp2f(s[n][i][r] - ref);
-                        sum += p;
-                        w[4 * i + r] = part && 4 * i + r >= live ? 0.0f : p * fv;
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            s[n][i][r] *= fk;
+                            if (part && 4 * i + r >= live) s[n][i][r] = -INFINITY;
+                            top = fmaxf(top, s[n][i][r]);
+                        }
+                    top = xor32_max(xor16_max(top));
+                    // the running maximum moves only when a score is 2^8 above it
+                    if (__any(top > m[n] + 8.0f)) {
+                        const float to = fmaxf(m[n], top);
+                        const float alpha = to == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - to);
+                        m[n] = to;
+                        l[n] *= alpha;
+#pragma unroll
+                        for (int d = 0; d < kDt; ++d)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) o[n][d][r] *= alpha;
                     }
-                l[n] += sum;
+                    const float ref = m[n] == -INFINITY ? 0.0f : m[n];
+                    float w[16];
+                    float sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    uint32_t e[PT];
-                    weight_terms<PT>(w[2 * i], w[2 * i + 1], e);
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int x = 0; x < PT; ++x) pw[n][x][i] = e[x];
+                        for (int r = 0; r < 4; ++r) {
+                            const float p = __builtin_amdgcn_exp2f(s[n][i][r] - ref);
+                            sum += p;
+                            w[4 * i + r] = part && 4 * i + r >= live ? 0.0f : p * fv;
+                        }
+                    l[n] += sum;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        uint32_t e[PT];
+                        weight_terms<PT>(w[2 * i], w[2 * i + 1], e);
+#pragma unroll
+                        for (int x = 0; x < PT; ++x) pw[n][x][i] = e[x];
+                    }
+                }
+                if (FP8 && part) {  // codes that no row sees may be NaN: 0 * NaN
+                    const int held = vok ? min(max(u.len - base, 0), 16) : 0;
+#pragma unroll
+                    for (int i = 0; i < kDt; ++i) {
+                        uint32_t* w = &vr[i].x;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int k = min(max(held - 4 * j, 0), 4);
+                            w[j] = k == 4 ? w[j] : w[j] & ((1u << (8 * k)) - 1u);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int d = 0; d < kDt; ++d) {
+                    if (d % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+                    const bf16x8 v0 = kv8_operand<FP8>(vr[d].x, vr[d].y), v1 = kv8_operand<FP8>(vr[d].z, vr[d].w);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int x = PT - 1; x >= 0; --x) {
+                            const uint32_t* p = pw[n][x];
+                            o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, as_bf16x8(make_uint4(p[0], p[1], p[2], p[3])), o[n][d], 0, 0, 0);
+                            o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, as_bf16x8(make_uint4(p[4], p[5], p[6], p[7])), o[n][d], 0, 0, 0);
+                        }
+                }
+                if (t + 1 < end) {
+                    load_v(page_v, sub_v);
+                    next = min(t + 2, end - 1);
+                    page_k = page_of(4 * next + (lr >> 2), sub_k);
+                    page_v = page_of(4 * next + lg, sub_v);
                 }
             }
-            if (FP8 && part) {  // codes that no row sees may be NaN: 0 * NaN
-                const int held = vok ? min(max(len - base, 0), 16) : 0;
+        }
+        // the waves of a column group, joined in LDS
 #pragma unroll
-                for (int i = 0; i < kDt; ++i) {
-                    uint32_t* w = &vr[i].x;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int k = min(max(held - 4 * j, 0), 4);
-                        w[j] = k == 4 ? w[j] : w[j] & ((1u << (8 * k)) - 1u);
-                    }
-                }
+        for (int n = 0; n < NT; ++n) {
+            l[n] = xor32_sum(xor16_sum(l[n]));
+            if (lg == 0) {
+                sm[wave][16 * n + lr] = m[n];
+                sl[wave][16 * n + lr] = l[n];
             }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float top = -INFINITY;
+            for (int w = wave % groups; w < 4; w += groups) top = fmaxf(top, sm[w][16 * n + lr]);
+            const float f = m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[n] - top);
 #pragma unroll
             for (int d = 0; d < kDt; ++d) {
-                const bf16x8 v0 = kv8_operand<FP8>(vr[d].x, vr[d].y), v1 = kv8_operand<FP8>(vr[d].z, vr[d].w);
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int x = PT - 1; x >= 0; --x) {
-                        const uint32_t* p = pw[n][x];
-                        o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, as_bf16x8(make_uint4(p[0], p[1], p[2], p[3])), o[n][d], 0, 0, 0);
-                        o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, as_bf16x8(make_uint4(p[4], p[5], p[6], p[7])), o[n][d], 0, 0, 0);
-                    }
-            }
-            if (t + 1 < end) {
-                load_v(page_v, sub_v);
-                next = min(t + 2, end - 1);
-                page_k = page_of(4 * next + (lr >> 2), sub_k);
-                page_v = page_of(4 * next + lg, sub_v);
+                const float4 v = make_float4(o[n][d][0] * f, o[n][d][1] * f, o[n][d][2] * f, o[n][d][3] * f);
+                *reinterpret_cast<float4*>(&sw[wave].o[16 * n + lr][16 * d + 4 * lg]) = v;
             }
         }
-    }
-    // the waves of a column group, joined in LDS
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        l[n] = xor32_sum(xor16_sum(l[n]));
-        if (lg == 0) {
-            sm[wave][16 * n + lr] = m[n];
-            sl[wave][16 * n + lr] = l[n];
+        __syncthreads();
+        const bool whole = count == u.tiles;
+        const int64_t part = (static_cast<int64_t>(how.each ? group : group + u.ord) * a.kv_heads + kvh) * a.width;
+        for (int e = threadIdx.x; e < groups * kCols * (D / 4); e += 256) {
+            const int c = e / (D / 4), d = e % (D / 4) * 4, gr = c / kCols, cc = c % kCols;
+            const int col = col0 + c;
+            if (col >= cols) break;
+            float top = -INFINITY, sum = 0.f;
+            for (int w = gr; w < 4; w += groups) top = fmaxf(top, sm[w][cc]);
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int w = gr; w < 4; w += groups) {
+                sum += sl[w][cc] * (sm[w][cc] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[w][cc] - top));
+                const float4 x = *reinterpret_cast<const float4*>(&sw[w].o[cc][d]);
+                v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+            }
+            const int i = col / a.group;
+            if (whole) {
+                kv8_store4(a, static_cast<int64_t>(u.t0 + i) * a.out_stride + static_cast<int64_t>(kvh * a.group + col - i * a.group) * D + d, v, sum);
+            } else {
+                *reinterpret_cast<float4*>(a.part_acc + (part + c) * D + d) = v;
+                if (d == 0) a.part_ml[part + c] = make_float2(top, sum);
+            }
         }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        float top = -INFINITY;
-        for (int w = wave % groups; w < 4; w += groups) top = fmaxf(top, sm[w][16 * n + lr]);
-        const float f = m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[n] - top);
-#pragma unroll
-        for (int d = 0; d < kDt; ++d) {
-            float4 v = make_float4(o[n][d][0] * f, o[n][d][1] * f, o[n][d][2] * f, o[n][d][3] * f);
-            *reinterpret_cast<float4*>(&so[wave][16 * n + lr][16 * d + 4 * lg]) = v;
+        // where the join finds a row's sequence, and the sequence's pieces or tiles among all
+        if (a.slot_of && tile0 == 0 && kvh == 0) {
+            if (u.block == 0 && threadIdx.x == 0) a.slot_of[u.b] = make_int4(u.before, how.each ? how.pieces(u.tiles) : u.ord, u.tiles, how.each ? 0 : all);
+            for (int e = threadIdx.x; e < groups * kCols; e += 256)
+                if (col0 + e < cols) a.sequence_of[u.t0 + (col0 + e) / a.group] = u.b;
         }
-    }
-    __syncthreads();
-    const int64_t part = static_cast<int64_t>(blockIdx.x) * a.width;
-    for (int e = threadIdx.x; e < groups * kCols * (D / 4); e += 256) {
-        const int c = e / (D / 4), d = e % (D / 4) * 4, gr = c / kCols, cc = c % kCols;
-        const int col = col0 + c;
-        if (col >= cols) break;
-        float top = -INFINITY, sum = 0.f;
-        for (int w = gr; w < 4; w += groups) top = fmaxf(top, sm[w][cc]);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int w = gr; w < 4; w += groups) {
-            sum += sl[w][cc] * (sm[w][cc] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[w][cc] - top));
-            const float4 x = *reinterpret_cast<const float4*>(&so[w][cc][d]);
-            v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-        }
-        const int i = col / a.group;
-        if (at.splits == 1) {
-            kv8_store4(a, static_cast<int64_t>(t0 + i) * a.out_stride + static_cast<int64_t>(kvh * a.group + col - i * a.group) * D + d, v, sum);
-        } else {
-            *reinterpret_cast<float4*>(a.part_acc + (part + c) * D + d) = v;
-            if (d == 0) a.part_ml[part + c] = make_float2(top, sum);
-        }
-    }
-    // where the join finds a row's sequence, and the sequence's slots
-    if (a.slot_of && at.split == 0 && kvh == 0) {
-        if (at.block == 0 && threadIdx.x == 0) a.slot_of[at.b] = make_int2(at.first, at.splits);
-        for (int e = threadIdx.x; e < groups * kCols; e += 256)
-            if (col0 + e < cols) a.sequence_of[t0 + (col0 + e) / a.group] = at.b;
+        if ((left -= count) <= 0) return;
+        next_unit<kCols>(a, u);
+        if (u.b >= a.batch) return;
+        tile0 = 0;
+        __syncthreads();  // (the sums have been read: the queries of the next unit go there)
     }
 }
 
-// The splits of a row and kv head: weights 2^(m_s - M), a sum in the splits' order.
+// The splits of a row and query head: weights 2^(m_s - M).  D / 4 lanes to a split, 8 or 16
+// splits at a time, then those sums in a fixed order.  (90 splits one after the other: 45 us.)
 template <int D, int WIDTH>
-__global__ __launch_bounds__(128) void attn_kv8_join_kernel(Kv8Args a) {
-    const int t = blockIdx.x, kvh = blockIdx.y;
+__global__ __launch_bounds__(256) void attn_kv8_join_kernel(Kv8Args a) {
+    constexpr int kLanes = D / 4, kWays = 256 / kLanes;  // lanes of a split, splits at a time
+    __shared__ float tops[4];
+    __shared__ float4 sv[kWays][kLanes];
+    __shared__ float ssum[kWays];
+    const int t = blockIdx.x, h = blockIdx.y, kvh = h / a.group;
     if (a.starts && t >= a.starts[a.batch]) return;
     const int b = min(max(a.sequence_of[t], 0), a.batch - 1);
+    const int4 at = a.slot_of[b];
     int t0, rows, len;
     a.sequence(b, t0, rows, len);
     const int i = t - t0;
     rows = min(rows, a.max_rows);
     if (i < 0 || i >= rows) return;  // (a row that no sequence computes)
-    const int2 at = a.slot_of[b];
-    const int cols = rows * a.group, wide = 4 / ways_of(cols, WIDTH) * WIDTH;
-    if (at.y <= 1) return;
-    for (int e = threadIdx.x; e < a.group * (D / 4); e += 128) {
-        const int g = e / (D / 4), d = e % (D / 4) * 4;
-        const int c = i * a.group + g, block = c / wide;
-        const int64_t slot = at.x + static_cast<int64_t>(block) * at.y;
-        if (slot < 0 || slot + at.y > a.slots) return;
-        const int64_t col = (slot * a.kv_heads + kvh) * a.width + c - block * wide, step = static_cast<int64_t>(a.kv_heads) * a.width;
-        float top = -INFINITY;
-        for (int s = 0; s < at.y; ++s) top = fmaxf(top, a.part_ml[col + s * step].x);
-        float sum = 0.f;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int s = 0; s < at.y; ++s) {
-            const float2 ml = a.part_ml[col + s * step];
-            const float4 x = *reinterpret_cast<const float4*>(a.part_acc + (col + s * step) * D + d);
-            const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top);
-            sum = fmaf(ml.y, f, sum);
-            v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
-        }
-        kv8_store4(a, static_cast<int64_t>(t) * a.out_stride + static_cast<int64_t>(kvh * a.group + g) * D + d, v, sum);
+    const int wide = 4 / ways_of(rows * a.group, WIDTH) * WIDTH;
+    const int c = i * a.group + h - kvh * a.group, block = c / wide;
+    int slot = at.x + block * at.y, splits = at.y;
+    if (at.w) {
+        const Shares how(a, at.w);
+        const int from = at.x + block * at.z;
+        slot = how.of(from);
+        splits = how.of(from + at.z - 1) - slot + 1;
+        slot += at.y + block;
     }
+    if (splits <= 1 || slot < 0 || slot > a.slots - splits) return;
+    const int64_t col = (static_cast<int64_t>(slot) * a.kv_heads + kvh) * a.width + c - block * wide, step = static_cast<int64_t>(a.kv_heads) * a.width;
+    float top = -INFINITY;
+    for (int s = threadIdx.x; s < splits; s += 256) top = fmaxf(top, a.part_ml[col + s * step].x);
+    top = wave_max(top);
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    const int way = threadIdx.x / kLanes, d = threadIdx.x % kLanes;
+    float sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = way; s < splits; s += kWays) {
+        const float2 ml = a.part_ml[col + s * step];
+        const float4 x = reinterpret_cast<const float4*>(a.part_acc + (col + s * step) * D)[d];
+        const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top);
+        sum = fmaf(ml.y, f, sum);
+        v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
+    }
+    sv[way][d] = v;
+    if (d == 0) ssum[way] = sum;
+    __syncthreads();
+    if (way) return;
+#pragma unroll
+    for (int w = 1; w < kWays; ++w) {
+        const float4 x = sv[w][d];
+        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+        sum += ssum[w];
+    }
+    kv8_store4(a, static_cast<int64_t>(t) * a.out_stride + static_cast<int64_t>(h) * D + 4 * d, v, sum);
 }
 
 namespace {
@@ -550,10 +645,17 @@ size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 size_t kv8_bytes(const sfg_kv8_attn_args& a, int64_t slots, int width) {
     const size_t columns = static_cast<size_t>(slots) * a.kv_heads * width;
-    return up256(a.batch * sizeof(int2)) + up256(a.tokens * sizeof(int)) + up256(columns * sizeof(float2)) + up256(columns * a.head_dim * sizeof(float));
+    return up256(a.batch * sizeof(int4)) + up256(a.tokens * sizeof(int)) + up256(columns * sizeof(float2)) + up256(columns * a.head_dim * sizeof(float));
 }
 
 constexpr int64_t kMostSlots = 1 << 22;  // workgroups of a launch: 256 threads each
+constexpr int64_t kMaxTiles = 1 << 30;
+// Workgroups that tiles are dealt to: two a compute unit, all of them resident at once.  (768, where
+// registers allow three: 64 sequences of up to 8192 tokens 108 us for 108, 64 with 8 rows
+// 187 for 159.)  Fewer than 16 tiles for each: pieces (32 sequences of up to 2000 tokens 28 us,
+// dealt 33; 16 fp32 rows over up to 8192 47, pieces from 24 tiles down 53).
+constexpr int64_t kRound = 512;
+constexpr int kFew = 16;
 
 }  // namespace
 
@@ -567,44 +669,42 @@ Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a) {
     p.width = 16 * p.nt * (cols > 32 * p.nt ? 4 : cols > 16 * p.nt ? 2 : 1);
     const int64_t blocks = a.tokens * group / (64 * p.nt) + a.batch;  // of all sequences, at most
     if (blocks * a.kv_heads > kMostSlots) return p;
+    if (blocks * tiles > kMaxTiles) return p;
     p.mfma = true;
-    p.least = 4;
-    p.slots = static_cast<int>(blocks);
-    p.direct = cols <= 64 * p.nt;
-    if (p.direct) p.slots = static_cast<int>(a.batch);
-    if (a.kv_splits > 0) {
-        const int64_t fixed = std::min<int64_t>({a.kv_splits, tiles, kMostSlots / (blocks * a.kv_heads)});
-        if (fixed > 1) {
-            p.fixed = static_cast<int>(fixed);
-            p.slots = static_cast<int>(blocks * fixed);
-        }
-    } else {
-        const int64_t share = 1024 / a.kv_heads;
-        const int64_t slots = std::min(share + blocks, blocks * ((tiles + p.least - 1) / p.least));
-        if (share > blocks && slots > blocks && kv8_bytes(a, slots, p.width) <= (size_t{128} << 20)) {
-            p.share = static_cast<int>(share);
-            p.slots = static_cast<int>(slots);
-        }
+    p.least = 4;  // (a tile a wave)
+    p.few = kFew;
+    p.fixed = static_cast<int>(std::min<int64_t>({std::max(a.kv_splits, 0), tiles, kMostSlots / (blocks * a.kv_heads)}));
+    if (!p.fixed && tiles > p.least) {
+        p.share = static_cast<int>(std::max<int64_t>(kRound / a.kv_heads, 1));
+        p.slots = static_cast<int>(std::min(p.share + blocks, blocks * ((tiles + p.least - 1) / p.least)));
+        if (kv8_bytes(a, p.slots, p.width) > (size_t{128} << 20)) p.share = 0;
     }
-    if (p.share || p.fixed) {
-        p.direct = false;
-        p.bytes = kv8_bytes(a, p.slots, p.width);
+    if (!p.share) {
+        p.fixed = std::max(p.fixed, 1);
+        p.slots = static_cast<int>(blocks * p.fixed);
     }
+    if (p.fixed != 1) p.bytes = kv8_bytes(a, p.slots, p.width);
     return p;
 }
 
 namespace {
 
-template <bool FP8, int D>
+template <bool FP8, int D, bool P16>
 void launch_kv8_mfma(const Kv8Args& a, const Kv8Plan& p, bool narrow, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>(p.slots * a.kv_heads));
-    if (!narrow) attn_kv8_kernel<FP8, D, 3, 3, 1><<<grid, 256, 0, stream>>>(a);
-    else if (p.nt == 2) attn_kv8_kernel<FP8, D, 1, 2, 2><<<grid, 256, 0, stream>>>(a);
-    else attn_kv8_kernel<FP8, D, 1, 2, 1><<<grid, 256, 0, stream>>>(a);
+    if (!narrow) attn_kv8_kernel<FP8, D, 3, 3, 1, P16><<<grid, 256, 0, stream>>>(a);
+    else if (p.nt == 2) attn_kv8_kernel<FP8, D, 1, 2, 2, P16><<<grid, 256, 0, stream>>>(a);
+    else attn_kv8_kernel<FP8, D, 1, 2, 1, P16><<<grid, 256, 0, stream>>>(a);
     if (!p.bytes) return;
-    const dim3 joins(static_cast<unsigned>(a.tokens), static_cast<unsigned>(a.kv_heads));
-    if (p.nt == 2) attn_kv8_join_kernel<D, 32><<<joins, 128, 0, stream>>>(a);
-    else attn_kv8_join_kernel<D, 16><<<joins, 128, 0, stream>>>(a);
+    const dim3 joins(static_cast<unsigned>(a.tokens), static_cast<unsigned>(a.q_heads));
+    if (p.nt == 2) attn_kv8_join_kernel<D, 32><<<joins, 256, 0, stream>>>(a);
+    else attn_kv8_join_kernel<D, 16><<<joins, 256, 0, stream>>>(a);
+}
+
+template <bool FP8, int D>
+void launch_kv8_pages(const Kv8Args& a, const Kv8Plan& p, bool narrow, hipStream_t stream) {
+    if (a.pt == kPageTok) launch_kv8_mfma<FP8, D, true>(a, p, narrow, stream);
+    else launch_kv8_mfma<FP8, D, false>(a, p, narrow, stream);
 }
 
 }  // namespace
@@ -626,24 +726,24 @@ void launch_attn_kv8(const sfg_kv8_attn_args& s, const Kv8Plan& plan, void* work
                          (reinterpret_cast<uintptr_t>(s.scales) & 7) == 0;
     if (plan.mfma && aligned) {
         a.group = a.q_heads / a.kv_heads;
-        a.slots = plan.slots; a.share = plan.share; a.fixed = plan.fixed; a.least = plan.least;
-        a.direct = plan.direct; a.width = plan.width;
+        a.slots = plan.slots; a.share = plan.share; a.fixed = plan.fixed; a.least = plan.least; a.few = plan.few;
+        a.width = plan.width;
         a.vec = (reinterpret_cast<uintptr_t>(s.q) & 15) == 0 && s.q_stride % 8 == 0;
         a.out_vec = (reinterpret_cast<uintptr_t>(s.out) & 15) == 0 && s.out_stride % 4 == 0;
         if (plan.bytes) {
             char* at = static_cast<char*>(workspace);
             const size_t columns = static_cast<size_t>(plan.slots) * a.kv_heads * plan.width;
-            a.slot_of = reinterpret_cast<int2*>(at); at += up256(a.batch * sizeof(int2));
+            a.slot_of = reinterpret_cast<int4*>(at); at += up256(a.batch * sizeof(int4));
             a.sequence_of = reinterpret_cast<int*>(at); at += up256(a.tokens * sizeof(int));
             a.part_ml = reinterpret_cast<float2*>(at); at += up256(columns * sizeof(float2));
             a.part_acc = reinterpret_cast<float*>(at);
         }
         if (s.pool_dtype == SFG_FP8) {
-            if (a.dim == 128) launch_kv8_mfma<true, 128>(a, plan, narrow, stream);
-            else launch_kv8_mfma<true, 64>(a, plan, narrow, stream);
+            if (a.dim == 128) launch_kv8_pages<true, 128>(a, plan, narrow, stream);
+            else launch_kv8_pages<true, 64>(a, plan, narrow, stream);
         } else {
-            if (a.dim == 128) launch_kv8_mfma<false, 128>(a, plan, narrow, stream);
-            else launch_kv8_mfma<false, 64>(a, plan, narrow, stream);
+            if (a.dim == 128) launch_kv8_pages<false, 128>(a, plan, narrow, stream);
+            else launch_kv8_pages<false, 64>(a, plan, narrow, stream);
         }
         return;
     }

@@ -41,13 +41,14 @@ __device__ __forceinline__ float kv8_larger(float a, float b) { return a >= b ||
 void launch_kv_plan(const sfg_kv_plan_args& a, hipStream_t stream);
 void launch_rope(const sfg_rope_args& a, hipStream_t stream);
 void launch_kv8_append(const sfg_kv8_append_args& a, hipStream_t stream);
-// How an attention runs.  slots: workgroups a kv head, each a block of a sequence's columns and
-// a split of its tiles; `share`: over how many of them all tiles are dealt, at least `least`
-// a split; fixed: splits a sequence, if the caller says; direct: a slot is a sequence; width: the
-// most columns of a block.  bytes: 0 if nothing is split.
+// How an attention runs.  A unit is a block of at most `width` columns of a sequence over all
+// its tiles.  share: the workgroups a kv head that all tiles are dealt to if there are more than
+// `few` for each; with fewer, units are split into pieces of `least` tiles or more, at most
+// share and the units together.  fixed: pieces a unit, instead of both.  slots: workgroups a kv
+// head, and partial results.  bytes: 0 if no unit is split.
 struct Kv8Plan {
-    bool mfma, direct;
-    int nt, width, slots, share, fixed, least;
+    bool mfma;
+    int nt, width, slots, share, fixed, least, few;
     size_t bytes;
 };
 Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a);

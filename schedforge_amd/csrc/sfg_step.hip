@@ -192,10 +192,19 @@ void launch_kv_plan(const sfg_kv_plan_args& s, hipStream_t stream) {
 // ===========================================================================
 namespace {
 
+constexpr int kRopeThreads = 256;
+constexpr int kRopeItems = 2;              // of a thread at a time
+// Bytes written from which stores pass the caches by (2048 rows of 40 heads of 128, 21 MB: 8.9 us,
+// 10.1 through them; what is smaller is left to the L2s, 32 MB together, for the next operator).
+constexpr int64_t kRopeStream = 16 << 20;
+
 struct RopeArgs {
     const void* in[2]; void* out[2]; int64_t in_stride[2], out_stride[2]; int heads[2];
     const int32_t* positions; const uint64_t* turns; float magnitude;
     int tokens, dim, pairs, interleaved;
+    // a workgroup's rows and heads; units of a head and how to divide by them and by a row's
+    int rows, chunk, units;
+    uint32_t by_units, by_row;
 };
 
 // Cosine and sine of a position's angle.  position * turns wraps modulo 2^64 as whole turns
@@ -207,47 +216,154 @@ __device__ __forceinline__ float2 rope_angle(int position, uint64_t turns, float
     return make_float2(c * magnitude, s * magnitude);
 }
 
-template <typename T>
-__device__ __forceinline__ float rope_load(const T* p) {
-    if constexpr (sizeof(T) == 4) return *p;
-    else return bf16_to_f32(*p);
+// A vector of N values (16 bytes, or one value) as fp32 and back.
+template <typename T, int N>
+__device__ __forceinline__ void rope_load(const T* p, float (&v)[N]) {
+    if constexpr (N == 1) {
+        v[0] = sizeof(T) == 4 ? *reinterpret_cast<const float*>(p) : bf16_to_f32(*reinterpret_cast<const uint16_t*>(p));
+    } else if constexpr (sizeof(T) == 4) {
+        const float4 w = *reinterpret_cast<const float4*>(p);
+        v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+    } else {
+        const uint4 w = *reinterpret_cast<const uint4*>(p);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(u[i] << 16);
+            v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+        }
+    }
 }
-template <typename T>
-__device__ __forceinline__ T rope_store(float v) {
-    if constexpr (sizeof(T) == 4) return v;
-    else return static_cast<uint16_t>(cvt_pk_bf16(v, v));  // (a NaN stays one)
+template <bool STREAM>
+__device__ __forceinline__ void rope_store16(void* p, const uint4& v) {
+    typedef uint32_t uint32x4 __attribute__((ext_vector_type(4)));
+    if constexpr (STREAM) __builtin_nontemporal_store(__builtin_bit_cast(uint32x4, v), static_cast<uint32x4*>(p));
+    else *static_cast<uint4*>(p) = v;
+}
+template <typename T, int N, bool STREAM>
+__device__ __forceinline__ void rope_store(T* p, const float (&v)[N]) {
+    if constexpr (N == 1) {
+        if constexpr (sizeof(T) == 4) *p = v[0];
+        else *p = static_cast<uint16_t>(cvt_pk_bf16(v[0], v[0]));  // (a NaN stays one)
+    } else if constexpr (sizeof(T) == 4) {
+        rope_store16<STREAM>(p, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
+    } else {
+        rope_store16<STREAM>(p, make_uint4(cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3]), cvt_pk_bf16(v[4], v[5]), cvt_pk_bf16(v[6], v[7])));
+    }
 }
 
 }  // namespace
 
-// A thread a pair (or a value behind the rotary part) of a row, for all heads.
-template <typename T>
-__global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
-    const int units = a.dim - a.pairs;  // pairs, then the values behind them
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    const int64_t t = i / units;
-    const int u = static_cast<int>(i % units);
-    if (t >= a.tokens) return;
-    const int pos = a.positions[t];
-    if (pos < 0) return;
-    const bool turned = u < a.pairs;
-    const int d0 = turned ? (a.interleaved ? 2 * u : u) : u + a.pairs;
-    const int d1 = turned ? (a.interleaved ? 2 * u + 1 : u + a.pairs) : d0;
-    const float2 cs = turned ? rope_angle(pos, a.turns[u], a.magnitude) : make_float2(1.f, 0.f);
-    for (int w = 0; w < 2; ++w) {
-        const T* x = static_cast<const T*>(a.in[w]) + t * a.in_stride[w];
-        T* y = static_cast<T*>(a.out[w]) + t * a.out_stride[w];
-        for (int h = 0; h < a.heads[w]; ++h, x += a.dim, y += a.dim) {
-            if (!turned) {
-                y[d0] = x[d0];
-                continue;
+// A workgroup turns `chunk` heads of `rows` rows.  Its threads first make the rows' cosines and
+// sines, one each, into LDS: every head of a row uses the same ones.  A unit is then N
+// values and the N they are paired with (half layout), N values that are pairs (interleaved; of
+// single values the pair), or N that are copied.  Bound by HBM, each value read and written once:
+// the vectors of kRopeItems units are in flight per thread, the first ones while the angles are
+// made.  8192 rows of 32 + 8 heads of 128, bf16: 30.1 us (5.6 TB/s; 38.2 with stores that stay in the
+// caches, 67 with a thread a pair for all heads); 512 rows 6.0 us either way.
+template <typename T, int N, bool STREAM>
+__global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a) {
+    extern __shared__ float2 angles[];  // [rows][pairs]
+    const int tid = threadIdx.x;
+    const int first_row = blockIdx.x * a.rows, first_head = blockIdx.y * a.chunk;
+    const int rows = min(a.rows, a.tokens - first_row), heads = min(a.chunk, a.heads[0] + a.heads[1] - first_head);
+    // units of a head: paired vectors, then copied ones
+    const int paired = a.interleaved ? (N == 1 ? a.pairs : 2 * a.pairs / N) : a.pairs / N;
+    const bool partner = !a.interleaved || N == 1;  // the second value of a pair lies elsewhere
+    const int items = rows * a.chunk * a.units;
+
+    struct Item {
+        T* out;
+        int at, second;  // its angles (-1: copied), and how far its partner lies
+        int position;
+    };
+    Item item[kRopeItems];
+    float x[kRopeItems][N], y[kRopeItems][N];
+    auto load = [&](int i, int e) {
+        Item& it = item[i];
+        it.position = -1;
+        if (e >= items) return;
+        const int row = a.by_row ? __umulhi(e, a.by_row) : 0;
+        const int in_row = e - row * a.chunk * a.units;
+        const int h = a.by_units ? __umulhi(in_row, a.by_units) : in_row, u = in_row - h * a.units;
+        if (h >= heads) return;
+        it.position = a.positions[first_row + row];  // (looked at behind the loads)
+        int head = first_head + h;
+        const int which = head >= a.heads[0];
+        head -= which ? a.heads[0] : 0;
+        const bool turned = u < paired;
+        const int d = !turned ? 2 * a.pairs + (u - paired) * N : a.interleaved && N == 1 ? 2 * u : u * N;
+        it.at = turned ? row * a.pairs + (a.interleaved && N > 1 ? d / 2 : a.interleaved ? u : d) : -1;
+        it.second = turned && partner ? (a.interleaved ? 1 : a.pairs) : 0;
+        const int64_t t = first_row + row, o = static_cast<int64_t>(head) * a.dim + d;
+        const T* in = static_cast<const T*>(a.in[which]) + t * a.in_stride[which] + o;
+        it.out = static_cast<T*>(a.out[which]) + t * a.out_stride[which] + o;
+        rope_load<T, N>(in, x[i]);
+        if (it.second) rope_load<T, N>(in + it.second, y[i]);
+    };
+#pragma unroll
+    for (int i = 0; i < kRopeItems; ++i) load(i, tid + i * kRopeThreads);
+    for (int e = tid; e < rows * a.pairs; e += kRopeThreads) {
+        const int row = e / a.pairs;
+        angles[e] = rope_angle(a.positions[first_row + row], a.turns[e - row * a.pairs], a.magnitude);
+    }
+    __syncthreads();
+    for (int base = tid;; base += kRopeItems * kRopeThreads) {
+#pragma unroll
+        for (int i = 0; i < kRopeItems; ++i) {
+            const Item& it = item[i];
+            if (it.position < 0) continue;
+            if (it.at < 0) {
+                rope_store<T, N, STREAM>(it.out, x[i]);
+            } else if (it.second) {
+                float p[N], q[N];
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const float2 cs = angles[it.at + j];
+                    p[j] = x[i][j] * cs.x - y[i][j] * cs.y;
+                    q[j] = y[i][j] * cs.x + x[i][j] * cs.y;
+                }
+                rope_store<T, N, STREAM>(it.out, p);
+                rope_store<T, N, STREAM>(it.out + it.second, q);
+            } else if constexpr (N > 1) {
+                float p[N];
+#pragma unroll
+                for (int j = 0; j < N; j += 2) {
+                    const float2 cs = angles[it.at + j / 2];
+                    p[j] = x[i][j] * cs.x - x[i][j + 1] * cs.y;
+                    p[j + 1] = x[i][j + 1] * cs.x + x[i][j] * cs.y;
+                }
+                rope_store<T, N, STREAM>(it.out, p);
             }
-            const float p = rope_load(x + d0), q = rope_load(x + d1);
-            y[d0] = rope_store<T>(p * cs.x - q * cs.y);
-            y[d1] = rope_store<T>(q * cs.x + p * cs.y);
         }
+        if (base - tid + kRopeItems * kRopeThreads >= items) return;
+#pragma unroll
+        for (int i = 0; i < kRopeItems; ++i) load(i, base + (kRopeItems + i) * kRopeThreads);
     }
 }
+
+namespace {
+
+// ceil(2^32 / d): its high product with x is x / d while x * d < 2^32 (0 stands for d = 1).
+uint32_t reciprocal(uint32_t d) { return d == 1 ? 0 : static_cast<uint32_t>(((uint64_t{1} << 32) + d - 1) / d); }
+
+template <typename T, int N>
+void launch_rope_n(RopeArgs a, hipStream_t stream) {
+    a.units = (a.interleaved ? (N == 1 ? a.pairs : 2 * a.pairs / N) : a.pairs / N) + (a.dim - 2 * a.pairs) / N;
+    const int heads = a.heads[0] + a.heads[1];
+    constexpr int kMost = 2 * kRopeItems * kRopeThreads;
+    a.chunk = std::max(1, std::min(heads, (kMost + a.units - 1) / a.units));
+    a.rows = std::max(1, std::min({a.tokens, kMost / (a.chunk * a.units), kMost / a.pairs}));
+    a.by_units = reciprocal(a.units);
+    a.by_row = a.rows > 1 ? reciprocal(a.chunk * a.units) : 0;
+    const dim3 grid(static_cast<unsigned>((a.tokens + a.rows - 1) / a.rows), static_cast<unsigned>((heads + a.chunk - 1) / a.chunk));
+    const size_t lds = a.rows * a.pairs * sizeof(float2);
+    const bool streams = N > 1 && static_cast<int64_t>(a.tokens) * heads * a.dim * static_cast<int64_t>(sizeof(T)) >= kRopeStream;
+    if (streams) rope_kernel<T, N, true><<<grid, kRopeThreads, lds, stream>>>(a);
+    else rope_kernel<T, N, false><<<grid, kRopeThreads, lds, stream>>>(a);
+}
+
+}  // namespace
 
 void launch_rope(const sfg_rope_args& s, hipStream_t stream) {
     RopeArgs a{};
@@ -258,10 +374,14 @@ void launch_rope(const sfg_rope_args& s, hipStream_t stream) {
     a.positions = s.positions; a.turns = s.turns; a.magnitude = s.magnitude;
     a.tokens = static_cast<int>(s.tokens); a.dim = static_cast<int>(s.head_dim);
     a.pairs = static_cast<int>(s.rotary_dim / 2); a.interleaved = s.layout == SFG_ROPE_INTERLEAVED;
-    const int64_t units = static_cast<int64_t>(a.tokens) * (a.dim - a.pairs);
-    const dim3 grid(static_cast<unsigned>((units + 255) / 256));
-    if (s.dtype == SFG_F32) rope_kernel<float><<<grid, 256, 0, stream>>>(a);
-    else rope_kernel<uint16_t><<<grid, 256, 0, stream>>>(a);
+    // vectors of 16 bytes where heads, halves and rows begin on their borders
+    const int64_t per = s.dtype == SFG_F32 ? 4 : 8;
+    const bool vec = ((reinterpret_cast<uintptr_t>(s.q) | reinterpret_cast<uintptr_t>(s.k) | reinterpret_cast<uintptr_t>(s.q_out) |
+                       reinterpret_cast<uintptr_t>(s.k_out)) & 15) == 0 &&
+                     (a.in_stride[0] | a.in_stride[1] | a.out_stride[0] | a.out_stride[1] | a.dim) % per == 0 &&
+                     (a.interleaved ? 2 * a.pairs : a.pairs) % per == 0;
+    if (s.dtype == SFG_F32) vec ? launch_rope_n<float, 4>(a, stream) : launch_rope_n<float, 1>(a, stream);
+    else vec ? launch_rope_n<uint16_t, 8>(a, stream) : launch_rope_n<uint16_t, 1>(a, stream);
 }
 
 }  // namespace sfg

@@ -12,155 +12,170 @@ namespace sfg {
 // ===========================================================================
 namespace {
 
-constexpr int kPlanThreads = 1024;
-
 struct PlanArgs {
     const int32_t* keep; const int32_t* counts; int32_t* seq_lens; int32_t* page_table;
     int32_t* free_pages; int32_t* free_count; int32_t* starts; int32_t* positions; int64_t* slots;
     int batch, per, pages, pt, max_tokens;
-    __device__ int pages_of(int tokens) const { return (tokens + pt - 1) / pt; }
+    int shift;  // log2 of the page's tokens, -1 if they are no power of two
+    __device__ __forceinline__ int page_of(int pos) const { return shift >= 0 ? pos >> shift : pos / pt; }
+    __device__ __forceinline__ int pages_of(int tokens) const { return page_of(tokens + pt - 1); }
 };
 
-// Sums of the lanes' values up to each thread of the workgroup (each sum cut to `most`,
-// which the values do not exceed) and over all of it.
-__device__ int block_inclusive(int v, uint32_t most, int* sums, int& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t x = static_cast<uint32_t>(v);
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t y = __shfl_up(x, off, kWave);
-        if (lane >= off) x = min(x + y, most);
-    }
-    __syncthreads();
-    if (lane == 63) sums[wave] = static_cast<int>(x);
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-    for (int w = 0; w < kPlanThreads / 64; ++w) {
-        if (w == wave) before = all;
-        all = min(all + static_cast<uint32_t>(sums[w]), most);
-    }
-    total = static_cast<int>(all);
-    return static_cast<int>(min(x + before, most));
+// A sequence's tokens, the kept ones, and the ones it asks for (none past the capacity).
+struct PlanSeq {
+    int len, kept, want;
+};
+__device__ __forceinline__ PlanSeq plan_seq(const PlanArgs& a, int b) {
+    PlanSeq s{0, 0, 0};
+    if (b >= a.batch) return s;
+    const int capacity = a.per * a.pt;
+    const int len = a.seq_lens[b], keep = a.keep ? a.keep[b] : 0x7FFFFFFF, want = a.counts[b];
+    s.len = min(max(len, 0), capacity);
+    s.kept = min(max(keep, 0), s.len);
+    s.want = max(want, 0) > capacity - s.kept ? 0 : max(want, 0);
+    return s;
 }
 
-// The last entry of at[0, kPlanThreads) that is not above i.
+// Sums of two values up to each thread of the workgroup and over all of it.  The second one's
+// sums are cut to `most`, which its values do not exceed (64 of them fit 32 bits).
+template <int THREADS>
+__device__ __forceinline__ int2 block_inclusive(int2 v, int most, int2* sums, int2& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int2 x = make_int2(wave_inclusive(v.x), wave_inclusive(v.y));
+    if (lane == 63) sums[wave] = x;
+    __syncthreads();
+    int2 before = make_int2(0, 0), all = make_int2(0, 0);
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+        if (w == wave) before = all;
+        const int2 y = sums[w];
+        all = make_int2(all.x + y.x, min(all.y + y.y, most));
+    }
+    total = all;
+    return make_int2(x.x + before.x, min(x.y + before.y, most));
+}
+
+// The last entry of at[0, THREADS) that is not above i.
+template <int THREADS>
 __device__ __forceinline__ int owner(const int* at, int i) {
     int lo = 0;
 #pragma unroll
-    for (int step = kPlanThreads / 2; step > 0; step >>= 1)
+    for (int step = THREADS / 2; step > 0; step >>= 1)
         if (at[lo + step] <= i) lo += step;
     return lo;
 }
 
 __device__ __forceinline__ void place(const PlanArgs& a, int t, int b, int pos) {
-    const int id = a.page_table[static_cast<int64_t>(b) * a.per + pos / a.pt];
+    const int page = a.page_of(pos), id = a.page_table[static_cast<int64_t>(b) * a.per + page];
     a.positions[t] = pos;
-    a.slots[t] = id < 0 || id >= a.pages ? -1 : static_cast<int64_t>(id) * a.pt + pos % a.pt;
+    a.slots[t] = id < 0 || id >= a.pages ? -1 : static_cast<int64_t>(id) * a.pt + (pos - page * a.pt);
 }
 
 }  // namespace
 
-// One workgroup, a thread a sequence (1024 of them at a time): prefix sums give each
+// One workgroup, a thread a sequence (THREADS of them at a time): prefix sums give each
 // sequence its place on the free list and among the rows, and the pages and rows
-// themselves are dealt over all threads, which find their sequence by bisection.
-__global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a, int tokens_too) {
-    __shared__ int sums[kPlanThreads / 64];
-    __shared__ int at[kPlanThreads], from[kPlanThreads];
+// themselves are dealt over all threads, which find their sequence by bisection.  Bound by latency: a
+// chain of loads, three sums and the list's and table's round trips.  64 sequences of one row 3.6 us
+// (7.9 with the lengths read again for each sum, sums by shuffles and divisions by the page).
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void kv_plan_kernel(PlanArgs a, int rows_too) {
+    __shared__ int2 sums[3][THREADS / 64];
+    __shared__ int page_at[THREADS], page_from[THREADS], row_at[THREADS], row_from[THREADS];
     const int tid = threadIdx.x;
-    const int capacity = a.per * a.pt;
-    constexpr uint32_t kAny = 0x7FFFFFFFu;
+    constexpr int kAny = 0x7FFFFFFF;
     const int had = min(max(a.free_count[0], 0), a.pages);
+    PlanSeq s = plan_seq(a, tid);
     // (the tables' entries are fewer than 2^31: so are the pages given back)
     int given = 0;
     if (a.keep) {
-        for (int base = 0; base < a.batch; base += kPlanThreads) {
-            const int b = base + tid;
-            int last = 0, gone = 0;
-            if (b < a.batch) {
-                const int len = min(max(a.seq_lens[b], 0), capacity);
-                last = a.pages_of(len);
-                gone = last - a.pages_of(min(max(a.keep[b], 0), len));
+        for (int base = 0;;) {
+            const int last = a.pages_of(s.len), gone = last - a.pages_of(s.kept);
+            int2 total;
+            const int upto = block_inclusive<THREADS>(make_int2(gone, 0), kAny, sums[0], total).x;
+            if (total.x) {
+                page_at[tid] = upto - gone;
+                page_from[tid] = last - 1;
+                __syncthreads();
+                for (int i = tid; i < total.x; i += THREADS) {
+                    const int q = owner<THREADS>(page_at, i);
+                    int32_t* entry = a.page_table + static_cast<int64_t>(base + q) * a.per + (page_from[q] - (i - page_at[q]));
+                    const int64_t to = static_cast<int64_t>(had) + given + i;
+                    if (to < a.pages) a.free_pages[to] = *entry;
+                    *entry = -1;
+                }
+                given += total.x;
+                __syncthreads();
             }
-            int total;
-            const int upto = block_inclusive(gone, kAny, sums, total);
-            at[tid] = upto - gone;
-            from[tid] = last - 1;
+            if ((base += THREADS) >= a.batch) break;
             __syncthreads();
-            for (int i = tid; i < total; i += kPlanThreads) {
-                const int q = owner(at, i);
-                int32_t* entry = a.page_table + static_cast<int64_t>(base + q) * a.per + (from[q] - (i - at[q]));
-                const int64_t to = static_cast<int64_t>(had) + given + i;
-                if (to < a.pages) a.free_pages[to] = *entry;
-                *entry = -1;
-            }
-            given += total;
-            __syncthreads();
+            s = plan_seq(a, base + tid);
         }
+        if (a.batch > THREADS) s = plan_seq(a, tid);
     }
     const int have = static_cast<int>(min(static_cast<int64_t>(had) + given, static_cast<int64_t>(a.pages)));
-    const uint32_t most = static_cast<uint32_t>(a.max_tokens) + 1;
+    const int most = a.max_tokens + 1;
     int asked = 0, rows_asked = 0, taken = 0, rows = 0;
-    for (int base = 0; base < a.batch; base += kPlanThreads) {
-        const int b = base + tid;
-        int kept = 0, want = 0, need = 0, first = 0;
+    for (int base = 0;;) {
+        const int b = base + tid, first = a.pages_of(s.kept);
+        int want = s.want, need = a.pages_of(s.kept + want) - first;
+        int2 total;
+        int2 upto = block_inclusive<THREADS>(make_int2(need, min(want, most)), most, sums[1], total);
+        if ((need > 0 && asked + upto.x > have) || rows_asked + upto.y >= most) want = need = 0;
+        asked += total.x;
+        rows_asked = min(rows_asked + total.y, most);
+        upto = block_inclusive<THREADS>(make_int2(need, want), kAny, sums[2], total);
+        page_at[tid] = upto.x - need;
+        page_from[tid] = first;
+        row_at[tid] = upto.y - want;
+        row_from[tid] = s.kept;
         if (b < a.batch) {
-            const int len = min(max(a.seq_lens[b], 0), capacity);
-            kept = a.keep ? min(max(a.keep[b], 0), len) : len;
-            want = max(a.counts[b], 0);
-            if (want > capacity - kept) want = 0;
-            first = a.pages_of(kept);
-            need = a.pages_of(kept + want) - first;
-        }
-        int total;
-        const int need_upto = asked + block_inclusive(need, kAny, sums, total);
-        asked += total;
-        const uint32_t cut = min(static_cast<uint32_t>(want), most);
-        const uint32_t want_upto = min(static_cast<uint32_t>(block_inclusive(static_cast<int>(cut), most, sums, total)) + rows_asked, most);
-        rows_asked = static_cast<int>(min(static_cast<uint32_t>(rows_asked) + total, most));
-        if ((need > 0 && need_upto > have) || want_upto >= most) want = need = 0;
-        // pages
-        int upto = block_inclusive(need, kAny, sums, total);
-        at[tid] = upto - need;
-        from[tid] = first;
-        __syncthreads();
-        for (int i = tid; i < total; i += kPlanThreads) {
-            const int q = owner(at, i);
-            a.page_table[static_cast<int64_t>(base + q) * a.per + from[q] + (i - at[q])] = a.free_pages[have - 1 - taken - i];
-        }
-        taken += total;
-        // rows
-        upto = block_inclusive(want, kAny, sums, total);  // (its barriers are behind the pages' last reads)
-        at[tid] = upto - want;
-        from[tid] = kept;
-        if (b < a.batch) {
-            a.seq_lens[b] = kept + want;
-            a.starts[b] = rows + upto - want;
+            a.seq_lens[b] = s.kept + want;
+            a.starts[b] = rows + upto.y - want;
         }
         __syncthreads();
-        if (tokens_too)
-            for (int i = tid; i < total; i += kPlanThreads) {
-                const int q = owner(at, i);
-                place(a, rows + i, base + q, from[q] + (i - at[q]));
+        for (int i = tid; i < total.x; i += THREADS) {
+            const int q = owner<THREADS>(page_at, i);
+            a.page_table[static_cast<int64_t>(base + q) * a.per + page_from[q] + (i - page_at[q])] = a.free_pages[have - 1 - taken - i];
+        }
+        if (rows_too) {
+            if (total.x) __syncthreads();
+            for (int i = tid; i < total.y; i += THREADS) {
+                const int q = owner<THREADS>(row_at, i);
+                place(a, rows + i, base + q, row_from[q] + (i - row_at[q]));
             }
-        rows += total;
+        }
+        taken += total.x;
+        rows += total.y;
+        if ((base += THREADS) >= a.batch) break;
+        s = plan_seq(a, base + tid);
         __syncthreads();
     }
     if (tid == 0) {
         a.starts[a.batch] = rows;
         a.free_count[0] = have - taken;
     }
-    if (tokens_too)
-        for (int t = rows + tid; t < a.max_tokens; t += kPlanThreads) {
+    if (rows_too)
+        for (int t = rows + tid; t < a.max_tokens; t += THREADS) {
             a.positions[t] = -1;
             a.slots[t] = -1;
         }
 }
 
-// The rows of a step of many tokens: a thread a row, its sequence by bisection.
+// The rows of a step of many: a thread a row, its sequence by bisection of the starts (in LDS
+// where they fit).
+constexpr int kPlanStarts = 2048;
 __global__ __launch_bounds__(256) void kv_plan_rows_kernel(PlanArgs a) {
+    __shared__ int begins[kPlanStarts];
+    const bool fit = a.batch < kPlanStarts;
+    if (fit) {
+        for (int i = threadIdx.x; i <= a.batch; i += 256) begins[i] = a.starts[i];
+        __syncthreads();
+    }
+    const int* starts = fit ? begins : a.starts;
     const int t = blockIdx.x * 256 + threadIdx.x;
     if (t >= a.max_tokens) return;
-    if (t >= a.starts[a.batch]) {
+    if (t >= starts[a.batch]) {
         a.positions[t] = -1;
         a.slots[t] = -1;
         return;
@@ -168,11 +183,15 @@ __global__ __launch_bounds__(256) void kv_plan_rows_kernel(PlanArgs a) {
     int lo = 0, hi = a.batch;  // starts[lo] <= t < starts[hi]
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (a.starts[mid] <= t) lo = mid;
+        if (starts[mid] <= t) lo = mid;
         else hi = mid;
     }
-    place(a, t, lo, a.seq_lens[lo] - (a.starts[lo + 1] - a.starts[lo]) + (t - a.starts[lo]));
+    place(a, t, lo, a.seq_lens[lo] - (starts[lo + 1] - starts[lo]) + (t - starts[lo]));
 }
+
+// Rows that the workgroup places itself: 8 x 250 in 7.3 us a call, 9.8 with a second launch; 8 x 500
+// 7.6 and 9.8; 16 x 500 9.8 and 9.5.
+constexpr int kPlanRows = 4096;
 
 void launch_kv_plan(const sfg_kv_plan_args& s, hipStream_t stream) {
     PlanArgs a{};
@@ -182,8 +201,10 @@ void launch_kv_plan(const sfg_kv_plan_args& s, hipStream_t stream) {
     a.batch = static_cast<int>(s.batch); a.per = static_cast<int>(s.pages_per_seq);
     a.pages = static_cast<int>(s.num_pages); a.pt = static_cast<int>(s.page_tokens);
     a.max_tokens = static_cast<int>(s.max_tokens);
-    const bool one = a.max_tokens <= 4 * kPlanThreads;
-    kv_plan_kernel<<<1, kPlanThreads, 0, stream>>>(a, one);
+    a.shift = (a.pt & (a.pt - 1)) == 0 ? __builtin_ctz(a.pt) : -1;
+    const bool one = a.max_tokens <= kPlanRows;
+    if (a.batch <= 256 && a.max_tokens <= 1024) kv_plan_kernel<256><<<1, 256, 0, stream>>>(a, 1);
+    else kv_plan_kernel<1024><<<1, 1024, 0, stream>>>(a, one);
     if (!one) kv_plan_rows_kernel<<<dim3(static_cast<unsigned>((a.max_tokens + 255) / 256)), 256, 0, stream>>>(a);
 }
 

@@ -154,7 +154,8 @@ __global__ __launch_bounds__(64) void attn_kv8_rows_kernel(Kv8Args a) {
 // them, V's after the second: a wave has up to 16 KB in flight.
 //
 // A workgroup is four waves: one column group, its tiles split four ways, for up to 16 NT
-// columns; two by two for twice that; else four column groups over the same tiles.
+// columns; two by two for twice that; else four column groups over the same tiles.  (Eight waves
+// where that makes a split and its join unnecessary.)
 // ===========================================================================
 namespace {
 
@@ -162,9 +163,9 @@ constexpr int kTile = 64;
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// Columns that a workgroup takes of a sequence: its waves' tiles split four ways, two ways or
-// not at all.
-__device__ __forceinline__ int ways_of(int cols, int width) { return cols > 2 * width ? 1 : cols > width ? 2 : 4; }
+// Column groups of `width` that a workgroup has of a sequence: each has its share of the waves, which
+// split the tiles.
+__device__ __forceinline__ int groups_of(int cols, int width) { return cols > 2 * width ? 4 : cols > width ? 2 : 1; }
 __device__ __forceinline__ int blocks_of(int cols, int width) { return cols > 4 * width ? ceil_div(cols, 4 * width) : cols > 0; }
 
 // A unit of work: a block of a sequence's columns over all its tiles.
@@ -289,8 +290,8 @@ __device__ __forceinline__ void weight_terms(float p0, float p1, uint32_t* t) {
 
 }  // namespace
 
-template <bool FP8, int D, int QT, int PT, int NT, bool P16>
-__global__ __launch_bounds__(256, QT == 3 ? (D == 64 ? 3 : 2) : NT == 2 ? 2 : D == 64 ? 4 : 3) void attn_kv8_kernel(Kv8Args a) {
+template <bool FP8, int D, int QT, int PT, int NT, bool P16, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : QT == 3 || NT == 2 ? (D == 64 ? 3 : 2) : D == 64 ? 4 : 3) void attn_kv8_kernel(Kv8Args a) {
     static_assert(D == 64 || D == 128, "16 bytes of 4 lanes make a k-step");
     constexpr int kF = D / 32, kDt = D / 16, kLd = D + 4, kCols = 16 * NT;
     // a wave's queries as operands, which the loop reads again for each tile; then its sums
@@ -298,8 +299,8 @@ __global__ __launch_bounds__(256, QT == 3 ? (D == 64 ? 3 : 2) : NT == 2 ? 2 : D 
         uint4 q[NT][kF][QT][kWave];
         float o[kCols][kLd];
     };
-    __shared__ Wave sw[4];
-    __shared__ float sm[4][kCols], sl[4][kCols];
+    __shared__ Wave sw[WAVES];
+    __shared__ float sm[WAVES][kCols], sl[WAVES][kCols];
     const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int group = blockIdx.x / a.kv_heads, kvh = blockIdx.x - group * a.kv_heads;
@@ -337,7 +338,7 @@ __global__ __launch_bounds__(256, QT == 3 ? (D == 64 ? 3 : 2) : NT == 2 ? 2 : D 
         same(left);
         const int count = min(left, u.tiles - tile0);
         const int cols = min(u.rows, a.max_rows) * a.group;
-        const int ways = ways_of(cols, kCols), groups = 4 / ways, col0 = u.block * groups * kCols;
+        const int groups = groups_of(cols, kCols), ways = WAVES / groups, col0 = u.block * groups * kCols;
         const int wcol = col0 + wave % groups * kCols;  // (may lie behind the columns)
         // tokens that all of the wave's columns see, and that any does
         const int seen_all = max(u.len - u.rows + wcol / a.group + 1, 0);
@@ -438,7 +439,6 @@ __global__ __launch_bounds__(256, QT == 3 ? (D == 64 ? 3 : 2) : NT == 2 ? 2 : D 
 #pragma unroll
                             for (int e = QT - 1; e >= 0; --e) s[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[n][e], s[n][i], 0, 0, 0);
                     }
-                    __builtin_amdgcn_sched_barrier(0);
                 }
                 if (t + 1 < end) load_k(page_k, sub_k);
                 const int base = t * kTile + lg * 16;  // the lane's run
@@ -448,15 +448,14 @@ __global__ __launch_bounds__(256, QT == 3 ? (D == 64 ? 3 : 2) : NT == 2 ? 2 : D 
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const int live = vok ? min(max(seen[n] - base, 0), 16) : 0;  // tokens of the run that the column sees
+                    if (part) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[n][i / 4][i % 4] = i < live ? s[n][i / 4][i % 4] : -INFINITY;
+                    }
                     float top = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            s[n][i][r] *= fk;
-                            if (part && 4 * i + r >= live) s[n][i][r] = -INFINITY;
-                            top = fmaxf(top, s[n][i][r]);
-                        }
+                    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i / 4][i % 4]);
+                    top = top == -INFINITY ? top : top * fk;  // (nothing seen, and fk may be 0)
                     top = xor32_max(xor16_max(top));
                     // the running maximum moves only when a score is 2^8 above it
                     if (__any(top > m[n] + 8.0f)) {
@@ -473,13 +472,20 @@ __global__ __launch_bounds__(256, QT == 3 ? (D == 64 ? 3 : 2) : NT == 2 ? 2 : D 
                     float w[16];
                     float sum = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                    for (int i = 0; i < 16; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(s[n][i / 4][i % 4], fk, -ref));
+                    if (part) {  // (0 * -inf, or a scale that is NaN, where nothing is seen)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const float p = __builtin_amdgcn_exp2f(s[n][i][r] - ref);
-                            sum += p;
-                            w[4 * i + r] = part && 4 * i + r >= live ? 0.0f : p * fv;
-                        }
+                        for (int i = 0; i < 16; ++i) w[i] = i < live ? w[i] : 0.0f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        sum += w[i];
+                        w[i] *= fv;
+                    }
+                    if (part) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) w[i] = i < live ? w[i] : 0.0f;
+                    }
                     l[n] += sum;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -503,7 +509,6 @@ __global__ __launch_bounds__(256, QT == 3 ? (D == 64 ? 3 : 2) : NT == 2 ? 2 : D 
                 }
 #pragma unroll
                 for (int d = 0; d < kDt; ++d) {
-                    if (d % 2 == 0) __builtin_amdgcn_sched_barrier(0);
                     const bf16x8 v0 = kv8_operand<FP8>(vr[d].x, vr[d].y), v1 = kv8_operand<FP8>(vr[d].z, vr[d].w);
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
@@ -535,7 +540,7 @@ __global__ __launch_bounds__(256, QT == 3 ? (D == 64 ? 3 : 2) : NT == 2 ? 2 : D 
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             float top = -INFINITY;
-            for (int w = wave % groups; w < 4; w += groups) top = fmaxf(top, sm[w][16 * n + lr]);
+            for (int w = wave % groups; w < WAVES; w += groups) top = fmaxf(top, sm[w][16 * n + lr]);
             const float f = m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[n] - top);
 #pragma unroll
             for (int d = 0; d < kDt; ++d) {
@@ -546,14 +551,14 @@ __global__ __launch_bounds__(256, QT == 3 ? (D == 64 ? 3 : 2) : NT == 2 ? 2 : D 
         __syncthreads();
         const bool whole = count == u.tiles;
         const int64_t part = (static_cast<int64_t>(how.each ? group : group + u.ord) * a.kv_heads + kvh) * a.width;
-        for (int e = threadIdx.x; e < groups * kCols * (D / 4); e += 256) {
+        for (int e = threadIdx.x; e < groups * kCols * (D / 4); e += 64 * WAVES) {
             const int c = e / (D / 4), d = e % (D / 4) * 4, gr = c / kCols, cc = c % kCols;
             const int col = col0 + c;
             if (col >= cols) break;
             float top = -INFINITY, sum = 0.f;
-            for (int w = gr; w < 4; w += groups) top = fmaxf(top, sm[w][cc]);
+            for (int w = gr; w < WAVES; w += groups) top = fmaxf(top, sm[w][cc]);
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int w = gr; w < 4; w += groups) {
+            for (int w = gr; w < WAVES; w += groups) {
                 sum += sl[w][cc] * (sm[w][cc] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[w][cc] - top));
                 const float4 x = *reinterpret_cast<const float4*>(&sw[w].o[cc][d]);
                 v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
@@ -569,7 +574,7 @@ __global__ __launch_bounds__(256, QT == 3 ? (D == 64 ? 3 : 2) : NT == 2 ? 2 : D 
         // where the join finds a row's sequence, and the sequence's pieces or tiles among all
         if (a.slot_of && tile0 == 0 && kvh == 0) {
             if (u.block == 0 && threadIdx.x == 0) a.slot_of[u.b] = make_int4(u.before, how.each ? how.pieces(u.tiles) : u.ord, u.tiles, how.each ? 0 : all);
-            for (int e = threadIdx.x; e < groups * kCols; e += 256)
+            for (int e = threadIdx.x; e < groups * kCols; e += 64 * WAVES)
                 if (col0 + e < cols) a.sequence_of[u.t0 + (col0 + e) / a.group] = u.b;
         }
         if ((left -= count) <= 0) return;
@@ -580,16 +585,20 @@ __global__ __launch_bounds__(256, QT == 3 ? (D == 64 ? 3 : 2) : NT == 2 ? 2 : D 
     }
 }
 
-// The splits of a row and query head: weights 2^(m_s - M).  D / 4 lanes to a split, 8 or 16
-// splits at a time, then those sums in a fixed order.  (90 splits one after the other: 45 us.)
-template <int D, int WIDTH>
+// The splits of a row and query head: weights 2^(m_s - M), sums in a fixed order.  D / 4 lanes to a
+// split.  TOGETHER: all of a workgroup's for one row and head, so many splits at a time; else
+// each D / 4 lanes for one of their own, which pays where there are many rows (519 of 32 heads,
+// about 5 splits: .. us, 30 together) and not where there are few (2 of 32 heads, 90 splits: 45 one
+// after the other, 5 together).
+template <int D, int WIDTH, bool TOGETHER>
 __global__ __launch_bounds__(256) void attn_kv8_join_kernel(Kv8Args a) {
-    constexpr int kLanes = D / 4, kWays = 256 / kLanes;  // lanes of a split, splits at a time
-    __shared__ float tops[4];
+    constexpr int kLanes = D / 4, kWays = TOGETHER ? 256 / kLanes : 1;
     __shared__ float4 sv[kWays][kLanes];
-    __shared__ float ssum[kWays];
-    const int t = blockIdx.x, h = blockIdx.y, kvh = h / a.group;
-    if (a.starts && t >= a.starts[a.batch]) return;
+    __shared__ float ssum[kWays], stop[kWays];
+    const int at_once = TOGETHER ? 1 : 256 / kLanes;
+    const int way = TOGETHER ? threadIdx.x / kLanes : 0, d = threadIdx.x % kLanes;
+    const int t = blockIdx.x, h = blockIdx.y * at_once + (TOGETHER ? 0 : threadIdx.x / kLanes), kvh = h / a.group;
+    if (h >= a.q_heads || (a.starts && t >= a.starts[a.batch])) return;  // (uniform where lanes work together)
     const int b = min(max(a.sequence_of[t], 0), a.batch - 1);
     const int4 at = a.slot_of[b];
     int t0, rows, len;
@@ -597,7 +606,7 @@ __global__ __launch_bounds__(256) void attn_kv8_join_kernel(Kv8Args a) {
     const int i = t - t0;
     rows = min(rows, a.max_rows);
     if (i < 0 || i >= rows) return;  // (a row that no sequence computes)
-    const int wide = 4 / ways_of(rows * a.group, WIDTH) * WIDTH;
+    const int wide = groups_of(rows * a.group, WIDTH) * WIDTH;
     const int c = i * a.group + h - kvh * a.group, block = c / wide;
     int slot = at.x + block * at.y, splits = at.y;
     if (at.w) {
@@ -609,32 +618,40 @@ __global__ __launch_bounds__(256) void attn_kv8_join_kernel(Kv8Args a) {
     }
     if (splits <= 1 || slot < 0 || slot > a.slots - splits) return;
     const int64_t col = (static_cast<int64_t>(slot) * a.kv_heads + kvh) * a.width + c - block * wide, step = static_cast<int64_t>(a.kv_heads) * a.width;
-    float top = -INFINITY;
-    for (int s = threadIdx.x; s < splits; s += 256) top = fmaxf(top, a.part_ml[col + s * step].x);
-    top = wave_max(top);
-    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    const int way = threadIdx.x / kLanes, d = threadIdx.x % kLanes;
-    float sum = 0.f;
+    // a running maximum: the splits' own are not known before
+    float top = -INFINITY, sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int s = way; s < splits; s += kWays) {
         const float2 ml = a.part_ml[col + s * step];
         const float4 x = reinterpret_cast<const float4*>(a.part_acc + (col + s * step) * D)[d];
-        const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top);
-        sum = fmaf(ml.y, f, sum);
-        v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
+        const float to = fmaxf(top, ml.x);
+        const float keep = top == to ? 1.0f : __builtin_amdgcn_exp2f(top - to);  // (-infinity for both: nothing yet)
+        const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - to);  // (NaN sums stay NaN)
+        top = to;
+        sum = fmaf(ml.y, f, sum * keep);
+        v.x = fmaf(x.x, f, v.x * keep); v.y = fmaf(x.y, f, v.y * keep); v.z = fmaf(x.z, f, v.z * keep); v.w = fmaf(x.w, f, v.w * keep);
     }
-    sv[way][d] = v;
-    if (d == 0) ssum[way] = sum;
-    __syncthreads();
-    if (way) return;
+    if constexpr (TOGETHER) {
+        sv[way][d] = v;
+        if (d == 0) {
+            ssum[way] = sum;
+            stop[way] = top;
+        }
+        __syncthreads();
+        if (way) return;
+        float all = -INFINITY;
 #pragma unroll
-    for (int w = 1; w < kWays; ++w) {
-        const float4 x = sv[w][d];
-        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-        sum += ssum[w];
+        for (int w = 0; w < kWays; ++w) all = fmaxf(all, stop[w]);
+        sum = 0.f;
+        v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWays; ++w) {
+            const float f = stop[w] == all ? 1.0f : __builtin_amdgcn_exp2f(stop[w] - all);
+            const float4 x = sv[w][d];
+            sum = fmaf(ssum[w], f, sum);
+            v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
+        }
     }
     kv8_store4(a, static_cast<int64_t>(t) * a.out_stride + static_cast<int64_t>(h) * D + 4 * d, v, sum);
 }
@@ -656,6 +673,14 @@ constexpr int64_t kMaxTiles = 1 << 30;
 // dealt 33; 16 fp32 rows over up to 8192 47, pieces from 24 tiles down 53).
 constexpr int64_t kRound = 512;
 constexpr int kFew = 16;
+#ifndef MANYR
+#define MANYR 4096
+#endif
+#ifndef SHORTT
+#define SHORTT 16
+#endif
+constexpr int64_t kManyRows = MANYR;  // rows by heads from which a join's lanes have one each
+constexpr int64_t kShort = SHORTT;    // tiles up to which eight waves take a unit whole
 
 }  // namespace
 
@@ -674,6 +699,11 @@ Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a) {
     p.least = 4;  // (a tile a wave)
     p.few = kFew;
     p.fixed = static_cast<int>(std::min<int64_t>({std::max(a.kv_splits, 0), tiles, kMostSlots / (blocks * a.kv_heads)}));
+    p.waves = 4;
+    if (!p.fixed && narrow && p.nt == 1 && tiles <= kShort && tiles > p.least) {
+        p.waves = 8;
+        p.fixed = 1;
+    }
     if (!p.fixed && tiles > p.least) {
         p.share = static_cast<int>(std::max<int64_t>(kRound / a.kv_heads, 1));
         p.slots = static_cast<int>(std::min(p.share + blocks, blocks * ((tiles + p.least - 1) / p.least)));
@@ -689,16 +719,25 @@ Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a) {
 
 namespace {
 
+template <int D, int WIDTH>
+void launch_kv8_join(const Kv8Args& a, hipStream_t stream) {
+    constexpr int kAtOnce = 256 / (D / 4);
+    if (static_cast<int64_t>(a.tokens) * a.q_heads >= kManyRows)
+        attn_kv8_join_kernel<D, WIDTH, false><<<dim3(static_cast<unsigned>(a.tokens), static_cast<unsigned>((a.q_heads + kAtOnce - 1) / kAtOnce)), 256, 0, stream>>>(a);
+    else
+        attn_kv8_join_kernel<D, WIDTH, true><<<dim3(static_cast<unsigned>(a.tokens), static_cast<unsigned>(a.q_heads)), 256, 0, stream>>>(a);
+}
+
 template <bool FP8, int D, bool P16>
 void launch_kv8_mfma(const Kv8Args& a, const Kv8Plan& p, bool narrow, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>(p.slots * a.kv_heads));
-    if (!narrow) attn_kv8_kernel<FP8, D, 3, 3, 1, P16><<<grid, 256, 0, stream>>>(a);
-    else if (p.nt == 2) attn_kv8_kernel<FP8, D, 1, 2, 2, P16><<<grid, 256, 0, stream>>>(a);
-    else attn_kv8_kernel<FP8, D, 1, 2, 1, P16><<<grid, 256, 0, stream>>>(a);
+    if (!narrow) attn_kv8_kernel<FP8, D, 3, 3, 1, P16, 4><<<grid, 256, 0, stream>>>(a);
+    else if (p.nt == 2) attn_kv8_kernel<FP8, D, 1, 2, 2, P16, 4><<<grid, 256, 0, stream>>>(a);
+    else if (p.waves == 8) attn_kv8_kernel<FP8, D, 1, 2, 1, P16, 8><<<grid, 512, 0, stream>>>(a);
+    else attn_kv8_kernel<FP8, D, 1, 2, 1, P16, 4><<<grid, 256, 0, stream>>>(a);
     if (!p.bytes) return;
-    const dim3 joins(static_cast<unsigned>(a.tokens), static_cast<unsigned>(a.q_heads));
-    if (p.nt == 2) attn_kv8_join_kernel<D, 32><<<joins, 256, 0, stream>>>(a);
-    else attn_kv8_join_kernel<D, 16><<<joins, 256, 0, stream>>>(a);
+    if (p.nt == 2) launch_kv8_join<D, 32>(a, stream);
+    else launch_kv8_join<D, 16>(a, stream);
 }
 
 template <bool FP8, int D>

@@ -48,7 +48,7 @@ void launch_kv8_append(const sfg_kv8_append_args& a, hipStream_t stream);
 // head, and partial results.  bytes: 0 if no unit is split.
 struct Kv8Plan {
     bool mfma;
-    int nt, width, slots, share, fixed, least, few;
+    int nt, waves, width, slots, share, fixed, least, few;
     size_t bytes;
 };
 Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a);

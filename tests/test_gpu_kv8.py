@@ -98,7 +98,7 @@ def test_plan_takes_lists_that_hold_anything():
 # ---------------------------------------------------------------- rotary positions
 ROPES = [  # tokens, q heads, kv heads, head dim, rotary dim
     (1, 32, 8, 128, 128), (1, 1, 1, 2, 2), (7, 4, 2, 64, 64), (130, 16, 4, 64, 16), (33, 3, 1, 80, 40), (5, 2, 2, 33, 30),
-    (3, 5, 5, 256, 128), (64, 8, 8, 128, 96), (9, 1, 1, 1024, 1024), (2000, 4, 1, 128, 128), (257, 6, 3, 96, 96)]
+    (3, 5, 5, 256, 128), (64, 8, 8, 128, 96), (9, 1, 1, 1024, 1024), (2000, 4, 1, 128, 128), (257, 6, 3, 96, 96), (1700, 32, 8, 128, 128)]  # (the last one writes over 16 MB)
 
 
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
@@ -332,6 +332,63 @@ def test_splits(hq, hkv, d, pt, rows, splits):
     lens = [900, 64, 9, 333]
     cache, model, table = filled(rng, lens, hkv, d, pt, "int8")
     check_attention(cache, model, table, lens, [rows] * 4, hq, BF16, rng, kv_splits=splits, max_rows=rows, max_context=900)
+
+
+def random_cache(rng, lens, heads, d, pt, kind, spare=5):
+    """As `filled`, with codes and scales drawn as they are."""
+    batch, capacity = len(lens), max(lens) + pt
+    need = [-(-n // pt) for n in lens]
+    cache = make(batch, heads, d, pt, capacity, kind, sum(need) + spare)
+    model = plain.Cache(cache.num_pages, heads, pt, d, kind)
+    model.codes[:] = rng.integers(0, 256, model.codes.shape)
+    model.codes[model.codes & 0x7F == 0x7F] = 3                       # (e4m3's NaN)
+    model.scales[:] = np.exp(rng.standard_normal(model.scales.shape)) * (0.02 if kind == "int8" else 0.01)
+    ids = rng.permutation(cache.num_pages)
+    table = np.full((batch, cache.config.pages_per_seq), -1)
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = ids[at: at + n]
+        at += n
+    model.upload(cache)
+    cache.page_table.copy_(dev(table, torch.int32))
+    cache.seq_lens.copy_(dev(lens, torch.int32))
+    return cache, model, table
+
+
+LONG = [  # q heads, kv heads, head dim, page tokens, lengths, rows
+    (4, 2, 128, 16, [2500, 1, 700], [1, 1, 1]),
+    (4, 2, 64, 32, [3000] + [90] * 69 + [1100], [1] * 35 + [0] + [1] * 35),
+    (6, 2, 128, 16, [1500, 2000, 64], [40, 3, 1]),
+    (20, 2, 64, 16, [1300, 1100], [2, 2]),
+    # more than 16 tiles for each of the 512 / 64 workgroups of a head: dealt across sequences
+    (64, 64, 64, 16, [4000, 3, 64, 0, 2111, 900, 1537], [1, 1, 1, 0, 1, 1, 1]),
+    (64, 64, 64, 64, [130] * 66 + [1000, 129], [1] * 3 + [0] * 2 + [1] * 63),
+    (64, 64, 128, 16, [2900, 5000, 1200], [4, 40, 1]),
+    (128, 64, 64, 16, [3000, 2000, 4100], [1, 17, 9])]
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hq,hkv,d,pt,lens,rows", LONG)
+def test_long_sequences(hq, hkv, d, pt, lens, rows, dtype, kind):
+    """Sequences in pieces, and workgroups that cross from one to the next; the bounds a captured call would have."""
+    rng = np.random.default_rng(len(lens) + d)
+    cache, model, table = random_cache(rng, lens, hkv, d, pt, kind)
+    got = check_attention(cache, model, table, lens, rows, hq, dtype, rng, max_rows=max(rows))
+    rng = np.random.default_rng(len(lens) + d + 1)
+    again = check_attention(cache, model, table, lens, rows, hq, dtype, rng)
+    assert got.shape == again.shape
+
+
+def test_the_same_call_gives_the_same_bits():
+    rng = np.random.default_rng(3)
+    lens = [4000, 100, 900, 2000]
+    cache, model, table = random_cache(rng, lens, 4, 128, 16, "int8")
+    q = dev(rounded(rng, (40, 16, 128), BF16), BF16)
+    starts = dev([0, 1, 2, 30, 40], torch.int32)
+    want = qk.quantized_attention(cache, q, starts)
+    for _ in range(5):
+        assert torch.equal(qk.quantized_attention(cache, q, starts), want)
 
 
 def test_rows_past_max_rows_stay():

@@ -18,9 +18,11 @@ struct Kv8Args {
     int batch, tokens, max_rows, q_heads, kv_heads, dim, pt, per, pages, max_context;
     float scale;
     // the matrix-core kernels'
-    int group, slots, share, fixed, least, few, width;  // (as in Kv8Plan)
+    int group, slots, share, quads, fixed, least, few, width;  // (as in Kv8Plan)
     int vec, out_vec;                                      // rows begin on 16-byte boundaries
     int4* slot_of; int* sequence_of; float2* part_ml; float* part_acc;
+    // A column's row (single rows without the division).
+    __device__ __forceinline__ int row_of(int col) const { return col < group ? 0 : col / group; }
     // Rows [t0, t0 + rows) of a sequence and its tokens.
     __device__ __forceinline__ void sequence(int b, int& t0, int& rows, int& len) const {
         t0 = b * max_rows;
@@ -43,7 +45,8 @@ __device__ __forceinline__ void kv8_store(void* p, int f32, int64_t i, float v) 
 }
 // Four values of a row over their sum of weights (nothing seen: 0 / 0).
 __device__ __forceinline__ void kv8_store4(const Kv8Args& a, int64_t i, const float4& v, float sum) {
-    const float4 y = make_float4(v.x / sum, v.y / sum, v.z / sum, v.w / sum);
+    const float inv = 1.0f / sum;  // (0 times its infinity is NaN)
+    const float4 y = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
     if (!a.out_vec) {
         kv8_store(a.out, a.out_f32, i, y.x);
         kv8_store(a.out, a.out_f32, i + 1, y.y);
@@ -191,8 +194,11 @@ __device__ __forceinline__ void load_unit(const Kv8Args& a, int b, Unit& u) {
 // pieces 117; four of up to 2001 with 5 fp32 rows: 20 and 14.
 struct Shares {
     int all, groups, each, fixed;
+    bool quads;  // a workgroup's waves take four kv heads, not a fourth of the tiles each
     __device__ Shares(const Kv8Args& a, int n) : all(n), groups(a.share), each(0), fixed(a.fixed) {
-        if (fixed || n <= a.share * a.few) each = max(ceil_div(n, max(a.share, 1)), a.least);
+        quads = !fixed && a.quads && static_cast<int64_t>(n) * a.kv_heads >= a.quads;
+        if (quads) groups *= 4;
+        if (fixed || n <= groups * a.few) each = max(ceil_div(n, max(groups, 1)), a.least);
     }
     __device__ int pieces(int tiles) const { return ceil_div(tiles, fixed ? ceil_div(tiles, fixed) : each); }
     __device__ int begin(int w) const { return static_cast<int>(static_cast<int64_t>(all) * w / groups); }
@@ -291,7 +297,7 @@ __device__ __forceinline__ void weight_terms(float p0, float p1, uint32_t* t) {
 }  // namespace
 
 template <bool FP8, int D, int QT, int PT, int NT, bool P16, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : QT == 3 || NT == 2 ? (D == 64 ? 3 : 2) : D == 64 ? 4 : 3) void attn_kv8_kernel(Kv8Args a) {
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NT == 2 ? 2 : QT == 3 ? (D == 64 ? 3 : 2) : D == 64 ? 4 : 3) void attn_kv8_kernel(Kv8Args a) {
     static_assert(D == 64 || D == 128, "16 bytes of 4 lanes make a k-step");
     constexpr int kF = D / 32, kDt = D / 16, kLd = D + 4, kCols = 16 * NT;
     // a wave's queries as operands, which the loop reads again for each tile; then its sums
@@ -303,7 +309,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : QT == 3 || NT == 2 ? (
     __shared__ float sm[WAVES][kCols], sl[WAVES][kCols];
     const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int group = blockIdx.x / a.kv_heads, kvh = blockIdx.x - group * a.kv_heads;
     const float scale = a.scale * kLog2e;
     const int pt = P16 ? 16 : a.pt, runs = pt >> 4;  // 16-token runs of a page
 
@@ -320,6 +325,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : QT == 3 || NT == 2 ? (
     }
     Shares how(a, all);
     same(how.each);
+    const bool quads = WAVES == 4 && NT == 1 && how.quads;
+    const int across = quads ? a.kv_heads >> 2 : a.kv_heads, group = blockIdx.x / across;
+    const int kvh = quads ? 4 * (blockIdx.x - group * across) + wave : blockIdx.x - group * across;
     int tile0, left;
     if (how.each) {
         if (!find_unit<kCols>(a, how, first, group, u, tile0)) return;
@@ -338,12 +346,12 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : QT == 3 || NT == 2 ? (
         same(left);
         const int count = min(left, u.tiles - tile0);
         const int cols = min(u.rows, a.max_rows) * a.group;
-        const int groups = groups_of(cols, kCols), ways = WAVES / groups, col0 = u.block * groups * kCols;
+        const int groups = quads ? 1 : groups_of(cols, kCols), ways = quads ? 1 : WAVES / groups, col0 = u.block * groups * kCols;
         const int wcol = col0 + wave % groups * kCols;  // (may lie behind the columns)
         // tokens that all of the wave's columns see, and that any does
-        const int seen_all = max(u.len - u.rows + wcol / a.group + 1, 0);
-        const int seen_any = wcol < cols ? max(u.len - u.rows + min(wcol + kCols - 1, cols - 1) / a.group + 1, 0) : 0;
-        const int span = max(min(tile0 + count, ceil_div(seen_any, kTile)) - tile0, 0), way = wave / groups;
+        const int seen_all = max(u.len - u.rows + a.row_of(wcol) + 1, 0);
+        const int seen_any = wcol < cols ? max(u.len - u.rows + a.row_of(min(wcol + kCols - 1, cols - 1)) + 1, 0) : 0;
+        const int span = max(min(tile0 + count, ceil_div(seen_any, kTile)) - tile0, 0), way = quads ? 0 : wave / groups;
         const int begin = tile0 + static_cast<int>(static_cast<int64_t>(span) * way / ways);
         const int end = tile0 + static_cast<int>(static_cast<int64_t>(span) * (way + 1) / ways);
         const int32_t* table = a.page_table + static_cast<int64_t>(u.b) * a.per;
@@ -362,10 +370,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : QT == 3 || NT == 2 ? (
         int seen[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int c = wcol + 16 * n + lr, i = c / a.group;
+            const int c = wcol + 16 * n + lr;
             const bool live = c < cols;
+            const int i = live ? a.row_of(c) : 0;
             seen[n] = live ? max(u.len - u.rows + i + 1, 0) : 0;
-            const int64_t row = static_cast<int64_t>(u.t0 + (live ? i : 0)) * a.q_stride + static_cast<int64_t>(kvh * a.group + (live ? c - i * a.group : 0)) * D + 16 * lg;
+            const int64_t row = static_cast<int64_t>(u.t0 + i) * a.q_stride + static_cast<int64_t>(kvh * a.group + (live ? c - i * a.group : 0)) * D + 16 * lg;
 #pragma unroll
             for (int f = 0; f < kF; ++f) {
                 const int64_t at = row + 64 * (f >> 1) + 8 * (f & 1);
@@ -527,21 +536,20 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : QT == 3 || NT == 2 ? (
                 }
             }
         }
-        // the waves of a column group, joined in LDS
+        // the waves of a column group, joined in LDS (of four heads: each one alone, laid out for its stores)
+        const int step = quads ? WAVES : groups;  // from one wave of a group to the next
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             l[n] = xor32_sum(xor16_sum(l[n]));
-            if (lg == 0) {
-                sm[wave][16 * n + lr] = m[n];
-                sl[wave][16 * n + lr] = l[n];
-            }
+            if (lg == 0) sm[wave][16 * n + lr] = m[n];
         }
         __syncthreads();
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             float top = -INFINITY;
-            for (int w = wave % groups; w < WAVES; w += groups) top = fmaxf(top, sm[w][16 * n + lr]);
+            for (int w = wave % step; w < WAVES; w += step) top = fmaxf(top, sm[w][16 * n + lr]);
             const float f = m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[n] - top);
+            if (lg == 0) sl[wave][16 * n + lr] = l[n] * f;
 #pragma unroll
             for (int d = 0; d < kDt; ++d) {
                 const float4 v = make_float4(o[n][d][0] * f, o[n][d][1] * f, o[n][d][2] * f, o[n][d][3] * f);
@@ -551,19 +559,20 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : QT == 3 || NT == 2 ? (
         __syncthreads();
         const bool whole = count == u.tiles;
         const int64_t part = (static_cast<int64_t>(how.each ? group : group + u.ord) * a.kv_heads + kvh) * a.width;
-        for (int e = threadIdx.x; e < groups * kCols * (D / 4); e += 64 * WAVES) {
-            const int c = e / (D / 4), d = e % (D / 4) * 4, gr = c / kCols, cc = c % kCols;
+        const int begin_e = quads ? lane : threadIdx.x, step_e = quads ? kWave : 64 * WAVES;
+        for (int e = begin_e; e < groups * kCols * (D / 4); e += step_e) {
+            const int c = e / (D / 4), d = e % (D / 4) * 4, gr = quads ? wave : c / kCols, cc = c % kCols;
             const int col = col0 + c;
             if (col >= cols) break;
             float top = -INFINITY, sum = 0.f;
-            for (int w = gr; w < WAVES; w += groups) top = fmaxf(top, sm[w][cc]);
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int w = gr; w < WAVES; w += groups) {
-                sum += sl[w][cc] * (sm[w][cc] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[w][cc] - top));
+            for (int w = gr; w < WAVES; w += step) {
+                top = fmaxf(top, sm[w][cc]);
+                sum += sl[w][cc];
                 const float4 x = *reinterpret_cast<const float4*>(&sw[w].o[cc][d]);
                 v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
             }
-            const int i = col / a.group;
+            const int i = a.row_of(col);
             if (whole) {
                 kv8_store4(a, static_cast<int64_t>(u.t0 + i) * a.out_stride + static_cast<int64_t>(kvh * a.group + col - i * a.group) * D + d, v, sum);
             } else {
@@ -574,8 +583,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : QT == 3 || NT == 2 ? (
         // where the join finds a row's sequence, and the sequence's pieces or tiles among all
         if (a.slot_of && tile0 == 0 && kvh == 0) {
             if (u.block == 0 && threadIdx.x == 0) a.slot_of[u.b] = make_int4(u.before, how.each ? how.pieces(u.tiles) : u.ord, u.tiles, how.each ? 0 : all);
-            for (int e = threadIdx.x; e < groups * kCols; e += 64 * WAVES)
-                if (col0 + e < cols) a.sequence_of[u.t0 + (col0 + e) / a.group] = u.b;
+            for (int e = begin_e; e < groups * kCols; e += step_e)
+                if (col0 + e < cols) a.sequence_of[u.t0 + a.row_of(col0 + e)] = u.b;
         }
         if ((left -= count) <= 0) return;
         next_unit<kCols>(a, u);
@@ -673,14 +682,14 @@ constexpr int64_t kMaxTiles = 1 << 30;
 // dealt 33; 16 fp32 rows over up to 8192 47, pieces from 24 tiles down 53).
 constexpr int64_t kRound = 512;
 constexpr int kFew = 16;
-#ifndef MANYR
-#define MANYR 4096
+#ifndef QUADS
+#define QUADS 8192
 #endif
-#ifndef SHORTT
-#define SHORTT 16
-#endif
-constexpr int64_t kManyRows = MANYR;  // rows by heads from which a join's lanes have one each
-constexpr int64_t kShort = SHORTT;    // tiles up to which eight waves take a unit whole
+constexpr int kQuads = QUADS;
+constexpr int64_t kManyRows = 4096;  // rows by heads from which a join's lanes have one each
+// Tiles up to which eight waves take a unit whole, a tile each, if every one of them has a compute
+// unit: one sequence of 500 tokens 10.2 us for 11.6, 32 of up to 500 12.2 for 15.5; 64 22.7 for 21.3.
+constexpr int64_t kShort = 8;
 
 }  // namespace
 
@@ -700,18 +709,22 @@ Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a) {
     p.few = kFew;
     p.fixed = static_cast<int>(std::min<int64_t>({std::max(a.kv_splits, 0), tiles, kMostSlots / (blocks * a.kv_heads)}));
     p.waves = 4;
-    if (!p.fixed && narrow && p.nt == 1 && tiles <= kShort && tiles > p.least) {
+    if (!p.fixed && narrow && p.nt == 1 && tiles <= kShort && tiles > p.least && blocks * a.kv_heads <= 256) {
         p.waves = 8;
         p.fixed = 1;
     }
     if (!p.fixed && tiles > p.least) {
         p.share = static_cast<int>(std::max<int64_t>(kRound / a.kv_heads, 1));
-        p.slots = static_cast<int>(std::min(p.share + blocks, blocks * ((tiles + p.least - 1) / p.least)));
+        p.quads = narrow && p.nt == 1 && a.kv_heads % 4 == 0 && 4 * a.batch >= p.share ? kQuads : 0;
+        const int64_t most = blocks * ((tiles + p.least - 1) / p.least);  // the shortest pieces
+        p.slots = static_cast<int>(std::min(p.share * (p.quads ? 4 : 1) + blocks, most));
+        p.groups = static_cast<int>(std::min(p.share + blocks, most) * a.kv_heads);
         if (kv8_bytes(a, p.slots, p.width) > (size_t{128} << 20)) p.share = 0;
     }
     if (!p.share) {
         p.fixed = std::max(p.fixed, 1);
         p.slots = static_cast<int>(blocks * p.fixed);
+        p.groups = static_cast<int>(p.slots * a.kv_heads);
     }
     if (p.fixed != 1) p.bytes = kv8_bytes(a, p.slots, p.width);
     return p;
@@ -730,7 +743,7 @@ void launch_kv8_join(const Kv8Args& a, hipStream_t stream) {
 
 template <bool FP8, int D, bool P16>
 void launch_kv8_mfma(const Kv8Args& a, const Kv8Plan& p, bool narrow, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(p.slots * a.kv_heads));
+    const dim3 grid(static_cast<unsigned>(p.groups));
     if (!narrow) attn_kv8_kernel<FP8, D, 3, 3, 1, P16, 4><<<grid, 256, 0, stream>>>(a);
     else if (p.nt == 2) attn_kv8_kernel<FP8, D, 1, 2, 2, P16, 4><<<grid, 256, 0, stream>>>(a);
     else if (p.waves == 8) attn_kv8_kernel<FP8, D, 1, 2, 1, P16, 8><<<grid, 512, 0, stream>>>(a);
@@ -765,7 +778,7 @@ void launch_attn_kv8(const sfg_kv8_attn_args& s, const Kv8Plan& plan, void* work
                          (reinterpret_cast<uintptr_t>(s.scales) & 7) == 0;
     if (plan.mfma && aligned) {
         a.group = a.q_heads / a.kv_heads;
-        a.slots = plan.slots; a.share = plan.share; a.fixed = plan.fixed; a.least = plan.least; a.few = plan.few;
+        a.slots = plan.slots; a.share = plan.share; a.fixed = plan.fixed; a.least = plan.least; a.few = plan.few; a.quads = plan.quads;
         a.width = plan.width;
         a.vec = (reinterpret_cast<uintptr_t>(s.q) & 15) == 0 && s.q_stride % 8 == 0;
         a.out_vec = (reinterpret_cast<uintptr_t>(s.out) & 15) == 0 && s.out_stride % 4 == 0;

@@ -44,11 +44,13 @@ void launch_kv8_append(const sfg_kv8_append_args& a, hipStream_t stream);
 // How an attention runs.  A unit is a block of at most `width` columns of a sequence over all
 // its tiles.  share: the workgroups a kv head that all tiles are dealt to if there are more than
 // `few` for each; with fewer, units are split into pieces of `least` tiles or more, at most
-// share and the units together.  fixed: pieces a unit, instead of both.  slots: workgroups a kv
-// head, and partial results.  bytes: 0 if no unit is split.
+// share and the units together.  quads (0: never): with so many tiles of all heads, a workgroup
+// takes four heads, and there are four times as many shares.  fixed: pieces a unit, instead of
+// all that.  slots: partial results a kv head, at most; groups: workgroups.  bytes: 0 if no unit
+// is split.
 struct Kv8Plan {
     bool mfma;
-    int nt, waves, width, slots, share, fixed, least, few;
+    int nt, waves, width, slots, groups, share, quads, fixed, least, few;
     size_t bytes;
 };
 Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a);

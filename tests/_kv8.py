@@ -155,27 +155,35 @@ def attend64(q, k, v, length, scale, wide):
     """Newest rows q [R][Hq][D] (float64) over k, v [Hkv][L][D] (float64): out and how far fp32 arithmetic may be off,
     before the output's own rounding.  wide: softmax weights of 24 bits instead of 16."""
     rows, hq, d = q.shape
-    group = hq // k.shape[0]
+    heads, group = k.shape[0], hq // k.shape[0]
     out, off = np.full(q.shape, np.nan), np.full(q.shape, np.nan)
     u = 2.0 ** -24
-    for i in range(rows):
-        end = length - rows + i + 1
-        if end <= 0:
-            continue
-        for h in range(hq):
-            kk, vv = k[h // group, :end], v[h // group, :end]
-            with np.errstate(all="ignore"):
-                x = kk @ q[i, h] * scale
-                m = x.max()
-                p = np.exp(x - m)
-                p /= p.sum()
-                out[i, h] = p @ vv
-                # sums over 3 D terms, each product exact; three products with scales and log2 e; the difference from
-                # the largest score; exp2 to 2 ulp
-                e = (3 * d + 8) * u * (np.abs(kk) @ np.abs(q[i, h])) * scale + 4 * u * np.abs(x)
-                e = e + e.max() + u * np.abs(x - m) * 2 + 4 * u
-                weight = (4 * u if wide else 2.0 ** -15) + (end + 16) * u
-                off[i, h] = (p * e) @ np.abs(vv) + (p @ np.abs(vv)) * weight + np.abs(out[i, h]) * (p @ e + (end + 16) * u)
+    end = np.repeat(length - rows + 1 + np.arange(rows), group)          # tokens that a column sees
+    live = end > 0
+    if not live.any():
+        return out, off
+    hidden = np.arange(length)[None] >= end[live][:, None]
+    for h in range(heads):
+        qq = q[:, h * group: (h + 1) * group].reshape(rows * group, d)[live]
+        with np.errstate(all="ignore"):
+            x = np.where(hidden, -np.inf, qq @ k[h].T * scale)
+            m = x.max(1, keepdims=True)
+            p = np.exp(x - m)
+            p /= p.sum(1, keepdims=True)
+            o = p @ v[h]
+            # sums over 3 D terms, each product exact; three products with scales and log2 e; the difference from
+            # the largest score; exp2 to 2 ulp
+            seen = np.where(hidden, 0.0, x)
+            e = (3 * d + 8) * u * (np.abs(qq) @ np.abs(k[h]).T) * scale + 4 * u * np.abs(seen)
+            e = np.where(hidden, 0.0, e)
+            e = e + e.max(1, keepdims=True) + u * np.abs(seen - m) * 2 + 4 * u
+            sums = (end[live][:, None] + 16) * u
+            weight = (4 * u if wide else 2.0 ** -15) + sums
+            bound = (p * e) @ np.abs(v[h]) + (p @ np.abs(v[h])) * weight + np.abs(o) * ((p * e).sum(1, keepdims=True) + sums + u)
+        for target, value in ((out, o), (off, bound)):
+            full = np.full((rows * group, d), np.nan)
+            full[live] = value
+            target[:, h * group: (h + 1) * group] = full.reshape(rows, group, d)
     return out, off
 
 

@@ -17,8 +17,9 @@ struct Kv8Args {
     const int32_t* page_table; const int32_t* seq_lens; const int32_t* starts;
     int batch, tokens, max_rows, q_heads, kv_heads, dim, pt, per, pages, max_context;
     float scale;
-    // the matrix-core kernels'
-    int group, slots, share, quads, fixed, least, few, width;  // (as in Kv8Plan)
+    int group;
+    // the matrix-core kernels' (the rows kernel: fixed)
+    int slots, share, quads, fixed, least, few, width;  // (as in Kv8Plan)
     int vec, out_vec;                                      // rows begin on 16-byte boundaries
     int4* slot_of; int* sequence_of; float2* part_ml; float* part_acc;
     // A column's row (single rows without the division).
@@ -61,12 +62,14 @@ __device__ __forceinline__ void kv8_store4(const Kv8Args& a, int64_t i, const fl
 
 }  // namespace
 
-// Any head dim up to kRowMaxD and any page size: a wave a row and query head, 64 tokens at a
-// time with a token a lane for the scores and a dim a lane for the values.
-template <bool FP8>
+// Any head dim up to kRowMaxD and any page size: a wave a row, query head and split of its
+// tokens, 64 of those at a time with a token a lane for the scores and a dim a lane for the
+// values.  WORDS: head dim and page are multiples of 4, codes are read four at a time.  16 sequences
+// of up to 4096 tokens, 32 heads of 80 over 8: 197 us (without splits and words 1220).
+template <bool FP8, bool WORDS>
 __global__ __launch_bounds__(64) void attn_kv8_rows_kernel(Kv8Args a) {
     __shared__ float sq[kRowMaxD];
-    const int lane = threadIdx.x, t = blockIdx.x, h = blockIdx.y;
+    const int lane = threadIdx.x, t = blockIdx.x, h = blockIdx.y, split = blockIdx.z;
     int b = t / a.max_rows;
     if (a.starts) {
         int hi = a.batch;
@@ -81,15 +84,17 @@ __global__ __launch_bounds__(64) void attn_kv8_rows_kernel(Kv8Args a) {
     a.sequence(b, t0, rows, len);
     const int i = t - t0;
     if (i < 0 || i >= rows || i >= a.max_rows) return;
-    const int D = a.dim, kvh = h / (a.q_heads / a.kv_heads);
-    const int end = min(max(len - rows + i + 1, 0), len);
+    const int D = a.dim, kvh = h / a.group;
+    const int seen = min(max(len - rows + i + 1, 0), len), chunks = (seen + 63) / 64;
+    const int begin = static_cast<int>(static_cast<int64_t>(chunks) * split / a.fixed) * 64;
+    const int end = min(static_cast<int>(static_cast<int64_t>(chunks) * (split + 1) / a.fixed) * 64, seen);
     for (int d = lane; d < D; d += 64) sq[d] = kv8_load(a.q, a.q_f32, t * a.q_stride + static_cast<int64_t>(h) * D + d);
     __syncthreads();
     const int32_t* table = a.page_table + static_cast<int64_t>(b) * a.per;
     float m = -INFINITY, l = 0.f;
     float acc[kRowMaxD / 64] = {};
-    for (int base = 0; base < end; base += 64) {
-        const int j = base + lane;
+    for (int base = begin; base < end; base += 64) {
+        const int j = base + lane, count = min(64, end - base);
         float s = -INFINITY, sv = 0.f;
         int page = -1;
         if (j < end) {
@@ -99,7 +104,16 @@ __global__ __launch_bounds__(64) void attn_kv8_rows_kernel(Kv8Args a) {
                 const int64_t unit = static_cast<int64_t>(id) * a.kv_heads + kvh;
                 const uint8_t* k = a.k_pool + (unit * a.pt + j % a.pt) * D;
                 float dot = 0.f;
-                for (int d = 0; d < D; ++d) dot = fmaf(sq[d], kv8_value<FP8>(k[d]), dot);
+                if constexpr (WORDS) {
+#pragma unroll 4
+                    for (int d = 0; d < D; d += 4) {
+                        const uint32_t w = *reinterpret_cast<const uint32_t*>(k + d);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) dot = fmaf(sq[d + e], kv8_value<FP8>(static_cast<uint8_t>(w >> (8 * e))), dot);
+                    }
+                } else {
+                    for (int d = 0; d < D; ++d) dot = fmaf(sq[d], kv8_value<FP8>(k[d]), dot);
+                }
                 s = dot * (a.scales[2 * unit] * a.scale);
                 sv = a.scales[2 * unit + 1];
             }
@@ -113,24 +127,70 @@ __global__ __launch_bounds__(64) void attn_kv8_rows_kernel(Kv8Args a) {
 #pragma unroll
         for (int r = 0; r < kRowMaxD / 64; ++r) acc[r] *= alpha;
         const float w = page >= 0 ? p * sv : 0.f;
-        for (int c = 0; c < min(64, end - base); ++c) {
-            const int pg = lane_bcast(page, c);
-            const float wc = lane_bcast(w, c);
-            if (pg < 0) continue;  // wave-uniform
+        constexpr int kStep = WORDS ? 4 : 1;
+        for (int c = 0; c < count; c += kStep) {
+            const int pg = lane_bcast(page, c);  // (of all kStep tokens)
+            if (pg < 0) continue;                // wave-uniform
             const uint8_t* v = a.v_pool + (static_cast<int64_t>(pg) * a.kv_heads + kvh) * D * a.pt + (base + c) % a.pt;
 #pragma unroll
             for (int r = 0; r < kRowMaxD / 64; ++r) {
                 const int d = lane + 64 * r;
-                if (d < D) acc[r] = fmaf(wc, kv8_value<FP8>(v[static_cast<int64_t>(d) * a.pt]), acc[r]);
+                if (d >= D) continue;
+                if constexpr (WORDS) {
+                    const uint32_t x = *reinterpret_cast<const uint32_t*>(v + static_cast<int64_t>(d) * a.pt);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c + e < count) acc[r] = fmaf(lane_bcast(w, c + e), kv8_value<FP8>(static_cast<uint8_t>(x >> (8 * e))), acc[r]);
+                } else {
+                    acc[r] = fmaf(lane_bcast(w, c), kv8_value<FP8>(v[static_cast<int64_t>(d) * a.pt]), acc[r]);
+                }
             }
         }
         m = m_new;
     }
+    const int64_t part = (static_cast<int64_t>(t) * a.q_heads + h) * a.fixed + split;
+    if (a.part_ml && lane == 0) a.part_ml[part] = make_float2(m, l);
 #pragma unroll
     for (int r = 0; r < kRowMaxD / 64; ++r) {
         const int d = lane + 64 * r;
-        if (d < D) kv8_store(a.out, a.out_f32, t * a.out_stride + static_cast<int64_t>(h) * D + d, acc[r] / l);  // (nothing seen: 0 / 0)
+        if (d >= D) continue;
+        if (a.part_ml) a.part_acc[part * D + d] = acc[r];
+        else kv8_store(a.out, a.out_f32, t * a.out_stride + static_cast<int64_t>(h) * D + d, acc[r] / l);  // (nothing seen: 0 / 0)
     }
+    if (a.part_ml && h == 0 && split == 0 && lane == 0) a.sequence_of[t] = 1;  // (a row that is computed)
+}
+
+// The splits of a row and query head.
+__global__ __launch_bounds__(64) void attn_kv8_rows_join_kernel(Kv8Args a) {
+    const int lane = threadIdx.x, t = blockIdx.x, h = blockIdx.y, D = a.dim;
+    if (a.sequence_of[t] == 0) return;
+    const int64_t part = (static_cast<int64_t>(t) * a.q_heads + h) * a.fixed;
+    float top = -INFINITY;
+    bool nan = false;
+    for (int s = 0; s < a.fixed; ++s) {
+        top = fmaxf(top, a.part_ml[part + s].x);
+        nan |= a.part_ml[part + s].x != a.part_ml[part + s].x;
+    }
+    float sum = nan ? __uint_as_float(0x7FC00000u) : 0.f;
+    float acc[kRowMaxD / 64] = {};
+#pragma unroll 4
+    for (int s = 0; s < a.fixed; ++s) {
+        const float2 ml = a.part_ml[part + s];
+        const float f = ml.x == -INFINITY ? 0.f : expf(ml.x - top);
+        sum = fmaf(ml.y, f, sum);
+#pragma unroll
+        for (int r = 0; r < kRowMaxD / 64; ++r)
+            if (lane + 64 * r < D) acc[r] = fmaf(a.part_acc[(part + s) * D + lane + 64 * r], f, acc[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < kRowMaxD / 64; ++r)
+        if (lane + 64 * r < D) kv8_store(a.out, a.out_f32, t * a.out_stride + static_cast<int64_t>(h) * D + lane + 64 * r, acc[r] / sum);
+}
+
+// Which rows a call computes (the join's others stay as they were).
+__global__ __launch_bounds__(256) void attn_kv8_rows_begin_kernel(int* computed, int tokens) {
+    const int t = blockIdx.x * 256 + threadIdx.x;
+    if (t < tokens) computed[t] = 0;
 }
 
 // ===========================================================================
@@ -597,7 +657,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NT == 2 ? 2 : QT == 3 ? (
 // The splits of a row and query head: weights 2^(m_s - M), sums in a fixed order.  D / 4 lanes to a
 // split.  TOGETHER: all of a workgroup's for one row and head, so many splits at a time; else
 // each D / 4 lanes for one of their own, which pays where there are many rows (519 of 32 heads,
-// about 5 splits: .. us, 30 together) and not where there are few (2 of 32 heads, 90 splits: 45 one
+// about 5 splits: 9 us, 30 together) and not where there are few (2 of 32 heads, 90 splits: 45 one
 // after the other, 5 together).
 template <int D, int WIDTH, bool TOGETHER>
 __global__ __launch_bounds__(256) void attn_kv8_join_kernel(Kv8Args a) {
@@ -674,6 +734,11 @@ size_t kv8_bytes(const sfg_kv8_attn_args& a, int64_t slots, int width) {
     return up256(a.batch * sizeof(int4)) + up256(a.tokens * sizeof(int)) + up256(columns * sizeof(float2)) + up256(columns * a.head_dim * sizeof(float));
 }
 
+size_t rows_bytes(const sfg_kv8_attn_args& a, int64_t splits) {
+    const size_t parts = static_cast<size_t>(a.tokens) * a.q_heads * splits;
+    return up256(a.tokens * sizeof(int)) + up256(parts * sizeof(float2)) + up256(parts * a.head_dim * sizeof(float));
+}
+
 constexpr int64_t kMostSlots = 1 << 22;  // workgroups of a launch: 256 threads each
 constexpr int64_t kMaxTiles = 1 << 30;
 // Workgroups that tiles are dealt to: two a compute unit, all of them resident at once.  (768, where
@@ -693,17 +758,31 @@ constexpr int64_t kShort = 8;
 
 }  // namespace
 
-Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a) {
+// The rows kernel: splits of 128 tokens or more until there are 2048 waves.
+Kv8Plan plan_rows(const sfg_kv8_attn_args& a) {
     Kv8Plan p{};
-    if ((a.head_dim != 64 && a.head_dim != 128) || a.page_tokens % 16) return p;
+    const int64_t waves = a.tokens * a.q_heads, chunks = std::max<int64_t>((a.max_context + 63) / 64, 1);
+    int64_t splits = 1;
+    if (a.kv_splits > 0) splits = std::min<int64_t>({a.kv_splits, chunks, 65535});
+    else
+        while (waves * splits < 2048 && chunks / (2 * splits) >= 2) splits *= 2;
+    // (a launch's threads and the workspace stay within bounds)
+    while (splits > 1 && (waves * splits > (1 << 25) || rows_bytes(a, splits) > (size_t{128} << 20))) splits /= 2;
+    p.fixed = static_cast<int>(splits);
+    p.bytes = splits > 1 ? rows_bytes(a, splits) : 0;
+    return p;
+}
+
+Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a) {
+    if ((a.head_dim != 64 && a.head_dim != 128) || a.page_tokens % 16) return plan_rows(a);
+    Kv8Plan p{};
     const bool narrow = a.q_dtype == SFG_BF16 && a.out_dtype == SFG_BF16;
     const int64_t group = a.q_heads / a.kv_heads, cols = a.max_rows * group;
     const int64_t tiles = std::max<int64_t>((a.max_context + kTile - 1) / kTile, 1);
     p.nt = narrow && cols > 16 ? 2 : 1;
     p.width = 16 * p.nt * (cols > 32 * p.nt ? 4 : cols > 16 * p.nt ? 2 : 1);
     const int64_t blocks = a.tokens * group / (64 * p.nt) + a.batch;  // of all sequences, at most
-    if (blocks * a.kv_heads > kMostSlots) return p;
-    if (blocks * tiles > kMaxTiles) return p;
+    if (blocks * a.kv_heads > kMostSlots || blocks * tiles > kMaxTiles) return plan_rows(a);
     p.mfma = true;
     p.least = 4;  // (a tile a wave)
     p.few = kFew;
@@ -776,9 +855,10 @@ void launch_attn_kv8(const sfg_kv8_attn_args& s, const Kv8Plan& plan, void* work
     // codes are read 16 bytes at a time, scales in pairs
     const bool aligned = ((reinterpret_cast<uintptr_t>(s.k_pool) | reinterpret_cast<uintptr_t>(s.v_pool)) & 15) == 0 &&
                          (reinterpret_cast<uintptr_t>(s.scales) & 7) == 0;
+    a.group = a.q_heads / a.kv_heads;
+    a.fixed = plan.fixed;
     if (plan.mfma && aligned) {
-        a.group = a.q_heads / a.kv_heads;
-        a.slots = plan.slots; a.share = plan.share; a.fixed = plan.fixed; a.least = plan.least; a.few = plan.few; a.quads = plan.quads;
+        a.slots = plan.slots; a.share = plan.share; a.least = plan.least; a.few = plan.few; a.quads = plan.quads;
         a.width = plan.width;
         a.vec = (reinterpret_cast<uintptr_t>(s.q) & 15) == 0 && s.q_stride % 8 == 0;
         a.out_vec = (reinterpret_cast<uintptr_t>(s.out) & 15) == 0 && s.out_stride % 4 == 0;
@@ -799,9 +879,26 @@ void launch_attn_kv8(const sfg_kv8_attn_args& s, const Kv8Plan& plan, void* work
         }
         return;
     }
-    const dim3 grid(static_cast<unsigned>(a.tokens), static_cast<unsigned>(a.q_heads));
-    if (s.pool_dtype == SFG_FP8) attn_kv8_rows_kernel<true><<<grid, 64, 0, stream>>>(a);
-    else attn_kv8_rows_kernel<false><<<grid, 64, 0, stream>>>(a);
+    // (pools off their boundaries: whole, in the plan's place)
+    if (plan.mfma) a.fixed = 1;
+    if (a.fixed > 1) {
+        const size_t parts = static_cast<size_t>(a.tokens) * a.q_heads * a.fixed;
+        char* at = static_cast<char*>(workspace);
+        a.sequence_of = reinterpret_cast<int*>(at); at += up256(a.tokens * sizeof(int));
+        a.part_ml = reinterpret_cast<float2*>(at); at += up256(parts * sizeof(float2));
+        a.part_acc = reinterpret_cast<float*>(at);
+        attn_kv8_rows_begin_kernel<<<dim3(static_cast<unsigned>((a.tokens + 255) / 256)), 256, 0, stream>>>(a.sequence_of, a.tokens);
+    }
+    const dim3 grid(static_cast<unsigned>(a.tokens), static_cast<unsigned>(a.q_heads), static_cast<unsigned>(a.fixed));
+    const bool words = a.dim % 4 == 0 && a.pt % 4 == 0 && ((reinterpret_cast<uintptr_t>(s.k_pool) | reinterpret_cast<uintptr_t>(s.v_pool)) & 3) == 0;
+    if (s.pool_dtype == SFG_FP8) {
+        if (words) attn_kv8_rows_kernel<true, true><<<grid, 64, 0, stream>>>(a);
+        else attn_kv8_rows_kernel<true, false><<<grid, 64, 0, stream>>>(a);
+    } else {
+        if (words) attn_kv8_rows_kernel<false, true><<<grid, 64, 0, stream>>>(a);
+        else attn_kv8_rows_kernel<false, false><<<grid, 64, 0, stream>>>(a);
+    }
+    if (a.fixed > 1) attn_kv8_rows_join_kernel<<<dim3(static_cast<unsigned>(a.tokens), static_cast<unsigned>(a.q_heads)), 64, 0, stream>>>(a);
 }
 
 }  // namespace sfg

@@ -237,6 +237,13 @@ struct Unit {
     int ord;      // units before it
     int before;   // tiles of the sequences before (where tiles are dealt), else their splits
 };
+// A sequence's tiles or pieces, for all its blocks.  Starts and lengths that a caller left in
+// disorder may give any product: what the host has checked never reaches the cuts, and with them
+// 64 of these and the sum before them fit 32 bits.
+constexpr int kMaxTiles = 1 << 23, kMaxAll = 1 << 29;
+__device__ __forceinline__ int in_all(int of_block, int blocks) {
+    return static_cast<int>(min(static_cast<int64_t>(of_block) * blocks, static_cast<int64_t>(kMaxTiles)));
+}
 template <int WIDTH>
 __device__ __forceinline__ void load_unit(const Kv8Args& a, int b, Unit& u) {
     u.tiles = u.blocks = u.t0 = u.rows = u.len = 0;
@@ -272,7 +279,7 @@ __device__ __forceinline__ bool find_unit(const Kv8Args& a, const Shares& how, c
     int sum = 0, ord = 0;
     Unit v = first;
     for (int base = 0;;) {
-        const int mine = v.blocks == 0 ? 0 : (how.each ? how.pieces(v.tiles) : v.tiles) * v.blocks;
+        const int mine = v.blocks == 0 ? 0 : in_all(how.each ? how.pieces(v.tiles) : v.tiles, v.blocks);
         const int upto = wave_inclusive(mine) + sum, units = wave_inclusive(v.blocks) + ord;
         const uint64_t behind = __ballot(upto > at);
         if (behind) {
@@ -377,10 +384,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NT == 2 ? 2 : QT == 3 ? (
     load_unit<kCols>(a, lane, first);
     int all = 0;
     if (!a.fixed) {
-        all = __builtin_amdgcn_readlane(wave_inclusive(first.tiles * first.blocks), 63);
+        all = __builtin_amdgcn_readlane(wave_inclusive(in_all(first.tiles, first.blocks)), 63);
         for (int base = kWave; base < a.batch; base += kWave) {
             load_unit<kCols>(a, base + lane, u);
-            all += __builtin_amdgcn_readlane(wave_inclusive(u.tiles * u.blocks), 63);
+            all = min(all + __builtin_amdgcn_readlane(wave_inclusive(in_all(u.tiles, u.blocks)), 63), kMaxAll);
         }
     }
     Shares how(a, all);
@@ -618,7 +625,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NT == 2 ? 2 : QT == 3 ? (
         }
         __syncthreads();
         const bool whole = count == u.tiles;
-        const int64_t part = (static_cast<int64_t>(how.each ? group : group + u.ord) * a.kv_heads + kvh) * a.width;
+        const int slot = how.each ? group : group + u.ord;
+        const int64_t part = (static_cast<int64_t>(slot) * a.kv_heads + kvh) * a.width;
         const int begin_e = quads ? lane : threadIdx.x, step_e = quads ? kWave : 64 * WAVES;
         for (int e = begin_e; e < groups * kCols * (D / 4); e += step_e) {
             const int c = e / (D / 4), d = e % (D / 4) * 4, gr = quads ? wave : c / kCols, cc = c % kCols;
@@ -635,7 +643,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NT == 2 ? 2 : QT == 3 ? (
             const int i = a.row_of(col);
             if (whole) {
                 kv8_store4(a, static_cast<int64_t>(u.t0 + i) * a.out_stride + static_cast<int64_t>(kvh * a.group + col - i * a.group) * D + d, v, sum);
-            } else {
+            } else if (slot < a.slots) {  // (it is, of sequences in order)
                 *reinterpret_cast<float4*>(a.part_acc + (part + c) * D + d) = v;
                 if (d == 0) a.part_ml[part + c] = make_float2(top, sum);
             }
@@ -740,7 +748,6 @@ size_t rows_bytes(const sfg_kv8_attn_args& a, int64_t splits) {
 }
 
 constexpr int64_t kMostSlots = 1 << 22;  // workgroups of a launch: 256 threads each
-constexpr int64_t kMaxTiles = 1 << 30;
 // Workgroups that tiles are dealt to: two a compute unit, all of them resident at once.  (768, where
 // registers allow three: 64 sequences of up to 8192 tokens 108 us for 108, 64 with 8 rows
 // 187 for 159.)  Fewer than 16 tiles for each: pieces (32 sequences of up to 2000 tokens 28 us,
@@ -782,7 +789,7 @@ Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a) {
     p.nt = narrow && cols > 16 ? 2 : 1;
     p.width = 16 * p.nt * (cols > 32 * p.nt ? 4 : cols > 16 * p.nt ? 2 : 1);
     const int64_t blocks = a.tokens * group / (64 * p.nt) + a.batch;  // of all sequences, at most
-    if (blocks * a.kv_heads > kMostSlots || blocks * tiles > kMaxTiles) return plan_rows(a);
+    if (blocks * a.kv_heads > kMostSlots || (cols / (64 * p.nt) + 1) * tiles > kMaxTiles || blocks * tiles > kMaxAll) return plan_rows(a);
     p.mfma = true;
     p.least = 4;  // (a tile a wave)
     p.few = kFew;

@@ -397,6 +397,83 @@ def test_rows_past_max_rows_stay():
     check_attention(cache, model, table, [100, 50], [7, 2], 4, BF16, rng, max_rows=4)
 
 
+@pytest.mark.parametrize("hq,hkv,d,pt", [(8, 2, 128, 16), (4, 2, 64, 32), (4, 2, 40, 16)])
+def test_starts_in_disorder_are_not_followed(hq, hkv, d, pt):
+    """Overlapping, falling and far starts: rows in range are computed for some sequence, others are not touched."""
+    rng = np.random.default_rng(4)
+    lens = [100, 50, 70, 20]
+    cache, model, table = filled(rng, lens, hkv, d, pt, "int8")
+    q = rounded(rng, (6, hq, d), BF16)
+    out = torch.full((6, hq, d), 9.0, dtype=BF16, device="cuda")
+    for splits in (0, 3):
+        qk.quantized_attention(cache, dev(q, BF16), dev([0, 2, 1, 2 ** 31 - 1, -7], torch.int32), out=out, kv_splits=splits)
+        torch.cuda.synchronize()
+        k, v = model.tokens(table[0], 100)
+        want, off = plain.attend64(q[:2].astype(np.float64), k, v, 100, d ** -0.5, False)
+        plain.close(out[:1].double().cpu().numpy(), want[:1], off[:1], 2.0 ** -8)   # row 1 is two sequences'
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (4, 2, 64), (4, 2, 48)])
+def test_rows_and_pools_off_their_borders(hq, hkv, d, dtype):
+    """Queries, outputs, keys, values and pools that begin anywhere; common lengths without a list of them: the C calls
+    that take what the Python layer does not make."""
+    import ctypes
+
+    from schedforge_amd import _abi
+    rng = np.random.default_rng(d)
+    lens, pt, lib = [70, 70], 16, _abi.load()
+    cache, model, table = filled(rng, lens, hkv, d, pt, "int8")
+    dt = _abi.F32 if dtype == F32 else _abi.BF16
+    odd = lambda n, kind: torch.full((n + 7,), 3, dtype=kind, device="cuda")[3:]  # noqa: E731
+    keys, values, q = (rounded(rng, (2, h, d), dtype) for h in (hkv, hkv, hq))
+    slots = np.array([table[b, 69 // pt] * pt + 69 % pt for b in range(2)], np.int64)
+    model.append(keys, values, slots)
+    kp, vp = odd(cache.k_pool.numel(), torch.uint8), odd(cache.k_pool.numel(), torch.uint8)
+    kp[: cache.k_pool.numel()] = cache.k_pool.view(torch.uint8).flatten()
+    vp[: cache.k_pool.numel()] = cache.v_pool.view(torch.uint8).flatten()
+    stride = hq * d + 1
+    rows = {n: odd(2 * stride, dtype) for n in ("k", "v", "q", "out")}
+    for n, x in (("k", keys), ("v", values), ("q", q)):
+        for t in range(2):
+            rows[n][t * stride: t * stride + x[t].size] = dev(x[t].ravel(), dtype)
+    begun = cache.scales.clone()
+    for kpool, vpool in ((cache.k_pool, cache.v_pool), (kp, vp)):
+        cache.scales.copy_(begun)                                     # the scales that these codes were stored under
+        a = _abi.Kv8AppendArgs()
+        a.keys, a.values, a.dtype, a.key_stride, a.value_stride = rows["k"].data_ptr(), rows["v"].data_ptr(), dt, stride, stride
+        a.k_pool, a.v_pool, a.pool_dtype, a.scales = kpool.data_ptr(), vpool.data_ptr(), _abi.I8, cache.scales.data_ptr()
+        at = dev(slots, torch.int64)
+        a.slots, a.tokens, a.kv_heads, a.head_dim, a.page_tokens, a.num_pages = at.data_ptr(), 2, hkv, d, pt, cache.num_pages
+        _abi.check(lib.sfg_hip_kv8_append_v1(ctypes.byref(a), None))
+        a = _abi.Kv8AttnArgs()
+        a.q, a.q_dtype, a.q_stride, a.out, a.out_dtype, a.out_stride = rows["q"].data_ptr(), dt, stride, rows["out"].data_ptr(), dt, stride
+        a.k_pool, a.v_pool, a.pool_dtype, a.scales = kpool.data_ptr(), vpool.data_ptr(), _abi.I8, cache.scales.data_ptr()
+        a.page_table, a.batch, a.tokens, a.max_rows, a.q_heads, a.kv_heads, a.head_dim = cache.page_table.data_ptr(), 2, 2, 1, hq, hkv, d
+        a.page_tokens, a.pages_per_seq, a.num_pages, a.max_context = pt, cache.config.pages_per_seq, cache.num_pages, 70
+        ws = torch.empty(max(1, lib.sfg_hip_attn_kv8_workspace_v1(ctypes.byref(a))), dtype=torch.uint8, device="cuda")
+        _abi.check(lib.sfg_hip_attn_kv8_v1(ctypes.byref(a), ws.data_ptr(), ws.numel(), None))
+        for b in range(2):
+            k, v = model.tokens(table[b], 70)
+            want, off = plain.attend64(q[b: b + 1].astype(np.float64), k, v, 70, d ** -0.5, dtype == F32)
+            got = rows["out"][b * stride: b * stride + hq * d].view(1, hq, d).double().cpu().numpy()
+            plain.close(got, want, off, plain.HALF[dtype])
+        assert float(rows["out"][hq * d]) == 3.0 and float(rows["out"][stride + hq * d]) == 3.0
+    codes, scales = plain.download(cache)
+    np.testing.assert_array_equal(codes, model.codes)
+    np.testing.assert_array_equal(scales, model.scales)
+    n = cache.k_pool.numel()
+    assert torch.equal(kp[:n], cache.k_pool.view(torch.uint8).flatten()) and torch.equal(vp[:n], cache.v_pool.view(torch.uint8).flatten())
+    assert (kp[n:] == 3).all() and (vp[n:] == 3).all()
+
+
+def test_no_context_at_all():
+    cache = make(2, 2, 64, 16, 32, "int8")
+    for d in (64, 40):
+        cache = make(2, 2, d, 16, 32, "int8")
+        assert torch.isnan(qk.quantized_attention(cache, torch.ones(4, 2, d, dtype=BF16, device="cuda"), max_context=0)).all()
+
+
 def test_lengths_are_cut_to_max_context():
     rng = np.random.default_rng(6)
     cache, model, table = filled(rng, [100, 50], 2, 64, 16, "fp8")

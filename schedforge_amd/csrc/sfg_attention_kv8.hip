@@ -499,6 +499,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NT == 2 ? 2 : QT == 3 ? (
             for (int t = begin; t < end; ++t) {
                 asm volatile("" ::: "memory");  // (the queries stay in LDS: in registers they cost a wave a SIMD)
                 floatx4 s[NT][4] = {};
+                __builtin_amdgcn_s_setprio(1);  // (matrix work of one wave beside the softmax of another)
 #pragma unroll
                 for (int f = 0; f < kF; ++f) {
                     bf16x8 q[NT][QT];
@@ -516,6 +517,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NT == 2 ? 2 : QT == 3 ? (
                             for (int e = QT - 1; e >= 0; --e) s[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[n][e], s[n][i], 0, 0, 0);
                     }
                 }
+                __builtin_amdgcn_s_setprio(0);
                 if (t + 1 < end) load_k(page_k, sub_k);
                 const int base = t * kTile + lg * 16;  // the lane's run
                 const float fk = sc.x * scale, fv = sc.y;
@@ -583,6 +585,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NT == 2 ? 2 : QT == 3 ? (
                         }
                     }
                 }
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int d = 0; d < kDt; ++d) {
                     const bf16x8 v0 = kv8_operand<FP8>(vr[d].x, vr[d].y), v1 = kv8_operand<FP8>(vr[d].z, vr[d].w);
@@ -595,6 +598,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NT == 2 ? 2 : QT == 3 ? (
                             o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, as_bf16x8(make_uint4(p[4], p[5], p[6], p[7])), o[n][d], 0, 0, 0);
                         }
                 }
+                __builtin_amdgcn_s_setprio(0);
                 if (t + 1 < end) {
                     load_v(page_v, sub_v);
                     next = min(t + 2, end - 1);
@@ -754,10 +758,12 @@ constexpr int64_t kMostSlots = 1 << 22;  // workgroups of a launch: 256 threads 
 // dealt 33; 16 fp32 rows over up to 8192 47, pieces from 24 tiles down 53).
 constexpr int64_t kRound = 512;
 constexpr int kFew = 16;
-#ifndef QUADS
-#define QUADS 8192
-#endif
-constexpr int kQuads = QUADS;
+// Tiles of all heads from which a workgroup takes four heads, its waves never waiting for each other
+// over a tile: 64 sequences of up to 2000 tokens 38.5 us for 43.8, 256 of up to 500 48.0 for 57.6, 64
+// of up to 8192, 16 heads of 64 over 4, 32.1 for 38.6; with fewer the waves' share is too long: 64
+// of up to 1000 31.1 for 28.1.  Few long sequences have more pieces to join for it (two of
+// 131072 tokens 74.9 for 70.6), so it takes a fourth as many sequences as shares.
+constexpr int kQuads = 8192;
 constexpr int64_t kManyRows = 4096;  // rows by heads from which a join's lanes have one each
 // Tiles up to which eight waves take a unit whole, a tile each, if every one of them has a compute
 // unit: one sequence of 500 tokens 10.2 us for 11.6, 32 of up to 500 12.2 for 15.5; 64 22.7 for 21.3.

@@ -243,6 +243,7 @@ int sfg_hip_abi_version(void) { return SFG_HIP_ABI_VERSION; }
 //   act / weights          activation dtypes and the weight dtypes each takes
 //   kv                     paged pools hold the activation dtype
 //   head_dim, page_tokens, decode_tokens   the widest shapes any path lowers
+//   kv8                    code types of the 8-bit caches
 //   mfma_*                 the shapes the MFMA kernels take (everything else
 //                          runs the row-per-wave attention / VALU GEMM paths)
 const char* sfg_hip_metadata_v1(void) {
@@ -250,6 +251,7 @@ const char* sfg_hip_metadata_v1(void) {
            "weights=f32:f32,bf16:bf16|i8;weight_layout=NK,TILED;"
            "kv_layout=page,kv_head,page_token,head_dim;kv=act_dtype;"
            "head_dim=1..256;page_tokens=any;decode_tokens=any;ffn=dense,moe;"
+           "kv8=i8,fp8;mfma_kv8=head_dim=64|128,page_tokens%16==0;"
            "mfma_decode=bf16,head_dim=64|128,page_tokens=16,decode_tokens=1,gqa_group=1|2|4|8|16;"
            "mfma_prefill=bf16,head_dim=64|128;mfma_gemm=bf16|i8,k%32==0;"
            "accumulate=f32;bf16_rounding=rne";

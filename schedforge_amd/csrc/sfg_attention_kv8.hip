@@ -3,6 +3,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <bit>
 
 #include "sfg_kernels.hpp"
 #include "sfg_kv8.hpp"
@@ -19,7 +20,7 @@ struct Kv8Args {
     float scale;
     int group;
     // the matrix-core kernels' (the rows kernel: fixed)
-    int slots, share, quads, fixed, least, few, width;  // (as in Kv8Plan)
+    int slots, share, quads, fixed, least, few, width, row_shift;  // (as in Kv8Plan)
     int vec, out_vec;                                      // rows begin on 16-byte boundaries
     int4* slot_of; int* sequence_of; float2* part_ml; float* part_acc;
     // A column's row (single rows without the division).
@@ -231,95 +232,171 @@ __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; 
 __device__ __forceinline__ int groups_of(int cols, int width) { return cols > 2 * width ? 4 : cols > width ? 2 : 1; }
 __device__ __forceinline__ int blocks_of(int cols, int width) { return cols > 4 * width ? ceil_div(cols, 4 * width) : cols > 0; }
 
-// A unit of work: a block of a sequence's columns over all its tiles.
-struct Unit {
-    int b, block, blocks, tiles, t0, rows, len;
-    int ord;      // units before it
-    int before;   // tiles of the sequences before (where tiles are dealt), else their splits
+// A sequence's blocks of columns, the tiles that each walks and what it costs.  A block walks up to
+// the last token that a row of it sees.  Where it has a whole number of rows, 2^row_shift, that and
+// its sums are in closed form; else every block counts the sequence's tiles.  Costs: a tile 1, or
+// 2 where each wave walks all of them (1.4 us for 3.5 with two workgroups a compute unit); a
+// block's queries and sums two tiles', or four (10 us or more).  A prompt of 4096 rows: 258 us, dealt
+// as if every block walked all tiles 343.  MANY: a sequence may have several blocks (for one, and 16
+// columns, the code that is left out costs 0.3 us of 11.5).
+template <bool MANY>
+struct Blocks {
+    int count, tiles;   // blocks, and tiles of the sequence (of the last block, where steps are known)
+    int before, shift;  // tokens before the first row; rows of a block (-1: steps are not known)
+    int twice;          // 1: a tile costs 2
+    template <int WIDTH>
+    __device__ __forceinline__ static Blocks of(const Kv8Args& a, int rows, int len) {
+        const int live = min(rows, a.max_rows), cols = live * a.group;
+        Blocks x{MANY ? blocks_of(cols, WIDTH) : cols > 0, max(ceil_div(len, kTile), 1), len - rows, -1, MANY && cols > 2 * WIDTH};
+        if (MANY && x.count > 1 && x.before >= 0) {
+            x.shift = a.row_shift;
+            if (x.shift >= 0) x.tiles = max(ceil_div(x.before + live, kTile), 1);
+        }
+        return x;
+    }
+    __device__ __forceinline__ int tiles_of(int block) const {
+        return MANY && shift >= 0 && block + 1 < count ? ceil_div(before + ((block + 1) << shift), kTile) : tiles;
+    }
+    // Tiles of the first n blocks, n < count.
+    __device__ __forceinline__ int64_t sum(int n) const {
+        if (shift < 0) return static_cast<int64_t>(n) * tiles;
+        const int64_t pairs = static_cast<int64_t>(n) * (n - 1) / 2;
+        if (shift >= 6) return static_cast<int64_t>(n) * ceil_div(before + (1 << shift), kTile) + (pairs << (shift - 6));
+        // sums of floor((at + i) / 2^k)
+        const int k = 6 - shift, at = (before + (1 << shift) + kTile - 1) >> shift;
+        return upto(at + n, k) - upto(at, k);
+    }
+    __device__ __forceinline__ static int64_t upto(int m, int k) {
+        const int64_t q = m >> k;
+        return ((q * (q - 1) / 2) << k) + (m & ((1 << k) - 1)) * q;
+    }
+    // Costs: of a block's own work, of the first n blocks, n < count, and of all.
+    __device__ __forceinline__ int own() const { return 2 + 2 * twice; }
+    __device__ __forceinline__ int64_t cost(int n) const { return (sum(n) + static_cast<int64_t>(n) * own()) << twice; }
+    __device__ __forceinline__ int64_t cost() const {
+        if (!MANY) return count * (tiles + own());
+        return ((count > 1 ? sum(count - 1) : 0) + (count > 0 ? tiles : 0) + static_cast<int64_t>(count) * own()) << twice;
+    }
+    // Where a block's tile begins among its costs.
+    __device__ __forceinline__ int at(int tile) const { return (tile + own()) << twice; }
+    // Its tiles that begin before a cost.
+    __device__ __forceinline__ int tiles_before(int cost) const { return max(((cost + twice) >> twice) - own(), 0); }
 };
-// A sequence's tiles or pieces, for all its blocks.  Starts and lengths that a caller left in
-// disorder may give any product: what the host has checked never reaches the cuts, and with them
-// 64 of these and the sum before them fit 32 bits.
-constexpr int kMaxTiles = 1 << 23, kMaxAll = 1 << 29;
-__device__ __forceinline__ int in_all(int of_block, int blocks) {
-    return static_cast<int>(min(static_cast<int64_t>(of_block) * blocks, static_cast<int64_t>(kMaxTiles)));
-}
-template <int WIDTH>
-__device__ __forceinline__ void load_unit(const Kv8Args& a, int b, Unit& u) {
-    u.tiles = u.blocks = u.t0 = u.rows = u.len = 0;
+
+// A unit of work: a block of a sequence's columns over its tiles.
+template <bool MANY>
+struct Unit {
+    int b, block, tiles, t0, rows, len;
+    Blocks<MANY> of;
+    int ord;    // units before it
+    int begin;  // costs before it, where tiles are dealt; else the pieces of the sequences before
+};
+// Starts and lengths that a caller left in disorder may give any cost: what the host has checked
+// never reaches the cuts, and with them 64 of these and the sum before them fit 32 bits.
+constexpr int kMostCost = 1 << 23, kMostCosts = 1 << 29;
+__device__ __forceinline__ int cut(int64_t n) { return static_cast<int>(min(n, static_cast<int64_t>(kMostCost))); }
+template <int WIDTH, bool MANY>
+__device__ __forceinline__ void load_unit(const Kv8Args& a, int b, Unit<MANY>& u) {
+    u.tiles = u.t0 = u.rows = u.len = 0;
+    u.of = {};
     if (b >= a.batch) return;
     a.sequence(b, u.t0, u.rows, u.len);
-    u.blocks = blocks_of(min(u.rows, a.max_rows) * a.group, WIDTH);
-    u.tiles = max(ceil_div(u.len, kTile), 1);
+    u.of = Blocks<MANY>::template of<WIDTH>(a, u.rows, u.len);
+    u.tiles = u.of.tiles_of(0);
 }
 
 // How the units' tiles are given to workgroups, which each one works out from the lengths.
-// Dealt (each 0): in units' order, the same number to each of `groups`, across units: with a
+// Dealt (each 0): in units' order, the same cost to each of `groups`, across units: with a
 // round of workgroups as long as the work, none waits for another's longer share.  Split: a unit
-// into pieces of `each` tiles, a workgroup a piece, where there are few: a second unit would
-// double a workgroup's time.  64 sequences of up to 8192 tokens: dealt 109 us, split into 1280
-// pieces 117; four of up to 2001 with 5 fp32 rows: 20 and 14.
+// into pieces of `each` tiles (of the sequence's, for each of its blocks), a workgroup a piece, where
+// there are few: a second unit would double a workgroup's time.  64 sequences of up to 8192 tokens:
+// dealt 109 us, split into 1280 pieces 117; four of up to 2001 with 5 fp32 rows: 20 and 14.
 struct Shares {
-    int all, groups, each, fixed;
+    int cost, groups, each, fixed;
     bool quads;  // a workgroup's waves take four kv heads, not a fourth of the tiles each
-    __device__ Shares(const Kv8Args& a, int n) : all(n), groups(a.share), each(0), fixed(a.fixed) {
+    // n: the sequences' tiles for each of their blocks
+    __device__ Shares(const Kv8Args& a, int n, int of_all) : cost(of_all), groups(a.share), each(0), fixed(a.fixed) {
         quads = !fixed && a.quads && static_cast<int64_t>(n) * a.kv_heads >= a.quads;
         if (quads) groups *= 4;
         if (fixed || n <= groups * a.few) each = max(ceil_div(n, max(groups, 1)), a.least);
     }
     __device__ int pieces(int tiles) const { return ceil_div(tiles, fixed ? ceil_div(tiles, fixed) : each); }
-    __device__ int begin(int w) const { return static_cast<int>(static_cast<int64_t>(all) * w / groups); }
-    __device__ int of(int tile) const { return static_cast<int>((static_cast<int64_t>(tile + 1) * groups - 1) / all); }
+    __device__ int begin(int w) const { return static_cast<int>(static_cast<int64_t>(cost) * w / groups); }
+    __device__ int of(int at) const { return static_cast<int>((static_cast<int64_t>(at + 1) * groups - 1) / cost); }
 };
 
-// The unit that tile `at` of all of them belongs to (where units are split: piece `at`), and its
-// place there.  first: the lane's sequence of the first 64.
-template <int WIDTH>
-__device__ __forceinline__ bool find_unit(const Kv8Args& a, const Shares& how, const Unit& first, int at, Unit& u, int& place) {
+// The unit that `at` of all costs belongs to (where units are split: piece `at`), and its place
+// there.  first: the lane's sequence of the first 64.
+template <int WIDTH, bool MANY>
+__device__ __forceinline__ bool find_unit(const Kv8Args& a, const Shares& how, const Unit<MANY>& first, int at, Unit<MANY>& u, int& place) {
+    const int lane = threadIdx.x & 63;
     int sum = 0, ord = 0;
-    Unit v = first;
+    Unit<MANY> v = first;
     for (int base = 0;;) {
-        const int mine = v.blocks == 0 ? 0 : in_all(how.each ? how.pieces(v.tiles) : v.tiles, v.blocks);
-        const int upto = wave_inclusive(mine) + sum, units = wave_inclusive(v.blocks) + ord;
+        const int mine = v.of.count == 0 ? 0 : cut(how.each ? static_cast<int64_t>(how.pieces(v.of.tiles)) * v.of.count : v.of.cost());
+        const int upto = wave_inclusive(mine) + sum, units = wave_inclusive(v.of.count) + ord;
         const uint64_t behind = __ballot(upto > at);
         if (behind) {
             const int l = __builtin_ctzll(behind);
             u.b = base + l;
-            u.blocks = __builtin_amdgcn_readlane(v.blocks, l);
-            u.tiles = __builtin_amdgcn_readlane(v.tiles, l);
+            u.of.count = __builtin_amdgcn_readlane(v.of.count, l);
+            u.of.tiles = __builtin_amdgcn_readlane(v.of.tiles, l);
+            u.of.before = __builtin_amdgcn_readlane(v.of.before, l);
+            u.of.shift = __builtin_amdgcn_readlane(v.of.shift, l);
             u.t0 = __builtin_amdgcn_readlane(v.t0, l);
             u.rows = __builtin_amdgcn_readlane(v.rows, l);
             u.len = __builtin_amdgcn_readlane(v.len, l);
-            u.before = __builtin_amdgcn_readlane(upto - mine, l);
-            const int of_block = how.each ? how.pieces(u.tiles) : u.tiles;
-            u.block = (at - u.before) / of_block;
-            place = at - u.before - u.block * of_block;
-            u.ord = __builtin_amdgcn_readlane(units - v.blocks, l) + u.block;
+            u.of.twice = __builtin_amdgcn_readlane(v.of.twice, l);
+            u.begin = __builtin_amdgcn_readlane(upto - mine, l);
+            const int rest = at - u.begin;
+            u.block = 0;
+            place = rest;
+            if (MANY && how.each) {
+                const int of_block = how.pieces(u.of.tiles);
+                u.block = rest / of_block;
+                place = rest - u.block * of_block;
+            } else if (MANY && u.of.count > 1) {  // the last block that begins there or before
+                for (int from = 0; from < u.of.count; from += kWave) {
+                    const uint64_t behind_it = __ballot(from + lane >= u.of.count || u.of.cost(from + lane) > rest);
+                    u.block = max(from + (behind_it ? __builtin_ctzll(behind_it) : kWave) - 1, 0);
+                    if (behind_it) break;
+                }
+                const int begin = static_cast<int>(u.of.cost(u.block));
+                place = rest - begin;
+                u.begin += begin;
+            }
+            u.ord = __builtin_amdgcn_readlane(units - v.of.count, l) + u.block;
+            u.tiles = how.each ? u.of.tiles : u.of.tiles_of(u.block);
             return true;
         }
         sum = __builtin_amdgcn_readlane(upto, 63);
         ord = __builtin_amdgcn_readlane(units, 63);
         if ((base += kWave) >= a.batch) return false;
-        load_unit<WIDTH>(a, base + (threadIdx.x & 63), v);
+        load_unit<WIDTH>(a, base + lane, v);
     }
 }
 
 // (the same in all lanes: kept in scalar registers)
 __device__ __forceinline__ void same(int& x) { x = __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ void same(Unit& u) {
-    same(u.b); same(u.block); same(u.blocks); same(u.tiles); same(u.t0); same(u.rows); same(u.len); same(u.ord); same(u.before);
+template <bool MANY>
+__device__ __forceinline__ void same(Unit<MANY>& u) {
+    same(u.b); same(u.block); same(u.tiles); same(u.t0); same(u.rows); same(u.len); same(u.ord); same(u.begin);
+    same(u.of.count); same(u.of.tiles); same(u.of.before); same(u.of.shift); same(u.of.twice);
 }
 
-// The unit behind u, if there is one.
-template <int WIDTH>
-__device__ __forceinline__ void next_unit(const Kv8Args& a, Unit& u) {
+// The unit behind u, if there is one, where tiles are dealt.
+template <int WIDTH, bool MANY>
+__device__ __forceinline__ void next_unit(const Kv8Args& a, Unit<MANY>& u) {
     ++u.ord;
-    if (++u.block < u.blocks) return;
-    u.before += u.tiles * u.blocks;
+    u.begin += u.of.at(u.tiles);
+    if (MANY && ++u.block < u.of.count) {
+        u.tiles = u.of.tiles_of(u.block);
+        return;
+    }
     u.block = 0;
     do {
         load_unit<WIDTH>(a, ++u.b, u);
-    } while (u.blocks == 0 && u.b < a.batch);
+    } while (u.of.count == 0 && u.b < a.batch);
 }
 
 // 8 codes as an MFMA operand.
@@ -380,38 +457,48 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NT == 2 ? 2 : QT == 3 ? (
     const int pt = P16 ? 16 : a.pt, runs = pt >> 4;  // 16-token runs of a page
 
     // what this workgroup walks: a piece of a unit, or tiles of one unit after the other
-    Unit first, u;
+    Unit<(NT == 2 || QT == 3)> first, u;  // (a row's 16 columns: one block)
     load_unit<kCols>(a, lane, first);
-    int all = 0;
+    int all = 0, cost = 0;
     if (!a.fixed) {
-        all = __builtin_amdgcn_readlane(wave_inclusive(in_all(first.tiles, first.blocks)), 63);
-        for (int base = kWave; base < a.batch; base += kWave) {
+        u = first;
+        for (int base = 0;;) {
+            const int64_t n = static_cast<int64_t>(u.of.tiles) * u.of.count;
+            all = min(all + __builtin_amdgcn_readlane(wave_inclusive(cut(n)), 63), kMostCosts);
+            cost = min(cost + __builtin_amdgcn_readlane(wave_inclusive(cut(u.of.cost())), 63), kMostCosts);
+            if ((base += kWave) >= a.batch) break;
             load_unit<kCols>(a, base + lane, u);
-            all = min(all + __builtin_amdgcn_readlane(wave_inclusive(in_all(u.tiles, u.blocks)), 63), kMaxAll);
         }
     }
-    Shares how(a, all);
+    Shares how(a, all, cost);
     same(how.each);
     const bool quads = WAVES == 4 && NT == 1 && how.quads;
     const int across = quads ? a.kv_heads >> 2 : a.kv_heads, group = blockIdx.x / across;
     const int kvh = quads ? 4 * (blockIdx.x - group * across) + wave : blockIdx.x - group * across;
-    int tile0, left;
+    int tile0, count, until = 0;
     if (how.each) {
         if (!find_unit<kCols>(a, how, first, group, u, tile0)) return;
         const int each = how.fixed ? ceil_div(u.tiles, how.fixed) : how.each;
         tile0 *= each;
-        left = min(each, u.tiles - tile0);
+        count = min(each, u.tiles - tile0);
     } else {
         if (group >= how.groups) return;
         const int from = how.begin(group);
-        left = how.begin(group + 1) - from;
+        until = how.begin(group + 1);
         if (!find_unit<kCols>(a, how, first, from, u, tile0)) return;
+        tile0 = u.of.tiles_before(tile0);
+        if (tile0 >= u.tiles) {
+            next_unit<kCols>(a, u);
+            tile0 = 0;
+        }
+        count = min(u.of.tiles_before(until - u.begin), u.tiles) - tile0;
     }
+    same(until);
     for (;;) {
         same(u);
         same(tile0);
-        same(left);
-        const int count = min(left, u.tiles - tile0);
+        same(count);
+        if (count <= 0 || u.b >= a.batch) return;
         const int cols = min(u.rows, a.max_rows) * a.group;
         const int groups = quads ? 1 : groups_of(cols, kCols), ways = quads ? 1 : WAVES / groups, col0 = u.block * groups * kCols;
         const int wcol = col0 + wave % groups * kCols;  // (may lie behind the columns)
@@ -654,14 +741,14 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NT == 2 ? 2 : QT == 3 ? (
         }
         // where the join finds a row's sequence, and the sequence's pieces or tiles among all
         if (a.slot_of && tile0 == 0 && kvh == 0) {
-            if (u.block == 0 && threadIdx.x == 0) a.slot_of[u.b] = make_int4(u.before, how.each ? how.pieces(u.tiles) : u.ord, u.tiles, how.each ? 0 : all);
+            if (u.block == 0 && threadIdx.x == 0) a.slot_of[u.b] = make_int4(u.begin, how.each ? how.pieces(u.tiles) : u.ord, cost, how.each ? 0 : all);
             for (int e = begin_e; e < groups * kCols; e += step_e)
                 if (col0 + e < cols) a.sequence_of[u.t0 + a.row_of(col0 + e)] = u.b;
         }
-        if ((left -= count) <= 0) return;
+        if (how.each) return;
         next_unit<kCols>(a, u);
-        if (u.b >= a.batch) return;
         tile0 = 0;
+        count = min(u.of.tiles_before(until - u.begin), u.tiles);
         __syncthreads();  // (the sums have been read: the queries of the next unit go there)
     }
 }
@@ -684,17 +771,18 @@ __global__ __launch_bounds__(256) void attn_kv8_join_kernel(Kv8Args a) {
     const int4 at = a.slot_of[b];
     int t0, rows, len;
     a.sequence(b, t0, rows, len);
-    const int i = t - t0;
+    const int i = t - t0, all_rows = rows;
     rows = min(rows, a.max_rows);
     if (i < 0 || i >= rows) return;  // (a row that no sequence computes)
     const int wide = groups_of(rows * a.group, WIDTH) * WIDTH;
     const int c = i * a.group + h - kvh * a.group, block = c / wide;
     int slot = at.x + block * at.y, splits = at.y;
     if (at.w) {
-        const Shares how(a, at.w);
-        const int from = at.x + block * at.z;
-        slot = how.of(from);
-        splits = how.of(from + at.z - 1) - slot + 1;
+        const Shares how(a, at.w, at.z);
+        const auto of = Blocks<true>::of<WIDTH>(a, all_rows, len);
+        const int from = at.x + static_cast<int>(of.cost(block));
+        slot = how.of(from + of.at(0));
+        splits = how.of(from + of.at(of.tiles_of(block) - 1)) - slot + 1;
         slot += at.y + block;
     }
     if (splits <= 1 || slot < 0 || slot > a.slots - splits) return;
@@ -795,8 +883,11 @@ Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a) {
     p.nt = narrow && cols > 16 ? 2 : 1;
     p.width = 16 * p.nt * (cols > 32 * p.nt ? 4 : cols > 16 * p.nt ? 2 : 1);
     const int64_t blocks = a.tokens * group / (64 * p.nt) + a.batch;  // of all sequences, at most
-    if (blocks * a.kv_heads > kMostSlots || (cols / (64 * p.nt) + 1) * tiles > kMaxTiles || blocks * tiles > kMaxAll) return plan_rows(a);
+    const int64_t cost = 2 * (tiles + 4);  // of a block, at most
+    if (blocks * a.kv_heads > kMostSlots || (cols / (64 * p.nt) + 1) * cost > kMostCost || blocks * cost > kMostCosts) return plan_rows(a);
     p.mfma = true;
+    const int64_t wide = 64 * p.nt;  // columns of a block where a sequence has several
+    p.row_shift = wide % group == 0 ? std::countr_zero(static_cast<uint64_t>(wide / group)) : -1;
     p.least = 4;  // (a tile a wave)
     p.few = kFew;
     p.fixed = static_cast<int>(std::min<int64_t>({std::max(a.kv_splits, 0), tiles, kMostSlots / (blocks * a.kv_heads)}));
@@ -872,7 +963,7 @@ void launch_attn_kv8(const sfg_kv8_attn_args& s, const Kv8Plan& plan, void* work
     a.fixed = plan.fixed;
     if (plan.mfma && aligned) {
         a.slots = plan.slots; a.share = plan.share; a.least = plan.least; a.few = plan.few; a.quads = plan.quads;
-        a.width = plan.width;
+        a.width = plan.width; a.row_shift = plan.row_shift;
         a.vec = (reinterpret_cast<uintptr_t>(s.q) & 15) == 0 && s.q_stride % 8 == 0;
         a.out_vec = (reinterpret_cast<uintptr_t>(s.out) & 15) == 0 && s.out_stride % 4 == 0;
         if (plan.bytes) {

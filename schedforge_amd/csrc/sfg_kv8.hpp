@@ -46,11 +46,11 @@ void launch_kv8_append(const sfg_kv8_append_args& a, hipStream_t stream);
 // `few` for each; with fewer, units are split into pieces of `least` tiles or more, at most
 // share and the units together.  quads (0: never): with so many tiles of all heads, a workgroup
 // takes four heads, and there are four times as many shares.  fixed: pieces a unit, instead of
-// all that.  slots: partial results a kv head, at most; groups: workgroups.  bytes: 0 if no unit
-// is split.
+// all that.  row_shift: a block has 2^row_shift whole rows (-1: it has not).  slots: partial
+// results a kv head, at most; groups: workgroups.  bytes: 0 if no unit is split.
 struct Kv8Plan {
     bool mfma;
-    int nt, waves, width, slots, groups, share, quads, fixed, least, few;
+    int nt, waves, width, slots, groups, share, quads, fixed, least, few, row_shift;
     size_t bytes;
 };
 Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a);

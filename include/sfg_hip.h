@@ -598,7 +598,7 @@ int sfg_hip_kv8_append_v1(const sfg_kv8_append_args* args, void* stream);
 /* Causal attention of each sequence's newest rows over its cache: with R = starts[b + 1] -
  * starts[b] rows and L = seq_lens[b] tokens (clamped to [0, max_context]; the rows' own
  * tokens included), row i sees token j iff j <= L - R + i.  q and out [T][Hq][D] with row
- * strides in elements, at least Hq D; out is not q.  starts NULL: every sequence has
+ * strides in elements, at least Hq D; out overlaps nothing else.  starts NULL: every sequence has
  * max_rows rows, T = batch * max_rows.  max_rows bounds the rows of any sequence: those
  * past it are not computed.  A row that sees nothing comes out NaN (0 / 0); tokens on a
  * page whose id is outside the pool are not seen; what no row sees may hold anything.

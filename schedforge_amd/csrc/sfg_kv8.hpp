@@ -41,8 +41,8 @@ __device__ __forceinline__ float kv8_larger(float a, float b) { return a >= b ||
 void launch_kv_plan(const sfg_kv_plan_args& a, hipStream_t stream);
 void launch_rope(const sfg_rope_args& a, hipStream_t stream);
 void launch_kv8_append(const sfg_kv8_append_args& a, hipStream_t stream);
-// How an attention runs.  A unit is a block of at most `width` columns of a sequence over all
-// its tiles.  share: the workgroups a kv head that all tiles are dealt to if there are more than
+// How an attention runs.  A unit is a block of at most `width` columns of a sequence over the
+// tiles it sees.  share: the workgroups a kv head that all tiles are dealt to if there are more than
 // `few` for each; with fewer, units are split into pieces of `least` tiles or more, at most
 // share and the units together.  quads (0: never): with so many tiles of all heads, a workgroup
 // takes four heads, and there are four times as many shares.  fixed: pieces a unit, instead of

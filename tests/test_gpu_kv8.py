@@ -380,6 +380,24 @@ def test_long_sequences(hq, hkv, d, pt, lens, rows, dtype, kind):
     assert got.shape == again.shape
 
 
+# more than 16 tiles for each of a head's workgroups, of sequences whose rows fill several blocks of 64 or 128 columns
+PROMPTS = [
+    (64, 64, 64, 16, [1100], [1100]),                               # a whole prompt: blocks see 1, 3, 5 ... tiles
+    (64, 64, 128, 16, [1100, 3, 640, 1000, 0], [500, 1, 130, 300, 2]),
+    (128, 64, 64, 32, [900, 77, 1300], [300, 0, 400]),
+    (192, 64, 64, 16, [700, 1500], [300, 100]),                     # no whole number of rows a block
+    (256, 32, 64, 48, [1000, 50, 900], [257, 180, 100])]            # 130 rows before the first token
+
+
+@pytest.mark.parametrize("dtype,kind", [(BF16, "fp8"), (F32, "int8")])
+@pytest.mark.parametrize("hq,hkv,d,pt,lens,rows", PROMPTS)
+def test_prompts_in_shares(hq, hkv, d, pt, lens, rows, dtype, kind):
+    """Workgroups whose shares begin and end inside blocks that see different numbers of tokens."""
+    rng = np.random.default_rng(sum(lens) + hq)
+    cache, model, table = random_cache(rng, lens, hkv, d, pt, kind)
+    check_attention(cache, model, table, lens, rows, hq, dtype, rng, max_rows=max(rows))
+
+
 def test_the_same_call_gives_the_same_bits():
     rng = np.random.default_rng(3)
     lens = [4000, 100, 900, 2000]

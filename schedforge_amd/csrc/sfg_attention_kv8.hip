@@ -376,6 +376,9 @@ __device__ __forceinline__ bool find_unit(const Kv8Args& a, const Shares& how, c
     }
 }
 
+// Memory operations before it stay before those behind it.
+__device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
+
 // (the same in all lanes: kept in scalar registers)
 __device__ __forceinline__ void same(int& x) { x = __builtin_amdgcn_readfirstlane(x); }
 template <bool MANY>
@@ -561,13 +564,19 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NT == 2 ? 2 : QT == 3 ? (
 #pragma unroll
                 for (int j = 0; j < D / 64; ++j) kr[i][j] = kv8_fetch<QT == 1 && NT == 1>(a.k_pool + at + i * 4 * D + j * 64);
         };
-        auto load_v = [&](int page, int sub) {
+        const uint8_t* v_at;
+        const float2* s_at;
+        auto find_v = [&](int page, int sub) {
             vok = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages);
             const int64_t at = static_cast<int64_t>(vok ? page : 0) * a.kv_heads + kvh;
-            sc = reinterpret_cast<const float2*>(a.scales)[at];
-            const uint8_t* p = a.v_pool + at * (pt * D) + static_cast<int64_t>(lr) * pt + sub * 16;
+            s_at = reinterpret_cast<const float2*>(a.scales) + at;
+            v_at = a.v_pool + at * (pt * D) + static_cast<int64_t>(lr) * pt + sub * 16;
+        };
+        auto load_v = [&]() {
+            sc = *s_at;
+            in_order();
 #pragma unroll
-            for (int i = 0; i < kDt; ++i) vr[i] = kv8_fetch<QT == 1 && NT == 1>(p + static_cast<int64_t>(i) * 16 * pt);
+            for (int i = 0; i < kDt; ++i) vr[i] = kv8_fetch<QT == 1 && NT == 1>(v_at + static_cast<int64_t>(i) * 16 * pt);
         };
         floatx4 o[NT][kDt] = {};
         float m[NT], l[NT];
@@ -576,15 +585,22 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NT == 2 ? 2 : QT == 3 ? (
             m[n] = -INFINITY;
             l[n] = 0.f;
         }
+        // A loop that waits for no load but the one it uses: loads are counted in order, so they are issued
+        // in one order on every path into it, K among them without a branch (behind the last tile a page that
+        // the caches hold), and page ids before the loads that may stay in flight.
+        auto pages = [&](int t) {
+            in_order();
+            page_k = page_of(4 * t + (lr >> 2), sub_k);
+            page_v = page_of(4 * t + lg, sub_v);
+            in_order();
+        };
         if (begin < end) {
             load_k(page_k, sub_k);
-            load_v(page_v, sub_v);
-            // the pages of the tile behind the one in flight
-            int next = min(begin + 1, end - 1);
-            page_k = page_of(4 * next + (lr >> 2), sub_k);
-            page_v = page_of(4 * next + lg, sub_v);
-            for (int t = begin; t < end; ++t) {
-                asm volatile("" ::: "memory");  // (the queries stay in LDS: in registers they cost a wave a SIMD)
+            find_v(page_v, sub_v);
+            pages(min(begin + 1, end - 1));
+            load_v();
+            for (int t = begin;; ++t) {
+                in_order();  // (and the queries stay in LDS: in registers they cost a wave a SIMD)
                 floatx4 s[NT][4] = {};
                 __builtin_amdgcn_s_setprio(1);  // (matrix work of one wave beside the softmax of another)
 #pragma unroll
@@ -605,9 +621,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NT == 2 ? 2 : QT == 3 ? (
                     }
                 }
                 __builtin_amdgcn_s_setprio(0);
-                if (t + 1 < end) load_k(page_k, sub_k);
                 const int base = t * kTile + lg * 16;  // the lane's run
                 const float fk = sc.x * scale, fv = sc.y;
+                in_order();
+                load_k(t + 1 < end ? page_k : -1, sub_k);
+                in_order();
                 const bool part = t * kTile + kTile > seen_all || __any(!vok);
                 uint32_t pw[NT][PT][8];
 #pragma unroll
@@ -686,12 +704,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NT == 2 ? 2 : QT == 3 ? (
                         }
                 }
                 __builtin_amdgcn_s_setprio(0);
-                if (t + 1 < end) {
-                    load_v(page_v, sub_v);
-                    next = min(t + 2, end - 1);
-                    page_k = page_of(4 * next + (lr >> 2), sub_k);
-                    page_v = page_of(4 * next + lg, sub_v);
-                }
+                if (t + 1 >= end) break;
+                find_v(page_v, sub_v);
+                pages(min(t + 2, end - 1));
+                load_v();
             }
         }
         // the waves of a column group, joined in LDS (of four heads: each one alone, laid out for its stores)

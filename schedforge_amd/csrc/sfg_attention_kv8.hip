@@ -630,8 +630,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || NT == 2 ? 2 : QT == 3 ? (
                 uint32_t pw[NT][PT][8];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const int live = vok ? min(max(seen[n] - base, 0), 16) : 0;  // tokens of the run that the column sees
+                    int live = 0;  // tokens of the run that the column sees
                     if (part) {
+                        live = vok ? min(max(seen[n] - base, 0), 16) : 0;
+                        asm volatile("" : "+v"(live));  // (its comparisons are not made for the tiles that need none)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) s[n][i / 4][i % 4] = i < live ? s[n][i / 4][i % 4] : -INFINITY;
                     }

@@ -215,7 +215,11 @@ __global__ __launch_bounds__(256) void attn_kv8_rows_begin_kernel(int* computed,
 //
 // Bound by HBM: a tile is 64 tokens x 2 D bytes, against 4 x (16 + 8 PT x 2) MFMA cycles and the
 // codes' conversion.  K's registers are loaded again as soon as the first product has read
-// them, V's after the second: a wave has up to 16 KB in flight.
+// them, V's after the second: a wave has up to 16 KB in flight.  64 sequences of up to 8192 tokens, 32
+// heads of 128 over 8, int8: 103 us (540 MB at 5.3 TB/s).  With many rows (four column groups over
+// the same tiles) by the units: beside one wave's matrix instructions of 16 cycles another one's
+// vector instructions get 6, and the clock is near 2 GHz.  4096 rows over 4096 tokens, e4m3:
+// 254 us, 540 TFLOP/s (32 x 32 x 16 products, which leave more to the other wave: 265; int8 301 and 292).
 //
 // A workgroup is four waves: one column group, its tiles split four ways, for up to 16 NT
 // columns; two by two for twice that; else four column groups over the same tiles.  (Eight waves
@@ -236,8 +240,8 @@ __device__ __forceinline__ int blocks_of(int cols, int width) { return cols > 4 
 // the last token that a row of it sees.  Where it has a whole number of rows, 2^row_shift, that and
 // its sums are in closed form; else every block counts the sequence's tiles.  Costs: a tile 1, or
 // 2 where each wave walks all of them (1.4 us for 3.5 with two workgroups a compute unit); a
-// block's queries and sums two tiles', or four (10 us or more).  A prompt of 4096 rows: 258 us, dealt
-// as if every block walked all tiles 343.  MANY: a sequence may have several blocks (for one, and 16
+// block's queries and sums two tiles', or four (10 us or more).  A prompt of 4096 rows: 254 us, dealt
+// as if every block walked all tiles 342.  MANY: a sequence may have several blocks (for one, and 16
 // columns, the code that is left out costs 0.3 us of 11.5).
 template <bool MANY>
 struct Blocks {
@@ -310,7 +314,7 @@ __device__ __forceinline__ void load_unit(const Kv8Args& a, int b, Unit<MANY>& u
 // round of workgroups as long as the work, none waits for another's longer share.  Split: a unit
 // into pieces of `each` tiles (of the sequence's, for each of its blocks), a workgroup a piece, where
 // there are few: a second unit would double a workgroup's time.  64 sequences of up to 8192 tokens:
-// dealt 109 us, split into 1280 pieces 117; four of up to 2001 with 5 fp32 rows: 20 and 14.
+// dealt 103 us, split into 1280 pieces 129; 32 of up to 2000: 30 and 27.
 struct Shares {
     int cost, groups, each, fixed;
     bool quads;  // a workgroup's waves take four kv heads, not a fourth of the tiles each
@@ -419,7 +423,7 @@ __device__ __forceinline__ bf16x8 kv8_operand(uint32_t lo, uint32_t hi) {
 }
 
 // 16 bytes of codes; ONCE: read by this workgroup alone, so not kept in the caches (64
-// sequences of up to 8192 tokens: 112 us -> 109, two of 131072: 76 -> 72).
+// sequences of up to 8192 tokens: 112.5 us -> 102.9, two of 131072: 75.9 -> 70.3).
 typedef uint32_t uint32x4 __attribute__((ext_vector_type(4)));
 template <bool ONCE>
 __device__ __forceinline__ uint4 kv8_fetch(const uint8_t* p) {
@@ -859,20 +863,22 @@ size_t rows_bytes(const sfg_kv8_attn_args& a, int64_t splits) {
 
 constexpr int64_t kMostSlots = 1 << 22;  // workgroups of a launch: 256 threads each
 // Workgroups that tiles are dealt to: two a compute unit, all of them resident at once.  (768, where
-// registers allow three: 64 sequences of up to 8192 tokens 108 us for 108, 64 with 8 rows
-// 187 for 159.)  Fewer than 16 tiles for each: pieces (32 sequences of up to 2000 tokens 28 us,
-// dealt 33; 16 fp32 rows over up to 8192 47, pieces from 24 tiles down 53).
+// registers allow three: 64 sequences of up to 8192 tokens 120 us for 103, 64 with 8 rows
+// 158 for 135.)  Fewer than 16 tiles for each: pieces (32 sequences of up to 2000 tokens 27 us,
+// dealt 30; 64 of up to 1000 27 and 31).  A piece is a tile a wave, and two tiles where each wave walks
+// them all: 256 rows over 300 tokens 25.4 us (four tiles 29.2, one 28.0), 16 fp32 rows over 8192
+// 16.8 (18.6, 18.9), 64 over 3000 21.5 (19.3, 21.3).
 constexpr int64_t kRound = 512;
 constexpr int kFew = 16;
 // Tiles of all heads from which a workgroup takes four heads, its waves never waiting for each other
-// over a tile: 64 sequences of up to 2000 tokens 38.5 us for 43.8, 256 of up to 500 48.0 for 57.6, 64
-// of up to 8192, 16 heads of 64 over 4, 32.1 for 38.6; with fewer the waves' share is too long: 64
-// of up to 1000 31.1 for 28.1.  Few long sequences have more pieces to join for it (two of
-// 131072 tokens 74.9 for 70.6), so it takes a fourth as many sequences as shares.
+// over a tile: 64 sequences of up to 2000 tokens 37.0 us for 41.3, 256 of up to 500 47.4 for 54.8, 64
+// of up to 8192, 16 heads of 64 over 4, 31.6 for 36.6; with fewer the waves' share is too long: 64
+// of up to 1000 29.7 for 27.6.  Few long sequences have more pieces to join for it (two of
+// 131072 tokens 74.1 for 70.9), so it takes a fourth as many sequences as shares.
 constexpr int kQuads = 8192;
 constexpr int64_t kManyRows = 4096;  // rows by heads from which a join's lanes have one each
 // Tiles up to which eight waves take a unit whole, a tile each, if every one of them has a compute
-// unit: one sequence of 500 tokens 10.2 us for 11.6, 32 of up to 500 12.2 for 15.5; 64 22.7 for 21.3.
+// unit: one sequence of 500 tokens 10.1 us for 11.2, 32 of up to 500 11.9 for 15.6; 64 21.3 for 21.9.
 constexpr int64_t kShort = 8;
 
 }  // namespace
@@ -900,13 +906,13 @@ Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a) {
     const int64_t tiles = std::max<int64_t>((a.max_context + kTile - 1) / kTile, 1);
     p.nt = narrow && cols > 16 ? 2 : 1;
     p.width = 16 * p.nt * (cols > 32 * p.nt ? 4 : cols > 16 * p.nt ? 2 : 1);
-    const int64_t blocks = a.tokens * group / (64 * p.nt) + a.batch;  // of all sequences, at most
+    const int64_t blocks = a.batch + (cols > 64 * p.nt ? a.tokens * group / (64 * p.nt) : 0);  // of all sequences, at most
     const int64_t cost = 2 * (tiles + 4);  // of a block, at most
     if (blocks * a.kv_heads > kMostSlots || (cols / (64 * p.nt) + 1) * cost > kMostCost || blocks * cost > kMostCosts) return plan_rows(a);
     p.mfma = true;
     const int64_t wide = 64 * p.nt;  // columns of a block where a sequence has several
     p.row_shift = wide % group == 0 ? std::countr_zero(static_cast<uint64_t>(wide / group)) : -1;
-    p.least = 4;  // (a tile a wave)
+    p.least = std::max(64 * p.nt / p.width, 2);  // (a tile a wave; two where each walks them all)
     p.few = kFew;
     p.fixed = static_cast<int>(std::min<int64_t>({std::max(a.kv_splits, 0), tiles, kMostSlots / (blocks * a.kv_heads)}));
     p.waves = 4;

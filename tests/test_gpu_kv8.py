@@ -621,6 +621,49 @@ def test_a_captured_step_serves_requests(kind, dtype, d, pt):
                 plain.close(out[t0:t1].double().cpu().numpy(), want, off, plain.HALF[dtype])
 
 
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("d", [128, 80])
+def test_pages_beyond_32_bit_offsets(d, kind):
+    """The same step in a pool of a few pages and, from the highest ids down, in one whose codes pass 2^31 bytes."""
+    rng = np.random.default_rng(d)
+    k, v = (dev(rounded(rng, (93, 8, d), BF16), BF16) for _ in range(2))
+    q = dev(rounded(rng, (93, 16, d), BF16), BF16)
+    found = []
+    for pages in (8, (1 << 31) // (8 * 16 * d) + 9):
+        cache = make(2, 8, d, 16, 100, kind, pages)
+        step = qk.plan_step(cache, dev([90, 3], torch.int32), 93)
+        assert int(cache.page_table.max()) == pages - 1
+        qk.append_quantized_kv(cache, k, v, step.slots)
+        found.append((qk.quantized_attention(cache, q, step.starts), cache.k_pool[pages - 7:].view(torch.int8),
+                      cache.v_pool[pages - 7:].view(torch.int8), cache.scales[pages - 7:]))
+        assert pages < 9 or cache.k_pool[: pages - 7].view(torch.int8).count_nonzero() == 0
+    for small, large in zip(*found):
+        assert torch.equal(small, large)
+    assert not found[1][0].isnan().any()
+
+
+def test_rows_beyond_32_bit_offsets():
+    """Queries, keys and values as columns of rows so wide that the last ones lie past 2^31 elements."""
+    rng = np.random.default_rng(8)
+    rows, wide, d = 2100, 1 << 20, 128
+    block = torch.zeros((rows, wide), dtype=BF16, device="cuda")
+    near = dev(rounded(rng, (rows, 4 * d), BF16), BF16)
+    block[:, wide - 4 * d:] = near
+    far = block[:, wide - 4 * d:]
+    found = []
+    for x in (near, far):
+        cache = make(1, 1, d, 16, rows, "int8")
+        step = qk.plan_step(cache, dev([rows], torch.int32), rows)
+        q, k, v = x[:, : 2 * d].view(rows, 2, d), x[:, 2 * d: 3 * d].view(rows, 1, d), x[:, 3 * d:].view(rows, 1, d)
+        q_out, k_out = qk.rotate(qk.RotaryAngles(d), step.positions, q, k, q_out=q, k_out=k)
+        qk.append_quantized_kv(cache, k_out, v, step.slots)
+        found.append((qk.quantized_attention(cache, q_out, step.starts, out=q_out.clone()), cache.k_pool, cache.v_pool, cache.scales))
+        found[-1] += (qk.quantized_attention(cache, q_out, step.starts, out=q_out.new_zeros((rows, 3, d))[:, :2]),)
+    for a, b in zip(*found):
+        assert torch.equal(a, b)
+    assert torch.equal(found[0][0], found[0][4])
+
+
 def test_on_a_stream_of_its_own():
     """The calls run on the stream they are given, behind what it holds, while another one is current."""
     rng = np.random.default_rng(12)

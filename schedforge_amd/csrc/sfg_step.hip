@@ -223,7 +223,7 @@ struct RopeArgs {
     const void* in[2]; void* out[2]; int64_t in_stride[2], out_stride[2]; int heads[2];
     const int32_t* positions; const uint64_t* turns; float magnitude;
     int tokens, dim, pairs, interleaved;
-    // a workgroup's rows and heads; units of a head and how to divide by them and by a row's
+    // a workgroup's rows and heads; units of a head and how to divide by them and by a row's (reciprocal: 0 for one)
     int rows, chunk, units;
     uint32_t by_units, by_row;
 };
@@ -304,7 +304,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a) {
         Item& it = item[i];
         it.position = -1;
         if (e >= items) return;
-        const int row = a.by_row ? __umulhi(e, a.by_row) : 0;
+        const int row = a.by_row ? __umulhi(e, a.by_row) : e;
         const int in_row = e - row * a.chunk * a.units;
         const int h = a.by_units ? __umulhi(in_row, a.by_units) : in_row, u = in_row - h * a.units;
         if (h >= heads) return;
@@ -376,7 +376,7 @@ void launch_rope_n(RopeArgs a, hipStream_t stream) {
     a.chunk = std::max(1, std::min(heads, (kMost + a.units - 1) / a.units));
     a.rows = std::max(1, std::min({a.tokens, kMost / (a.chunk * a.units), kMost / a.pairs}));
     a.by_units = reciprocal(a.units);
-    a.by_row = a.rows > 1 ? reciprocal(a.chunk * a.units) : 0;
+    a.by_row = reciprocal(a.chunk * a.units);
     const dim3 grid(static_cast<unsigned>((a.tokens + a.rows - 1) / a.rows), static_cast<unsigned>((heads + a.chunk - 1) / a.chunk));
     const size_t lds = a.rows * a.pairs * sizeof(float2);
     const bool streams = N > 1 && static_cast<int64_t>(a.tokens) * heads * a.dim * static_cast<int64_t>(sizeof(T)) >= kRopeStream;

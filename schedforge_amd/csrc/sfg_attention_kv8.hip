@@ -908,8 +908,10 @@ Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a) {
     p.width = 16 * p.nt * (cols > 32 * p.nt ? 4 : cols > 16 * p.nt ? 2 : 1);
     const int64_t blocks = a.batch + (cols > 64 * p.nt ? a.tokens * group / (64 * p.nt) : 0);  // of all sequences, at most
     const int64_t cost = 2 * (tiles + 4);  // of a block, at most
-    if (blocks * a.kv_heads > kMostSlots || (cols / (64 * p.nt) + 1) * cost > kMostCost || blocks * cost > kMostCosts) return plan_rows(a);
+    if (blocks * a.kv_heads > kMostSlots) return plan_rows(a);
     p.mfma = true;
+    // tiles are dealt by sums of costs in 32 bits; where those of the bounds pass them, units run whole
+    const bool summed = (cols / (64 * p.nt) + 1) * cost <= kMostCost && blocks * cost <= kMostCosts;
     const int64_t wide = 64 * p.nt;  // columns of a block where a sequence has several
     p.row_shift = wide % group == 0 ? std::countr_zero(static_cast<uint64_t>(wide / group)) : -1;
     p.least = std::max(64 * p.nt / p.width, 2);  // (a tile a wave; two where each walks them all)
@@ -920,7 +922,7 @@ Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a) {
         p.waves = 8;
         p.fixed = 1;
     }
-    if (!p.fixed && tiles > p.least) {
+    if (!p.fixed && summed && tiles > p.least) {
         p.share = static_cast<int>(std::max<int64_t>(kRound / a.kv_heads, 1));
         p.quads = narrow && p.nt == 1 && a.kv_heads % 4 == 0 && 4 * a.batch >= p.share ? kQuads : 0;
         const int64_t most = blocks * ((tiles + p.least - 1) / p.least);  // the shortest pieces

@@ -606,7 +606,9 @@ int sfg_hip_kv8_append_v1(const sfg_kv8_append_args* args, void* stream);
  * softmax and sums are fp32; with bf16 queries and a bf16 output the softmax weights times
  * V's scale enter the product with 16 bits, else with 24.  head_dim up to 256, any group
  * Hq / Hkv, any page size; head_dim 64 and 128 over pages of whole 16 tokens run on the
- * matrix cores.  The same call gives the same bits (no atomics). */
+ * matrix cores.  The same call gives the same bits (no atomics).  The workspace query answers
+ * for these bounds and all shorter ones: the bytes serve every call with the same other
+ * sizes and no larger tokens, max_rows and max_context. */
 typedef struct {
     const void* q; int32_t q_dtype; int64_t q_stride;
     void* out; int32_t out_dtype; int64_t out_stride;                       /* SFG_F32 or SFG_BF16 */

@@ -151,7 +151,7 @@ int sfg_hip_kv8_append_v1(const sfg_kv8_append_args* a, void* stream) {
     return check_launch("kv8_append");
 }
 
-size_t sfg_hip_attn_kv8_workspace_v1(const sfg_kv8_attn_args* a) { return a && sized(*a) ? sfg::plan_attn_kv8(*a).bytes : 0; }
+size_t sfg_hip_attn_kv8_workspace_v1(const sfg_kv8_attn_args* a) { return a && sized(*a) ? sfg::workspace_attn_kv8(*a) : 0; }
 
 int sfg_hip_attn_kv8_v1(const sfg_kv8_attn_args* a, void* workspace, size_t workspace_bytes, void* stream) {
     if (!a) return fail(SFG_ERR_SHAPE, "attn_kv8: null arguments");

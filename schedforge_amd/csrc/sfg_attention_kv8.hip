@@ -856,12 +856,13 @@ size_t kv8_bytes(const sfg_kv8_attn_args& a, int64_t slots, int width) {
     return up256(a.batch * sizeof(int4)) + up256(a.tokens * sizeof(int)) + up256(columns * sizeof(float2)) + up256(columns * a.head_dim * sizeof(float));
 }
 
-size_t rows_bytes(const sfg_kv8_attn_args& a, int64_t splits) {
-    const size_t parts = static_cast<size_t>(a.tokens) * a.q_heads * splits;
+size_t parts_bytes(const sfg_kv8_attn_args& a, size_t parts) {
     return up256(a.tokens * sizeof(int)) + up256(parts * sizeof(float2)) + up256(parts * a.head_dim * sizeof(float));
 }
+size_t rows_bytes(const sfg_kv8_attn_args& a, int64_t splits) { return parts_bytes(a, static_cast<size_t>(a.tokens) * a.q_heads * splits); }
 
 constexpr int64_t kMostSlots = 1 << 22;  // workgroups of a launch: 256 threads each
+constexpr size_t kMostBytes = size_t{128} << 20;  // partial results, unless the caller says how many splits
 // Workgroups that tiles are dealt to: two a compute unit, all of them resident at once.  (768, where
 // registers allow three: 64 sequences of up to 8192 tokens 120 us for 103, 64 with 8 rows
 // 158 for 135.)  Fewer than 16 tiles for each: pieces (32 sequences of up to 2000 tokens 27 us,
@@ -892,21 +893,42 @@ Kv8Plan plan_rows(const sfg_kv8_attn_args& a) {
     else
         while (waves * splits < 2048 && chunks / (2 * splits) >= 2) splits *= 2;
     // (a launch's threads and the workspace stay within bounds)
-    while (splits > 1 && (waves * splits > (1 << 25) || rows_bytes(a, splits) > (size_t{128} << 20))) splits /= 2;
+    while (splits > 1 && (waves * splits > (1 << 25) || rows_bytes(a, splits) > kMostBytes)) splits /= 2;
     p.fixed = static_cast<int>(splits);
     p.bytes = splits > 1 ? rows_bytes(a, splits) : 0;
     return p;
 }
 
+namespace {
+
+bool mfma_dims(const sfg_kv8_attn_args& a) { return (a.head_dim == 64 || a.head_dim == 128) && a.page_tokens % 16 == 0; }
+// What the matrix-core kernels' plan and the workspace follow from.
+struct Kv8Sizes {
+    bool narrow;
+    int64_t group, cols, tiles, blocks, share;
+    int nt, width;
+    explicit Kv8Sizes(const sfg_kv8_attn_args& a) {
+        narrow = a.q_dtype == SFG_BF16 && a.out_dtype == SFG_BF16;
+        group = a.q_heads / a.kv_heads;
+        cols = a.max_rows * group;
+        tiles = std::max<int64_t>((a.max_context + kTile - 1) / kTile, 1);
+        nt = narrow && cols > 16 ? 2 : 1;
+        width = 16 * nt * (cols > 32 * nt ? 4 : cols > 16 * nt ? 2 : 1);
+        blocks = a.batch + (cols > 64 * nt ? a.tokens * group / (64 * nt) : 0);  // of all sequences, at most
+        share = std::max<int64_t>(kRound / a.kv_heads, 1);
+    }
+};
+
+}  // namespace
+
 Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a) {
-    if ((a.head_dim != 64 && a.head_dim != 128) || a.page_tokens % 16) return plan_rows(a);
+    if (!mfma_dims(a)) return plan_rows(a);
     Kv8Plan p{};
-    const bool narrow = a.q_dtype == SFG_BF16 && a.out_dtype == SFG_BF16;
-    const int64_t group = a.q_heads / a.kv_heads, cols = a.max_rows * group;
-    const int64_t tiles = std::max<int64_t>((a.max_context + kTile - 1) / kTile, 1);
-    p.nt = narrow && cols > 16 ? 2 : 1;
-    p.width = 16 * p.nt * (cols > 32 * p.nt ? 4 : cols > 16 * p.nt ? 2 : 1);
-    const int64_t blocks = a.batch + (cols > 64 * p.nt ? a.tokens * group / (64 * p.nt) : 0);  // of all sequences, at most
+    const Kv8Sizes z(a);
+    const bool narrow = z.narrow;
+    const int64_t group = z.group, cols = z.cols, tiles = z.tiles, blocks = z.blocks;
+    p.nt = z.nt;
+    p.width = z.width;
     const int64_t cost = 2 * (tiles + 4);  // of a block, at most
     if (blocks * a.kv_heads > kMostSlots) return plan_rows(a);
     p.mfma = true;
@@ -923,12 +945,12 @@ Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a) {
         p.fixed = 1;
     }
     if (!p.fixed && summed && tiles > p.least) {
-        p.share = static_cast<int>(std::max<int64_t>(kRound / a.kv_heads, 1));
+        p.share = static_cast<int>(z.share);
         p.quads = narrow && p.nt == 1 && a.kv_heads % 4 == 0 && 4 * a.batch >= p.share ? kQuads : 0;
         const int64_t most = blocks * ((tiles + p.least - 1) / p.least);  // the shortest pieces
         p.slots = static_cast<int>(std::min(p.share * (p.quads ? 4 : 1) + blocks, most));
         p.groups = static_cast<int>(std::min(p.share + blocks, most) * a.kv_heads);
-        if (kv8_bytes(a, p.slots, p.width) > (size_t{128} << 20)) p.share = 0;
+        if (kv8_bytes(a, p.slots, p.width) > kMostBytes) p.share = 0;  // (more rows: units run whole)
     }
     if (!p.share) {
         p.fixed = std::max(p.fixed, 1);
@@ -937,6 +959,32 @@ Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a) {
     }
     if (p.fixed != 1) p.bytes = kv8_bytes(a, p.slots, p.width);
     return p;
+}
+
+// Plans do not grow with their bounds: fewer columns take narrower blocks and other kernels, many rows
+// run whole.  The workspace does: it is what no plan of these or shorter bounds passes, each term
+// growing with tokens, max_rows and max_context.  (64 sequences of up to 131072 tokens, 32 + 8 heads of
+// 128: one row each 20 MiB, up to 2048 rows 98 MiB, 4096 and more 128 MiB, of which they take none.)
+size_t workspace_attn_kv8(const sfg_kv8_attn_args& a) {
+    const Kv8Sizes z(a);
+    const bool mfma = mfma_dims(a);
+    const int64_t splits = std::max(a.kv_splits, 0), units = kMostSlots / a.kv_heads;
+    size_t most = 0;
+    if (mfma && splits) {
+        const int64_t each = std::min(splits, z.tiles);
+        if (each > 1) most = kv8_bytes(a, std::min(z.blocks * each, units), z.width);
+    } else if (mfma && z.tiles > 2) {
+        most = kv8_bytes(a, std::min(z.share + z.blocks, z.blocks * ((z.tiles + 1) / 2)), z.width);
+        if (z.narrow && z.group <= 16 && a.kv_heads % 4 == 0 && 4 * a.batch >= z.share)  // (four heads a workgroup)
+            most = std::max(most, kv8_bytes(a, std::min(4 * z.share + a.batch, a.batch * ((z.tiles + 3) / 4)), 16));
+        most = std::min(most, kMostBytes);
+    }
+    if (mfma && z.blocks * a.kv_heads <= kMostSlots) return most;
+    // the rows kernel: as many splits as asked for, or until there are 2048 waves
+    const int64_t chunks = (a.max_context + 63) / 64, each = splits ? std::min(splits, chunks) : chunks / 2;
+    if (each < 2) return most;
+    const int64_t parts = std::min<int64_t>(a.tokens * a.q_heads * each, splits ? 1 << 25 : 4096);
+    return std::max(most, std::min(parts_bytes(a, parts), kMostBytes));
 }
 
 namespace {

@@ -54,6 +54,7 @@ struct Kv8Plan {
     size_t bytes;
 };
 Kv8Plan plan_attn_kv8(const sfg_kv8_attn_args& a);
+size_t workspace_attn_kv8(const sfg_kv8_attn_args& a);  // for these and all shorter bounds: plans' bytes or more
 void launch_attn_kv8(const sfg_kv8_attn_args& a, const Kv8Plan& plan, void* workspace, hipStream_t stream);
 
 }  // namespace sfg

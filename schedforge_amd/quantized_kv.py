@@ -266,7 +266,8 @@ def _attention(cache: QuantizedKVCache, tokens: int, q_heads: int, starts, max_r
 
 def attention_workspace(cache: QuantizedKVCache, tokens: int, q_heads: int, dtype: torch.dtype, starts=True,
                         max_rows: Optional[int] = None, max_context: Optional[int] = None, kv_splits: int = 0) -> int:
-    """Bytes of workspace that quantized_attention takes for queries of these sizes (and no larger ones)."""
+    """Bytes of workspace for quantized_attention with queries of these sizes, or of no larger tokens, max_rows and
+    max_context."""
     a = _attention(cache, tokens, q_heads, starts, max_rows, max_context, kv_splits, 0.0)
     a.q_dtype = a.out_dtype = _DTYPES[dtype]
     return cache.lib.sfg_hip_attn_kv8_workspace_v1(ctypes.byref(a))

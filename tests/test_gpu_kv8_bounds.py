@@ -72,3 +72,24 @@ def test_long_bounds_stay_on_the_matrix_cores(dtype, hq, hkv, d, pt, rows, capac
     whole = qk.quantized_attention(cache, q, at, kv_splits=1)
     near = qk.quantized_attention(cache, q, at, kv_splits=1, max_context=2048)
     assert torch.equal(whole[: starts[-1]], near[: starts[-1]])
+
+
+@pytest.mark.parametrize("dtype,d,pt", [(BF16, 128, 16), (F32, 64, 32), (BF16, 80, 16)])
+def test_one_workspace_for_all_steps(dtype, d, pt):
+    """A workspace of the largest step and the capacity serves every smaller call, with the bits that its own gives."""
+    rng = np.random.default_rng(d)
+    hq, hkv, most = 16, 4, 6000
+    lens = [3000, 900, 64, 1, 2049]
+    cache, _, _ = bounded(rng, lens, hkv, d, pt, "int8", 8192)
+    q = torch.from_numpy(rng.standard_normal((most, hq, d)).astype(np.float32)).to(dtype).cuda()
+    ws = torch.empty(qk.attention_workspace(cache, most, hq, dtype), dtype=torch.uint8, device="cuda")
+    for own, rows, context in (([1] * 5, 1, None), ([1] * 5, 1, 3000), ([1] * 5, 1, 500), ([1] * 5, 5, None), ([3, 1, 9, 0, 4], 9, None),
+                               ([600, 3, 1, 1, 70], 600, None), ([2500, 800, 1, 1, 2000], 2500, None), ([1, 2, 0, 0, 3], 4096, None)):
+        starts = dev(np.concatenate(([0], np.cumsum(own))), torch.int32)
+        for total in sorted({max(sum(own), rows), most}):
+            more = dict(max_rows=rows, max_context=context)
+            got = qk.quantized_attention(cache, q[:total], starts, workspace=ws, **more)
+            need = qk.attention_workspace(cache, total, hq, dtype, **more)
+            assert need <= ws.numel()
+            want = qk.quantized_attention(cache, q[:total], starts, **more)
+            assert torch.equal(torch.nan_to_num(got[: sum(own)].float(), 7.0), torch.nan_to_num(want[: sum(own)].float(), 7.0))

@@ -559,7 +559,7 @@ int sfg_hip_rope_turns_host_v1(uint64_t* turns, const double* inv_freq, int64_t 
  * INTERLEAVED one.  q [T][Hq][D] and k [T][Hkv][D] have strides of their own between
  * rows (in elements, at least Hq D and Hkv D): parts of a QKV product's rows, say; either may
  * be absent (NULL, 0 heads).  An output may be its input (same pointer and stride), and
- * overlaps nothing else.  Rows of negative positions are left as they were. */
+ * overlaps nothing else (refused; it may lie between other rows).  Rows of negative positions are left as they were. */
 enum sfg_rope_layout { SFG_ROPE_HALF = 0, SFG_ROPE_INTERLEAVED = 1 };
 typedef struct {
     const void* q; const void* k; void* q_out; void* k_out; int32_t dtype;  /* SFG_F32 or SFG_BF16 */
@@ -598,7 +598,7 @@ int sfg_hip_kv8_append_v1(const sfg_kv8_append_args* args, void* stream);
 /* Causal attention of each sequence's newest rows over its cache: with R = starts[b + 1] -
  * starts[b] rows and L = seq_lens[b] tokens (clamped to [0, max_context]; the rows' own
  * tokens included), row i sees token j iff j <= L - R + i.  q and out [T][Hq][D] with row
- * strides in elements, at least Hq D; out overlaps nothing else.  starts NULL: every sequence has
+ * strides in elements, at least Hq D; out and workspace overlap nothing else (refused).  starts NULL: every sequence has
  * max_rows rows, T = batch * max_rows.  max_rows bounds the rows of any sequence: those
  * past it are not computed.  A row that sees nothing comes out NaN (0 / 0); tokens on a
  * page whose id is outside the pool are not seen; what no row sees may hold anything.

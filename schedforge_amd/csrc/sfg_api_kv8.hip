@@ -30,6 +30,32 @@ struct Span {
     }
 };
 
+// `count` rows of `bytes`, `stride` bytes from one to the next (at least `bytes`).
+struct Rows {
+    const void* p;
+    int64_t stride, bytes, count;
+    int64_t at() const { return static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)); }
+    int64_t end() const { return at() + (count - 1) * stride + bytes; }
+    static Rows all(const void* p, int64_t bytes) { return {p, bytes, bytes, 1}; }
+    // n rows from `from` on: does one of them meet [b, b + size)?  The first that ends behind b does, or none.
+    static bool one(int64_t from, int64_t stride, int64_t bytes, int64_t n, int64_t b, int64_t size) {
+        const int64_t ahead = b - bytes - from, i = ahead < 0 ? 0 : ahead / stride + 1;
+        return i < n && from + i * stride < b + size;
+    }
+    bool meets(const Rows& o) const {
+        if (!p || !o.p || at() >= o.end() || o.at() >= end()) return false;
+        if (o.count == 1) return one(at(), stride, bytes, count, o.at(), o.bytes);
+        if (count == 1) return o.meets(*this);
+        // of one stride: row i and row j lie as row i - j and row 0 do
+        if (stride == o.stride) return one(at() - (o.count - 1) * stride, stride, bytes, count + o.count - 1, o.at(), o.bytes);
+        for (int64_t i = 0; i < count; ++i)
+            if (one(o.at(), o.stride, o.bytes, o.count, at() + i * stride, bytes)) return true;
+        return false;
+    }
+};
+// (sizes that no memory has are cut)
+int64_t times(int64_t a, int64_t b) { return a > (int64_t{1} << 56) / b ? int64_t{1} << 56 : a * b; }
+
 // What the attention's checks and its workspace query share; pointers apart.
 bool sized(const sfg_kv8_attn_args& a) {
     return a.batch > 0 && a.q_heads > 0 && a.kv_heads > 0 && a.q_heads % a.kv_heads == 0 && a.head_dim > 0 &&
@@ -130,6 +156,17 @@ int sfg_hip_rope_v1(const sfg_rope_args* a, void* stream) {
             return fail(SFG_ERR_SHAPE, "rope: heads without rows, or rows closer than their heads");
         if (p.in == p.out && p.in_stride != p.out_stride) return fail(SFG_ERR_SHAPE, "rope: in place with two strides");
     }
+    const int64_t size = a->dtype == SFG_F32 ? 4 : 2;
+    auto rows = [&](const void* p, int64_t stride, int64_t heads) { return Rows{p, stride * size, heads * a->head_dim * size, a->tokens}; };
+    for (const auto& w : part) {
+        const Rows out = rows(w.out, w.out_stride, w.heads);
+        for (const auto& r : part)
+            if ((!(&r == &w && r.in == w.out) && out.meets(rows(r.in, r.in_stride, r.heads))) ||
+                (&r > &w && out.meets(rows(r.out, r.out_stride, r.heads))))
+                return fail(SFG_ERR_SHAPE, "rope: an output overlaps other rows");
+        if (out.meets(Rows::all(a->positions, 4 * a->tokens)) || out.meets(Rows::all(a->turns, 8 * (a->rotary_dim / 2))))
+            return fail(SFG_ERR_SHAPE, "rope: an output overlaps positions or turns");
+    }
     sfg::launch_rope(*a, as_stream(stream));
     return check_launch("rope");
 }
@@ -182,6 +219,16 @@ int sfg_hip_attn_kv8_v1(const sfg_kv8_attn_args* a, void* workspace, size_t work
         return fail(SFG_ERR_WORKSPACE, "attn_kv8: workspace off a 16-byte boundary");
     if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes))
         return fail(SFG_ERR_WORKSPACE, "attn_kv8: workspace %zu < %zu", workspace ? workspace_bytes : 0, plan.bytes);
+    const int64_t units = times(a->num_pages, a->kv_heads), pool = times(units, a->page_tokens * a->head_dim);
+    const int64_t q_size = a->q_dtype == SFG_F32 ? 4 : 2, out_size = a->out_dtype == SFG_F32 ? 4 : 2;
+    const Rows q{a->q, a->q_stride * q_size, row * q_size, a->tokens}, out{a->out, a->out_stride * out_size, row * out_size, a->tokens};
+    const Rows scratch = Rows::all(plan.bytes > 0 ? workspace : nullptr, static_cast<int64_t>(plan.bytes));
+    const Rows read[] = {q, Rows::all(a->k_pool, pool), Rows::all(a->v_pool, pool), Rows::all(a->scales, times(units, 8)),
+                         Rows::all(a->page_table, 4 * a->batch * a->pages_per_seq), Rows::all(a->seq_lens, 4 * a->batch),
+                         Rows::all(a->starts, 4 * a->batch + 4)};
+    if (out.meets(scratch)) return fail(SFG_ERR_SHAPE, "attn_kv8: the output and the workspace overlap");
+    for (const Rows& r : read)
+        if (out.meets(r) || scratch.meets(r)) return fail(SFG_ERR_SHAPE, "attn_kv8: the output or the workspace overlaps what is read");
     sfg::launch_attn_kv8(*a, plan, workspace, as_stream(stream));
     return check_launch("attn_kv8");
 }

@@ -17,6 +17,8 @@ Tensors stay on the device and no call waits for it; each runs on `stream`, or t
 and the caller orders calls on different streams.  A `workspace` (uint8, as large as
 attention_workspace says) may be passed to calls that are captured or repeated, else it is
 allocated; calls that overlap need workspaces of their own.
+
+Nothing here computes gradients: rows that require them are refused while autograd records.
 """
 from __future__ import annotations
 
@@ -166,6 +168,11 @@ class RotaryAngles:
         self.turns = torch.from_numpy(turns.view(np.int64)).to(self.device)
 
 
+def _no_gradients(*tensors) -> None:
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        raise ValueError("gradients are not computed: call under torch.no_grad(), or with detached tensors")
+
+
 def _rows(where, t, name: str, dtypes, shape=None) -> int:
     """A row's stride, in elements, of t [T][heads][D], whose heads lie one behind the other."""
     if not isinstance(t, torch.Tensor) or t.dim() != 3 or t.dtype not in dtypes or 0 in t.shape:
@@ -190,6 +197,7 @@ def rotate(angles: RotaryAngles, positions: torch.Tensor, q: Optional[torch.Tens
     by default outputs are allocated.  Returns (q_out, k_out)."""
     if layout not in _LAYOUTS:
         raise ValueError(f"unknown rotary layout {layout}")
+    _no_gradients(q, k, q_out, k_out)
     given = [x for x in (q, k) if x is not None]
     if not given:
         raise ValueError("rotate needs queries or keys")
@@ -284,6 +292,7 @@ def quantized_attention(cache: QuantizedKVCache, query: torch.Tensor, starts: Op
     (default: the capacity).  Both are the bounds that a captured call is built for."""
     if not isinstance(query, torch.Tensor) or query.dim() != 3:
         raise ValueError("query must be a tensor [tokens][q_heads][head_dim]")
+    _no_gradients(query, out)
     tokens, q_heads = int(query.shape[0]), int(query.shape[1])
     q_stride = _rows(cache, query, "query", tuple(_DTYPES), (tokens, q_heads, cache.config.head_dim))
     a = _attention(cache, tokens, q_heads, starts, max_rows, max_context, kv_splits, scale)

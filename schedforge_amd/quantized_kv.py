@@ -273,11 +273,14 @@ def _attention(cache: QuantizedKVCache, tokens: int, q_heads: int, starts, max_r
 
 
 def attention_workspace(cache: QuantizedKVCache, tokens: int, q_heads: int, dtype: torch.dtype, starts=True,
-                        max_rows: Optional[int] = None, max_context: Optional[int] = None, kv_splits: int = 0) -> int:
+                        max_rows: Optional[int] = None, max_context: Optional[int] = None, kv_splits: int = 0,
+                        out_dtype: Optional[torch.dtype] = None) -> int:
     """Bytes of workspace for quantized_attention with queries of these sizes, or of no larger tokens, max_rows and
-    max_context."""
+    max_context.  dtype: the queries'; out_dtype: the output's (default: the same)."""
+    if dtype not in _DTYPES or (out_dtype is not None and out_dtype not in _DTYPES):
+        raise ValueError(f"queries and outputs must be of {' or '.join(str(d) for d in _DTYPES)}")
     a = _attention(cache, tokens, q_heads, starts, max_rows, max_context, kv_splits, 0.0)
-    a.q_dtype = a.out_dtype = _DTYPES[dtype]
+    a.q_dtype, a.out_dtype = _DTYPES[dtype], _DTYPES[dtype if out_dtype is None else out_dtype]
     return cache.lib.sfg_hip_attn_kv8_workspace_v1(ctypes.byref(a))
 
 

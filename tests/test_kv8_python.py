@@ -34,3 +34,19 @@ def test_gradients_that_nobody_asks_for():
             with torch.set_grad_enabled(grad), pytest.raises(Exception) as e:
                 call(x)                                               # (a device of the host cannot run it)
             assert "gradient" not in str(e.value)
+
+
+def test_workspace_of_another_output_type():
+    """bf16 queries with an fp32 output run on other kernels, whose workspace is larger at some sizes."""
+    c = cache(2, 128)
+    same, other = (qk.attention_workspace(c, 64, 16, BF16, max_rows=16, out_dtype=t) for t in (BF16, F32))
+    assert qk.attention_workspace(c, 64, 16, BF16, max_rows=16) == same != other
+    assert qk.attention_workspace(c, 64, 16, F32, max_rows=16) == other == qk.attention_workspace(c, 64, 16, F32, max_rows=16, out_dtype=BF16)
+
+
+def test_workspace_refusals():
+    c = cache()
+    for more in (dict(dtype=torch.float16), dict(dtype="bf16"), dict(dtype=BF16, out_dtype=torch.int8), dict(dtype=BF16, starts=None, tokens=7),
+                 dict(dtype=BF16, q_heads=3)):
+        with pytest.raises(ValueError):
+            qk.attention_workspace(c, **{"tokens": 8, "q_heads": 4, **more})

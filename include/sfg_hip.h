@@ -492,7 +492,10 @@ int sfg_hip_attn_sparse_v1(const sfg_paged_attn_args* args, const void* bounds, 
  *     lengths and counts;
  *   - device-side indices are clamped or skipped, never followed out of range;
  *   - rows behind the last sequence (padding to a captured size) carry position and
- *     slot -1 and are left as they were.
+ *     slot -1 and are left as they were;
+ *   - fewer than 2^22 rows and 2^16 heads, and in attention fewer than 2^22 rows times query
+ *     heads; up to 2^20 sequences, fewer than 2^30 positions, head_dim up to 256 (rotary
+ *     positions 1024).  What is larger is refused (SFG_ERR_UNSUPPORTED).
  *
  * The cache: K pool [page][Hkv][page_tokens][D] and V pool [page][Hkv][D][page_tokens] of
  * one-byte codes, SFG_I8 (-127 .. 127) or SFG_FP8 (e4m3: 4 exponent and 3 mantissa bits,
@@ -550,7 +553,8 @@ int sfg_hip_rope_inv_freq_host_v1(double* inv_freq, float* magnitude, int64_t ro
                                   const sfg_rope_scaling* scaling);
 /* The same angles as turns per position in 64-bit fixed point, round(inv_freq 2^64 / (2 pi))
  * modulo 2^64: a position times it wraps as whole turns do, so that the angle of any
- * position is known to 2^-33 turns. */
+ * position is known to 2^-33 turns before it is rounded to fp32 (to 2^-25 near half a turn)
+ * for its cosine and sine. */
 int sfg_hip_rope_turns_host_v1(uint64_t* turns, const double* inv_freq, int64_t pairs);
 
 /* Rotary positions.  Of each head of row t the first rotary_dim values are pairs that are
@@ -602,11 +606,12 @@ int sfg_hip_kv8_append_v1(const sfg_kv8_append_args* args, void* stream);
  * max_rows rows, T = batch * max_rows.  max_rows bounds the rows of any sequence: those
  * past it are not computed.  A row that sees nothing comes out NaN (0 / 0); tokens on a
  * page whose id is outside the pool are not seen; what no row sees may hold anything.
- * kv_splits <= 0 picks how far sequences are split, scale <= 0 means 1 / sqrt(D).  Scores,
+ * kv_splits <= 0 picks how far sequences are split (not at all where the bounds would have more
+ * than 128 MiB of partial results: from about 4000 rows of 32 + 8 heads of 128), scale <= 0 means 1 / sqrt(D).  Scores,
  * softmax and sums are fp32; with bf16 queries and a bf16 output the softmax weights times
  * V's scale enter the product with 16 bits, else with 24.  head_dim up to 256, any group
  * Hq / Hkv, any page size; head_dim 64 and 128 over pages of whole 16 tokens run on the
- * matrix cores.  The same call gives the same bits (no atomics).  The workspace query answers
+ * matrix cores (pools on 16-byte boundaries, up to 2^21 sequences times kv heads).  The same call gives the same bits (no atomics).  The workspace query answers
  * for these bounds and all shorter ones: the bytes serve every call with the same other
  * sizes and no larger tokens, max_rows and max_context. */
 typedef struct {

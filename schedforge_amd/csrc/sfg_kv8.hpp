@@ -47,7 +47,9 @@ void launch_kv8_append(const sfg_kv8_append_args& a, hipStream_t stream);
 // share and the units together.  quads (0: never): with so many tiles of all heads, a workgroup
 // takes four heads, and there are four times as many shares.  fixed: pieces a unit, instead of
 // all that.  row_shift: a block has 2^row_shift whole rows (-1: it has not).  slots: partial
-// results a kv head, at most; groups: workgroups.  bytes: 0 if no unit is split.
+// results a kv head, at most; groups: workgroups.  bytes: 0 if no unit is split.  Units run whole (fixed
+// 1, share 0) where the bounds' partial results pass 128 MiB or their costs the 32-bit sums: two sequences of
+// 131072 tokens take 70 us under a bound of one row, 1377 under one of 8192.
 struct Kv8Plan {
     bool mfma;
     int nt, waves, width, slots, groups, share, quads, fixed, least, few, row_shift;

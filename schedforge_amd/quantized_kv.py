@@ -292,7 +292,8 @@ def quantized_attention(cache: QuantizedKVCache, query: torch.Tensor, starts: Op
     cache) over its cached tokens: of a sequence's R rows and L tokens row i sees token j iff j <= L - R + i; a row that
     sees nothing is NaN.  starts: int32 [B + 1] (StepPlan.starts), None: as many rows for every sequence.  max_rows: the
     most rows of any sequence (default: all T; rows past it are not computed); max_context: no sequence is longer
-    (default: the capacity).  Both are the bounds that a captured call is built for."""
+    (default: the capacity).  Both are the bounds that a captured call is built for: with a max_rows of thousands
+    sequences are not split, so a decode step is better captured with its own.  T * Hq stays below 2^22."""
     if not isinstance(query, torch.Tensor) or query.dim() != 3:
         raise ValueError("query must be a tensor [tokens][q_heads][head_dim]")
     _no_gradients(query, out)

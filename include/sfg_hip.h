@@ -537,7 +537,7 @@ int sfg_hip_kv_plan_v1(const sfg_kv_plan_args* args, void* stream);
  * factor on cosine and sine, computed on the host in 64 bits.  With w_i = theta^(-2 i / R), R
  * the rotary dim, s the factor and r_i = context w_i / (2 pi) the turns over the context that
  * the weights were trained on:
- *   PLAIN   w_i;  LINEAR  w_i / s;  BASE  theta becomes theta s^(R / (R - 2));
+ *   PLAIN   w_i;  LINEAR  w_i / s;  BASE  theta becomes theta s^(R / (R - 2)) (R > 2);
  *   BANDS   w_i (t + (1 - t) / s), t = (r_i - low) / (high - low) in [0, 1];
  *   RAMP    w_i (1 - t + t / s), t = (i - a) / max(b - a, 0.001) in [0, 1], a the floor (at
  *           least 0) of d(high) and b the ceiling (at most R - 1) of d(low), d(x) =
